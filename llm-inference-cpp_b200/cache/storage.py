@@ -9,6 +9,9 @@ A mixer says what it needs per sequence with a *request*:
   reference's layout, include/llmi/model/transformer.hpp:39-44).  Values may have a
   head count and a head size of their own (``v_heads``, ``v_dim``): the V tensor is then
   ``[calls, pages, v_heads, page_size, v_dim]`` over the same pages.
+  With ``held`` ("int8", "float8_e4m3") keys and values are held in 8 bits: each row of a head is ``head_dim`` codes
+  and one fp32 scale (:class:`Rows8`; ``csrc/rows8.cuh`` says how a row is made), so that a group has
+  ``[calls, pages, kv_heads, page_size]`` scales beside its codes.
 * :class:`StateRequest` — a fixed-size state per sequence, ``[calls, slots, *shape]``,
   zeroed when a slot is handed out.  The Llama architecture asks for none; the slab is
   here so that a mixer with a recurrent state needs no change of the cache.
@@ -19,11 +22,29 @@ from __future__ import annotations
 
 import itertools
 from dataclasses import dataclass, field
+from typing import NamedTuple
 
 import numpy as np
 import torch
 
 from .pages import PAGE_SIZE, CacheError, PagePool, SlotTable, pages_for
+
+
+HELD_TYPES = {"int8": torch.int8, "float8_e4m3": torch.float8_e4m3fn}
+
+
+def held_type(name: str) -> str:
+    """The name of an 8-bit type that a cache can hold its keys and values in, checked."""
+    if name not in HELD_TYPES:
+        raise CacheError(f"cache: keys and values are held in the compute type, int8 or float8_e4m3, not {name!r}")
+    return name
+
+
+class Rows8(NamedTuple):
+    """Keys or values of one call held in 8 bits: ``codes`` int8 or float8_e4m3fn [pages, heads, 64, dim] and ``scales`` fp32
+    [pages, heads, 64]; a row stands for codes * scale."""
+    codes: torch.Tensor
+    scales: torch.Tensor
 
 
 @dataclass(frozen=True)
@@ -35,6 +56,7 @@ class KVRequest:
     v_heads: int = 0         # value heads and their size, where they differ from the keys' (0: as the keys)
     v_dim: int = 0
     every: int = 1           # > 1: one row per block of that many positions (row b once the block's last position is there)
+    held: str = ""           # the 8-bit type that keys and values are held in ("": the compute type)
 
 
 @dataclass(frozen=True)
@@ -66,15 +88,24 @@ class KVGroup:
             n_pages = min(n_pages, -(-n_pages // self.every) + max(1, n_slots if n_slots > 0 else n_pages))
         self.pool = PagePool(n_pages, page_size, request.window, n_slots, max_pages_per_slot, self.every)
         shape = (n_calls, n_pages, request.n_kv_heads, page_size, request.head_dim)
+        if request.held:
+            dtype = HELD_TYPES[held_type(request.held)]
         self.k = torch.zeros(shape, dtype=dtype, device=device)
         self.v_heads, self.v_dim = request.v_heads or request.n_kv_heads, request.v_dim or request.head_dim
         v_shape = (n_calls, n_pages, self.v_heads, page_size, self.v_dim)
         self.v = torch.zeros(v_shape, dtype=dtype, device=device) if request.values else None
+        self.k_scale = torch.zeros(shape[:-1], dtype=torch.float32, device=device) if request.held else None
+        self.v_scale = torch.zeros(v_shape[:-1], dtype=torch.float32, device=device) if request.held and request.values else None
+
+    def rows8(self, call: int) -> tuple:
+        """Keys and values of one call of a group held in 8 bits: (Rows8, Rows8)."""
+        return Rows8(self.k[call], self.k_scale[call]), Rows8(self.v[call], self.v_scale[call])
 
     def bytes_per_token(self) -> int:
         r = self.request
         per = r.n_kv_heads * r.head_dim + (self.v_heads * self.v_dim if r.values else 0)
-        return self.n_calls * per * self.k.element_size() // self.every
+        scales = 4 * (r.n_kv_heads + (self.v_heads if r.values else 0)) if r.held else 0
+        return self.n_calls * (per * self.k.element_size() + scales) // self.every
 
 
 class StateGroup:

@@ -5,7 +5,7 @@ Option names and meanings are the reference's where it has them
 
     llmi-generate MODEL_DIR --ids N,N,... [--max-new N] [--ignore-eos] [--json] [--dump FILE]
                   [--kv-cache] [--temperature T] [--top-k N] [--top-p P] [--seed N]
-                  [--dtype bf16|fp32] [--ids-file FILE] [--max-batch N]
+                  [--dtype bf16|fp32] [--kv-type int8|float8_e4m3] [--ids-file FILE] [--max-batch N]
     llmi-generate --random CONFIG.json [--seed-weights S] --ids ...
 
 ``--max-new`` defaults to 32; generation is greedy unless ``--temperature`` is given; stop
@@ -14,6 +14,7 @@ tokens are the configuration's ``eos_token_id`` unless ``--ignore-eos``.  ``--js
 (main.cpp:339-344).  ``--dump FILE`` writes one whole-prompt pass as the reference does
 (main.cpp:85-97): a JSON header line, then fp32 little-endian states and all-position logits.
 ``--kv-cache`` is accepted and changes nothing: this engine always runs from its cache.
+``--kv-type`` holds the cache's keys and values in 8 bits (default: the compute type).
 ``--ids-file`` holds one comma-separated prompt per line; the prompts run as batches.
 Text prompts need a tokenizer, which this library does not have: ``--prompt`` is refused.
 Exit codes: 2 for a usage error, 1 for a runtime error (main.cpp:206-211, 268-276).
@@ -26,7 +27,7 @@ import time
 
 USAGE = ("usage: llmi-generate (MODEL_DIR | --random CONFIG.json [--seed-weights S]) (--ids N,N,... | --ids-file FILE) "
          "[--max-new N] [--ignore-eos] [--json] [--dump FILE] [--kv-cache] [--temperature T] [--top-k N] [--top-p P] "
-         "[--seed N] [--dtype bf16|fp32] [--max-batch N]\n")
+         "[--seed N] [--dtype bf16|fp32] [--kv-type int8|float8_e4m3] [--max-batch N]\n")
 
 
 def parse_ids(s: str):
@@ -48,13 +49,13 @@ def parse_args(argv):
         raise UsageError(USAGE.rstrip())
     opts = {"dir": None, "random": None, "seed_weights": 0, "ids": [], "max_new": 32, "ignore_eos": False, "json": False,
             "dump": None, "temperature": 0.0, "top_k": 0, "top_p": 1.0, "seed": 0, "dtype": "bf16", "max_batch": 64,
-            "prompt": None}
+            "prompt": None, "kv_type": None}
     i = 0
     if not argv[0].startswith("--"):
         opts["dir"] = argv[0]
         i = 1
     valued = {"--ids", "--ids-file", "--max-new", "--dump", "--temperature", "--top-k", "--top-p", "--seed", "--dtype",
-              "--random", "--seed-weights", "--max-batch", "--prompt", "--quant"}
+              "--random", "--seed-weights", "--max-batch", "--prompt", "--quant", "--kv-type"}
     while i < len(argv):
         a = argv[i]
         if a in valued and i + 1 < len(argv):
@@ -94,6 +95,10 @@ def parse_args(argv):
                     opts["seed_weights"] = int(v)
                 elif a == "--max-batch":
                     opts["max_batch"] = int(v)
+                elif a == "--kv-type":
+                    if v not in ("int8", "float8_e4m3"):
+                        raise UsageError("error: --kv-type takes int8 or float8_e4m3")
+                    opts["kv_type"] = v
                 elif a == "--prompt":
                     opts["prompt"] = v
                 elif a == "--quant":
@@ -155,7 +160,7 @@ def run(argv) -> int:
     try:
         if o["dump"]:
             ids = o["ids"][0]
-            cache = model.new_cache(max(64, (len(ids) + 63) // 64 * 64))
+            cache = model.new_cache(max(64, (len(ids) + 63) // 64 * 64), kv_type=o["kv_type"])
             slot = cache.alloc_slot()
             states = []
             logits = model.step(cache, [SequenceStep(slot, ids, list(range(len(ids))))], trace=states).cpu().numpy()
@@ -166,7 +171,7 @@ def run(argv) -> int:
         t1 = time.perf_counter()
         sampling = SamplingParams(o["temperature"], o["top_k"], o["top_p"], o["seed"])
         outs = generate(model, o["ids"], max_new=o["max_new"], ignore_eos=o["ignore_eos"], sampling=sampling,
-                        max_batch=o["max_batch"])
+                        max_batch=o["max_batch"], kv_type=o["kv_type"])
         gen_s = time.perf_counter() - t1
     except Exception as e:
         sys.stderr.write(f"error: {e}\n")

@@ -118,12 +118,13 @@ class ModelBackend:
 
 def generate(model, prompts, max_new=32, stop_ids=None, ignore_eos: bool = False,
              sampling: SamplingParams | None = None, max_batch: int = 64, cache=None, max_tokens: int | None = None,
-             use_graphs: bool = True, return_details: bool = False):
+             use_graphs: bool = True, return_details: bool = False, kv_type: str | None = None):
     """Generate for a list of prompts (lists of token ids).  Returns one list of new ids per prompt.
 
     ``max_new`` is one number or one per prompt.  ``stop_ids=None`` takes the configuration's end
     tokens; ``ignore_eos`` empties them.  ``cache`` reuses a cache of this model; otherwise one is
-    made for ``max_tokens`` (default: what the largest batch needs).
+    made for ``max_tokens`` (default: what the largest batch needs), with keys and values held in ``kv_type``
+    ("int8", "float8_e4m3"; default: the compute type).
     """
     sampling = sampling or SamplingParams()
     per = list(max_new) if isinstance(max_new, (list, tuple)) else [int(max_new)] * len(prompts)
@@ -138,11 +139,13 @@ def generate(model, prompts, max_new=32, stop_ids=None, ignore_eos: bool = False
     elif ignore_eos:
         stop_ids = ()
     page = PAGE_SIZE
+    if cache is not None and kv_type is not None:
+        raise ValueError("generate: kv_type is for the cache made here; a cache that is given has its own")
     if cache is None:
         if max_tokens is None:
             needs = sorted((pages_for(len(r.prompt) + max(r.max_new - 1, 0), page) * page for r in requests), reverse=True)
             max_tokens = max(page, sum(needs[:max_batch]))
-        cache = model.new_cache(max_tokens)
+        cache = model.new_cache(max_tokens, kv_type=kv_type)
     else:
         max_tokens = cache.kv_groups[0].pool.n_pages * cache.page_size if cache.kv_groups else 1 << 30
     batches = plan_batches(requests, max_batch, max_tokens, page)

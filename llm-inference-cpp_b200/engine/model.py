@@ -9,9 +9,12 @@ sequences with unequal lengths in one call.
 """
 from __future__ import annotations
 
+from dataclasses import replace
+
 import torch
 
-from ..cache.storage import CacheBinding, KVRequest, SequenceCache, StateRequest
+from ..cache.pages import CacheError
+from ..cache.storage import CacheBinding, KVRequest, SequenceCache, StateRequest, held_type
 from ..parts.build import build_entries, build_exits, build_parts, expected_tensors
 from ..parts.spec import ModelSpec
 from .batch import SequenceStep, StepBuffers, plan_step
@@ -72,13 +75,21 @@ class Model:
         return total
 
     # -- cache -----------------------------------------------------------------------------
-    def new_cache(self, max_tokens: int, n_slots: int | None = None) -> SequenceCache:
+    def new_cache(self, max_tokens: int, n_slots: int | None = None, kv_type: str | None = None) -> SequenceCache:
         """A cache for at most ``max_tokens`` live tokens (each sequence rounded up to whole pages).
 
         Scheduled calls with equal cache requests share a group; a call that reads another
         call's cache gets that call's place in the group and writes nothing.
+
+        ``kv_type`` ("int8" or "float8_e4m3"; default: the compute type) holds keys and values in 8 bits with an fp32
+        scale per position and kv head: about half the bytes of a bf16 cache, to keep and to read.  Every mixer that keeps
+        keys and values must be one that reads such a cache (``holds_8bit``).
         """
-        requests = [self.layers[c.layer].mixer.cache_request() for c in self.spec.schedule]
+        if kv_type is not None:
+            held_type(kv_type)
+        requests = [self._mixer_request(c.layer, kv_type) for c in self.spec.schedule]
+        if kv_type is not None and not any(isinstance(r, KVRequest) for r in requests):
+            raise CacheError(f"cache: no mixer of this model keeps keys and values (kv_type {kv_type!r})")
         kv_groups: dict = {}
         state_groups: dict = {}
 
@@ -135,6 +146,16 @@ class Model:
                                     (mixer, binding))
         cache.planners = list(planners.values())
         return cache
+
+    def _mixer_request(self, layer: int, kv_type: str | None):
+        mixer = self.layers[layer].mixer
+        request = mixer.cache_request()
+        if kv_type is None or not isinstance(request, KVRequest):
+            return request
+        if not getattr(mixer, "holds_8bit", False):
+            raise CacheError(f"cache: the mixer {getattr(mixer, 'kind', type(mixer).__name__)!r} of layer {layer} does not read a cache "
+                             f"held in 8 bits (kv_type {kv_type!r})")
+        return replace(request, held=kv_type)
 
     def step_plan_token(self, ctx, cache) -> tuple:
         """What a recorded step depends on beside its padded shape: the mixers' own plans for this step (a decode

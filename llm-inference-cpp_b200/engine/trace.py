@@ -23,12 +23,12 @@ SPARE_PAGES = 64     # every live request may leave most of its last page unused
 
 
 class TraceReplayer:
-    def __init__(self, model, max_tokens: int, spare_pages: int = SPARE_PAGES):
+    def __init__(self, model, max_tokens: int, spare_pages: int = SPARE_PAGES, kv_type: str | None = None):
         """``max_tokens``: the most tokens live requests hold at once, padding not counted; the cache is sized for them
-        in whole pages plus ``spare_pages`` pages for the requests' partly filled last pages."""
+        in whole pages plus ``spare_pages`` pages for the requests' partly filled last pages.  ``kv_type``: see ``Model.new_cache``."""
         self.model = model
         pages = (max(max_tokens, 1) + PAGE_SIZE - 1) // PAGE_SIZE + max(spare_pages, 0)
-        self.cache = model.new_cache(pages * PAGE_SIZE)
+        self.cache = model.new_cache(pages * PAGE_SIZE, kv_type=kv_type)
         self.slots: dict[str, int] = {}
 
     def run_step(self, step: dict):
@@ -61,11 +61,12 @@ def main(argv=None) -> int:
     ap.add_argument("--max-tokens", type=int, required=True,
                     help=f"most tokens live requests hold at once, padding not counted (the cache keeps {SPARE_PAGES} pages "
                          f"of {PAGE_SIZE} beyond that for partly filled last pages)")
+    ap.add_argument("--kv-type", choices=["int8", "float8_e4m3"], help="hold keys and values in 8 bits")
     ap.add_argument("--device", default="cuda:0")
     args = ap.parse_args(argv)
     os.makedirs(args.out, exist_ok=True)
     model = load_model(args.model, args.dtype, args.device)
-    replayer = TraceReplayer(model, args.max_tokens)
+    replayer = TraceReplayer(model, args.max_tokens, kv_type=args.kv_type)
     for line in sys.stdin:
         line = line.strip()
         if not line:

@@ -14,6 +14,7 @@ from ctypes import c_double, c_float, c_int, c_long, c_void_p
 
 import torch
 
+from ..cache.storage import Rows8
 from . import library
 
 OUT_STORE = 0        # y (compute type) = x·Wᵀ
@@ -168,7 +169,8 @@ def lib():
                      "llmi_moe_identity_add", "llmi_channel_decay", "llmi_rows_activate", "llmi_decay_recurrence",
                      "llmi_normed_pair", "llmi_stream_axpy_norm", "llmi_stream_postnorm", "llmi_softcap_rows", "llmi_moe_table",
                      "llmi_qkv_unit_prepare", "llmi_latent_prepare_direct", "llmi_channel_token_supported",
-                     "llmi_channel_token_prepare", "llmi_channel_token_step", "llmi_cast_rows", "llmi_heads_token", "llmi_heads_token_supported"):
+                     "llmi_channel_token_prepare", "llmi_channel_token_step", "llmi_cast_rows", "llmi_heads_token", "llmi_heads_token_supported",
+                     "llmi_rope_store8", "llmi_attention_any8"):
             getattr(l, name).restype = c_int
         l.llmi_gemm_tc_workspace.restype = c_long
         l.llmi_delta_state_floats.restype = c_long
@@ -183,6 +185,8 @@ def lib():
         l.llmi_rmsnorm.argtypes = [I, P, P, P, P, I, I, F, P]
         l.llmi_rope_store.argtypes = [I, P, L, P, I, P, P, P, I, I, P, P, I, I, I, I, I, P]
         l.llmi_attention_prefill_tc.argtypes = [P, L, L, P, L, P, P, L, P, I, P, P, I, I, I, I, I, F, I, I, I, P, L, P, I, P, I, P, P, L, P, I, P, L, P, P, P, I, I, I, P, P]
+        l.llmi_rope_store8.argtypes = [I, I, P, L, P, L, P, I, P, P, P, I, I, I, P, P, P, P, I, I, I, I, I, I, P]
+        l.llmi_attention_any8.argtypes = [I, I, P, L, P, L, P, P, P, P, P, P, P, I, I, I, I, I, I, I, I, F, I, P]
         _configured = True
     return l
 
@@ -2115,3 +2119,109 @@ def softcap_rows(v: torch.Tensor, cap: float) -> None:
     _need_cuda(v)
     assert v.dtype == torch.float32 and v.is_contiguous() and cap > 0
     _check("softcap_rows", lib().llmi_softcap_rows(_ptr(v), c_long(v.numel()), c_float(cap), _stream()))
+
+
+# -- keys and values held in 8 bits ---------------------------------------------------------------------------------------------
+
+_HELD_CODE = {torch.int8: 0, torch.float8_e4m3fn: 1}
+
+
+def _refuse(name: str, wrong: bool, why: str) -> None:
+    if wrong:
+        raise KernelError(f"{name}: {why}")
+
+
+def _check8(name: str, x: torch.Tensor, k: Rows8, v: Rows8, seq_pages, n_heads: int, n_kv_heads: int, head_dim: int, more=()) -> int:
+    """The checks that the 8-bit kernels share; the code of the type that the rows are held in."""
+    if not (x.is_cuda and all(t.is_cuda for t in (*k, *v, seq_pages, *more))):
+        raise KernelError(f"{name}: kernels take CUDA tensors only (there is no CPU path)")
+    device = x.get_device()
+    _refuse(name, device != torch.cuda.current_device() or any(t.get_device() != device for t in (*k, *v, seq_pages, *more)),
+            "all tensors must lie on the current device")
+    _refuse(name, x.dtype not in (torch.bfloat16, torch.float32), f"unsupported element type {x.dtype}")
+    _refuse(name, k.codes.dtype not in _HELD_CODE or v.codes.dtype != k.codes.dtype, "keys and values are held in int8 or float8_e4m3fn, both in one of them")
+    _refuse(name, n_heads < 1 or n_kv_heads < 1 or n_heads % n_kv_heads != 0, "n_heads must be a multiple of n_kv_heads")
+    _refuse(name, not 1 <= head_dim <= 256, "head_dim must be 1 to 256")
+    shape = k.codes.shape
+    _refuse(name, tuple(shape[1:]) != (n_kv_heads, 64, head_dim) or shape[0] < 1 or v.codes.shape != shape, "codes must be [pages, n_kv_heads, 64, head_dim]")
+    for s in (k.scales, v.scales):
+        _refuse(name, s.dtype != torch.float32 or s.shape != shape[:-1], "scales must be fp32 [pages, n_kv_heads, 64]")
+    _refuse(name, not all(t.is_contiguous() for t in (*k, *v)), "codes and scales must be contiguous")
+    _refuse(name, seq_pages.dtype != torch.int32 or seq_pages.dim() != 2 or (seq_pages.shape[1] > 1 and seq_pages.stride(1) != 1),
+            "the page table must be int32 [sequences, pages]")
+    return _HELD_CODE[k.codes.dtype]
+
+
+def _check_index(name: str, what: str, t: torch.Tensor, n: int) -> None:
+    _refuse(name, t.dtype != torch.int32 or t.dim() != 1 or t.shape[0] < n or (n > 1 and t.stride(0) != 1), f"{what} must be int32 [{n}]")
+
+
+def rope_store8(qkv: torch.Tensor, q_out: torch.Tensor, inv_freq: torch.Tensor | None, rotary_dim: int, tok_seq, tok_pos, seq_pages,
+                k: Rows8, v: Rows8, n_heads: int, n_kv_heads: int, head_dim: int, write_kv: bool = True) -> None:
+    """Rotate q and k of each token's row [q | k | v] and append k, v to its sequence's pages, held in 8 bits.
+
+    The rotated q goes to ``q_out`` [T, n_heads * head_dim] (rows may be strided; ``qkv[:, :n_heads * head_dim]`` rotates in
+    place).  ``tok_seq`` -1 marks a token of no sequence: nothing of it is written.  Two tokens of a call must not have the same
+    place.  ``write_kv`` False: q only.  How a row is held: ``csrc/rows8.cuh``."""
+    name = "rope_store8"
+    held = _check8(name, qkv, k, v, seq_pages, n_heads, n_kv_heads, head_dim, (q_out, tok_seq, tok_pos))
+    T = qkv.shape[0]
+    _refuse(name, qkv.dim() != 2 or qkv.shape[1] != (n_heads + 2 * n_kv_heads) * head_dim or qkv.stride(1) != 1, "qkv must be [tokens, (n_heads + 2 n_kv_heads) * head_dim]")
+    _refuse(name, q_out.shape != (T, n_heads * head_dim) or q_out.dtype != qkv.dtype or q_out.stride(1) != 1, "q_out must be [tokens, n_heads * head_dim] of qkv's type")
+    _refuse(name, rotary_dim < 0 or rotary_dim % 2 != 0 or rotary_dim > head_dim, "rotary_dim must be even and at most head_dim")
+    if rotary_dim:
+        _refuse(name, inv_freq is None or not inv_freq.is_cuda or inv_freq.get_device() != qkv.get_device() or inv_freq.dtype != torch.float32
+                or inv_freq.numel() < rotary_dim // 2 or not inv_freq.is_contiguous(), "inv_freq must be fp32 with rotary_dim / 2 entries on the same device")
+    _check_index(name, "tok_seq", tok_seq, T)
+    _check_index(name, "tok_pos", tok_pos, T)
+    if T == 0 or seq_pages.numel() == 0:
+        return
+    _check(name, lib().llmi_rope_store8(
+        _dtype_code(qkv), held, qkv.data_ptr(), qkv.stride(0), q_out.data_ptr(), q_out.stride(0), _addr(inv_freq) if rotary_dim else None, rotary_dim,
+        tok_seq.data_ptr(), tok_pos.data_ptr(), seq_pages.data_ptr(), seq_pages.stride(0), seq_pages.shape[1], seq_pages.shape[0],
+        k.codes.data_ptr(), k.scales.data_ptr(), v.codes.data_ptr(), v.scales.data_ptr(), k.codes.shape[0], T, n_heads, n_kv_heads, head_dim,
+        1 if write_kv else 0, _stream8(qkv)))
+
+
+def _stream8(t: torch.Tensor) -> int:
+    """The current stream of the tensor's device."""
+    return torch.cuda.current_stream(t.device).cuda_stream if _raw_stream is None else _raw_stream(t.get_device())
+
+
+def attention_any8(q: torch.Tensor, out: torch.Tensor, k: Rows8, v: Rows8, tok_seq, tok_pos, seq_pages, n_heads: int, n_kv_heads: int,
+                   head_dim: int, scale: float, window: int = 0) -> None:
+    """:func:`attention8` by the kernel that takes any sizes."""
+    name = "attention_any8"
+    held = _check8(name, q, k, v, seq_pages, n_heads, n_kv_heads, head_dim, (out, tok_seq, tok_pos))
+    T = out.shape[0]
+    _check_index(name, "tok_seq", tok_seq, T)
+    _check_index(name, "tok_pos", tok_pos, T)
+    _check(name, lib().llmi_attention_any8(
+        _dtype_code(q), held, q.data_ptr(), q.stride(0), out.data_ptr(), out.stride(0), k.codes.data_ptr(), k.scales.data_ptr(), v.codes.data_ptr(),
+        v.scales.data_ptr(), tok_seq.data_ptr(), tok_pos.data_ptr(), seq_pages.data_ptr(), seq_pages.stride(0), seq_pages.shape[1],
+        seq_pages.shape[0], k.codes.shape[0], T, n_heads, n_kv_heads, head_dim, scale, window, _stream8(q)))
+
+
+def attention8(q: torch.Tensor, out: torch.Tensor, k: Rows8, v: Rows8, ctx, seq_pages, n_heads: int, n_kv_heads: int, head_dim: int,
+               scale: float, window: int = 0, rt=None, rope=None) -> None:
+    """Causal attention of a step's tokens over a cache that holds keys and values in 8 bits: :func:`attention`'s counterpart.
+
+    ``q`` [T, >= n_heads * head_dim], rotated; its first n_heads * head_dim columns count.  With ``rope=(inv_freq, rotary_dim,
+    write_kv)`` it holds the rows [q | k | v] before their rotation instead: q and k are rotated and k, v appended first
+    (:func:`rope_store8`); the rows themselves stay as they are.  ``out`` [T, n_heads * head_dim] of q's type; rows of no
+    sequence are left as they are.  ``ctx`` says which tokens those are (the fields of a ``StepContext``: ``tok_seq``,
+    ``tok_pos``, ``seq_q_start``, ``seq_kv_len``, ``max_q_len``).  ``rt``: scratch is taken from it where it is given."""
+    name = "attention8"
+    _check8(name, q, k, v, seq_pages, n_heads, n_kv_heads, head_dim, (out, ctx.tok_seq, ctx.tok_pos, ctx.seq_q_start, ctx.seq_kv_len))
+    T, width = out.shape[0], n_heads * head_dim
+    _refuse(name, out.dim() != 2 or out.shape[1] != width or out.dtype != q.dtype or out.stride(1) != 1, "out must be [tokens, n_heads * head_dim] of q's type")
+    _refuse(name, q.dim() != 2 or q.shape[0] != T or q.shape[1] < width or q.stride(1) != 1, "q must be [tokens, >= n_heads * head_dim]")
+    _refuse(name, window < 0, "a window has at least one position (0: none)")
+    if T == 0 or seq_pages.numel() == 0:
+        return
+    if rope is not None:
+        inv_freq, rotary_dim, write_kv = rope
+        rotated = rt.scratch("attn_q8", (T, width)) if rt is not None else torch.empty((T, width), dtype=q.dtype, device=q.device)
+        rope_store8(q, rotated, inv_freq, rotary_dim, ctx.tok_seq, ctx.tok_pos, seq_pages, k, v, n_heads, n_kv_heads, head_dim, write_kv)
+        q = rotated
+    attention_any8(q, out, k, v, ctx.tok_seq, ctx.tok_pos, seq_pages, n_heads, n_kv_heads, head_dim, scale, window)

@@ -55,6 +55,11 @@ class GQAttention:
     def cache_request(self):
         return KVRequest(self.n_kv_heads, self.head_dim, self.window)
 
+    @property
+    def holds_8bit(self) -> bool:
+        """Whether the cache may hold keys and values in 8 bits: if all the position part does is the rotation of pairs."""
+        return self.position.fused_rotation() is not None
+
     def weight_bytes(self) -> int:
         return sum(t.numel() * t.element_size() for t in (self.w_qkv, self.w_o))
 
@@ -69,7 +74,7 @@ class GQAttention:
     def step_plan(self, ctx, binding):
         """What of this step's launches depends on more than the step's padded shape (a recorded step is replayed
         only for a step with the same answer): the decode kernel's split and variant."""
-        if not ctx.decode or self.rt.dtype != torch.bfloat16:
+        if not ctx.decode or self.rt.dtype != torch.bfloat16 or binding.group.request.held:
             return None
         g = binding.group
         S, P = ctx.pages_of(g).shape
@@ -87,6 +92,11 @@ class GQAttention:
         g = binding.group
         pages = ctx.pages_of(g)
         fused = self.position.fused_rotation()
+        if g.request.held:
+            k, v = g.rows8(binding.index)
+            kernels.attention8(qkv, attn, k, v, ctx, pages, nh, nkv, hd, self.scale, self.window, rt=self.rt,
+                               rope=(*fused, binding.writes))
+            return kernels.linear(attn, self.w_o, x, None, kernels.OUT_ADD_F32, then_norm)
         if fused is not None and kernels.attention_fuses_rotation(qkv, ctx, pages, g.page_size, nh, nkv, hd, fused[1], self.rt):
             rope = (fused[0], fused[1], binding.writes)        # a decode step: the attention kernel rotates and appends
         else:

@@ -170,7 +170,7 @@ def lib():
                      "llmi_normed_pair", "llmi_stream_axpy_norm", "llmi_stream_postnorm", "llmi_softcap_rows", "llmi_moe_table",
                      "llmi_qkv_unit_prepare", "llmi_latent_prepare_direct", "llmi_channel_token_supported",
                      "llmi_channel_token_prepare", "llmi_channel_token_step", "llmi_cast_rows", "llmi_heads_token", "llmi_heads_token_supported",
-                     "llmi_rope_store8", "llmi_attention_any8"):
+                     "llmi_rope_store8", "llmi_attention_any8", "llmi_attention_rows8", "llmi_attention_rows8_workspace"):
             getattr(l, name).restype = c_int
         l.llmi_gemm_tc_workspace.restype = c_long
         l.llmi_delta_state_floats.restype = c_long
@@ -187,6 +187,7 @@ def lib():
         l.llmi_attention_prefill_tc.argtypes = [P, L, L, P, L, P, P, L, P, I, P, P, I, I, I, I, I, F, I, I, I, P, L, P, I, P, I, P, P, L, P, I, P, L, P, P, P, I, I, I, P, P]
         l.llmi_rope_store8.argtypes = [I, I, P, L, P, L, P, I, P, P, P, I, I, I, P, P, P, P, I, I, I, I, I, I, P]
         l.llmi_attention_any8.argtypes = [I, I, P, L, P, L, P, P, P, P, P, P, P, I, I, I, I, I, I, I, I, F, I, P]
+        l.llmi_attention_rows8.argtypes = [I, P, L, P, L, P, P, P, P, P, P, P, I, I, I, I, I, I, I, I, F, I, P, L, P, L, P]
         _configured = True
     return l
 
@@ -2202,6 +2203,73 @@ def attention_any8(q: torch.Tensor, out: torch.Tensor, k: Rows8, v: Rows8, tok_s
         seq_pages.shape[0], k.codes.shape[0], T, n_heads, n_kv_heads, head_dim, scale, window, _stream8(q)))
 
 
+_sizes8: dict = {}
+_kept8: dict = {}
+
+
+def _rows8_sizes(n_seqs: int, max_q: int, n_heads: int, n_kv_heads: int, head_dim: int, table_pages: int) -> tuple | None:
+    """(floats of scratch, tickets) that attention_rows8 needs, None where it does not take the sizes."""
+    key = (n_seqs, max_q, n_heads, n_kv_heads, head_dim, table_pages)
+    if key not in _sizes8:
+        floats, ints = c_long(0), c_long(0)
+        rc = lib().llmi_attention_rows8_workspace(*map(c_int, key), ctypes.byref(floats), ctypes.byref(ints))
+        if len(_sizes8) >= 4096:
+            _sizes8.clear()
+        _sizes8[key] = (floats.value, ints.value) if rc == 0 else None
+    return _sizes8[key]
+
+
+def _workspace8(q: torch.Tensor, rt, n_floats: int, n_ints: int) -> tuple:
+    """Scratch and zeroed tickets: the model's (``rt``), else kept per device and stream; a call that is captured has its own, since a
+    graph may be replayed beside anything."""
+    if rt is not None:
+        return rt.scratch("attn8_slots", (max(n_floats, 1),), torch.float32), rt.zeroed("attn8_tickets", max(n_ints, 1))
+    capturing = torch.cuda.is_current_stream_capturing()
+    key = (q.get_device(), _stream8(q))
+    kept = None if capturing else _kept8.get(key)
+    if kept is None or kept[0].numel() < n_floats or kept[1].numel() < n_ints:
+        kept = (torch.empty(max(n_floats, 1), dtype=torch.float32, device=q.device), torch.zeros(max(n_ints, 1), dtype=torch.int32, device=q.device))
+        if not capturing:
+            _kept8[key] = kept
+    return kept
+
+
+def _aligned8(q, out, k: Rows8, v: Rows8) -> bool:
+    return ((q.data_ptr() | out.data_ptr() | k.codes.data_ptr() | v.codes.data_ptr() | k.scales.data_ptr() | v.scales.data_ptr()) % 16 == 0
+            and q.stride(0) % 8 == 0 and out.stride(0) % 8 == 0)
+
+
+def attention_rows8(q: torch.Tensor, out: torch.Tensor, k: Rows8, v: Rows8, seq_q_start, seq_kv_len, max_q: int, seq_pages, n_heads: int,
+                    n_kv_heads: int, head_dim: int, scale: float, window: int = 0, rt=None) -> None:
+    """:func:`attention8` by the kernel for few query rows a sequence (bf16, head size 64 or 128): ``seq_q_start`` [sequences + 1],
+    ``seq_kv_len`` [sequences], ``max_q`` the most tokens that a sequence brings."""
+    name = "attention_rows8"
+    held = _check8(name, q, k, v, seq_pages, n_heads, n_kv_heads, head_dim, (out, seq_q_start, seq_kv_len))
+    S, P = seq_pages.shape
+    _refuse(name, q.dtype != torch.bfloat16 or out.dtype != torch.bfloat16, "takes bf16 only")
+    _check_index(name, "seq_q_start", seq_q_start, S + 1)
+    _check_index(name, "seq_kv_len", seq_kv_len, S)
+    sizes = _rows8_sizes(S, max_q, n_heads, n_kv_heads, head_dim, P)
+    _refuse(name, sizes is None, "a size is out of the range this kernel takes")
+    slots, tickets = _workspace8(q, rt, *sizes)
+    _check(name, lib().llmi_attention_rows8(
+        held, q.data_ptr(), q.stride(0), out.data_ptr(), out.stride(0), k.codes.data_ptr(), k.scales.data_ptr(), v.codes.data_ptr(),
+        v.scales.data_ptr(), seq_q_start.data_ptr(), seq_kv_len.data_ptr(), seq_pages.data_ptr(), seq_pages.stride(0), P, S, k.codes.shape[0],
+        max_q, n_heads, n_kv_heads, head_dim, scale, window, slots.data_ptr(), slots.numel(), tickets.data_ptr(), tickets.numel(), _stream8(q)))
+
+
+def _most_new(ctx) -> int:
+    """A bound on the tokens that a sequence of the step brings, the same for every step that a recorded one is replayed for: a
+    prompt step may be padded to a shape, whose recording is told apart by ``short_message`` (the bound itself, or 0)."""
+    if ctx.decode:
+        return 1
+    return decide(ctx, _message_bound) or ctx.n_tokens
+
+
+def _message_bound(ctx) -> int:
+    return int(getattr(ctx, "short_message", 0))
+
+
 def attention8(q: torch.Tensor, out: torch.Tensor, k: Rows8, v: Rows8, ctx, seq_pages, n_heads: int, n_kv_heads: int, head_dim: int,
                scale: float, window: int = 0, rt=None, rope=None) -> None:
     """Causal attention of a step's tokens over a cache that holds keys and values in 8 bits: :func:`attention`'s counterpart.
@@ -2224,4 +2292,9 @@ def attention8(q: torch.Tensor, out: torch.Tensor, k: Rows8, v: Rows8, ctx, seq_
         rotated = rt.scratch("attn_q8", (T, width)) if rt is not None else torch.empty((T, width), dtype=q.dtype, device=q.device)
         rope_store8(q, rotated, inv_freq, rotary_dim, ctx.tok_seq, ctx.tok_pos, seq_pages, k, v, n_heads, n_kv_heads, head_dim, write_kv)
         q = rotated
+    max_q = _most_new(ctx)
+    if (q.dtype == torch.bfloat16 and head_dim in (64, 128) and _aligned8(q, out, k, v)
+            and _rows8_sizes(seq_pages.shape[0], max_q, n_heads, n_kv_heads, head_dim, seq_pages.shape[1]) is not None):
+        attention_rows8(q, out, k, v, ctx.seq_q_start, ctx.seq_kv_len, max_q, seq_pages, n_heads, n_kv_heads, head_dim, scale, window, rt)
+        return
     attention_any8(q, out, k, v, ctx.tok_seq, ctx.tok_pos, seq_pages, n_heads, n_kv_heads, head_dim, scale, window)

@@ -1,8 +1,8 @@
-// Attention of few query rows a sequence — single tokens, short messages — over the paged cache held in 8 bits (rows8.cuh), bf16
-// queries, head size 64 or 128.  For a row at position p of kv head g, over the keys j of its sequence it sees:
+// Attention of few query rows a sequence — single tokens, short messages — over the paged cache held in 8 bits (rows8.cuh), head
+// size 64 or 128.  For a row at position p of kv head g, over the keys j of its sequence it sees:
 //     s_j = scale * k_scale[j] * (q . k_code[j]),   w = softmax(s),   out = sum_j w_j * v_scale[j] * v_code[j]
 // (reference loop: src/model/transformer.cpp:263-282).  Every code is read once and takes part in a handful of operations, so what
-// bounds the kernel is HBM: 2 (D + 4) bytes a position and kv head.
+// bounds the kernel is HBM: 2 (D + 4) bytes a position and kv head; behind that the instructions that make codes fp16 numbers.
 //
 //  * All pages that the step's rows see, kv head by kv head and sequence by sequence, are one line of units (a unit: one page of one
 //    kv head), cut into as many equal ranges as there are blocks resident on the device.  A block works through its range whatever
@@ -10,13 +10,17 @@
 //    A (sequence, kv head) whose units several ranges share is joined by the block that comes last (a ticket per kv head and
 //    sequence), in the order of the ranges: the same call gives the same bits.
 //  * Within a block each warp takes every eighth chunk (2 KB of key codes, 2 KB of value codes, their scales) into a ring of its own
-//    in shared memory with cp.async, across the borders of sequences; warps meet only where a (sequence, kv head) ends.
+//    in shared memory with cp.async, across the borders of sequences; warps meet only where a (sequence, kv head) ends, through the
+//    stages that they have just read.
 //  * The products run on mma.sync (m16n8k16, fp16): a chunk's keys are the 16 rows, the query rows the 8 columns, the G heads of the
 //    group together.  A code is an fp16 number exactly; a query row is divided by a power of two so that its entries are at most 1.
-//    Both scales stay in fp32: k_scale on the scores, v_scale on the weights, before they are rounded to fp16.
+//    Both scales stay in fp32: k_scale on the scores, v_scale on the weights, before they are rounded to fp16.  In the 32-bit path
+//    queries and weights are the sums of two fp16 numbers (22 bits), and a chunk's sum is added to the output's in fp32.
 //  * The weights are kept relative to a maximum M of s_j + log2 v_scale[j] (not of s_j), so that the fp16 number w_j * v_scale[j] is at
 //    most 2^8 and small scales lose nothing.  M moves only when a weight passes 2^8: the common chunk has one vote and no shuffles.
 #include <math.h>
+
+#include <type_traits>
 
 #include "mma_sync.cuh"
 #include "rows8.cuh"
@@ -26,12 +30,13 @@ namespace llmi {
 constexpr int RW8_WARPS = 8;
 constexpr int RW8_MAX_ENTRIES = 4096;      // (sequence, row tile)s of a call
 constexpr float RW8_LAZY = 256.f;          // weights up to this before the reference maximum moves
-constexpr float RW8_TINY = 6.1629758e-33f; // 2^-107: no scale but 0 is smaller
+constexpr float RW8_SUM = 5.192296858534828e33f;   // 2^112: a sum of weights up to this (keys whose values are zeros may weigh that much)
+constexpr float RW8_TINY = 7.888609052210118e-31f; // 2^-100: smaller value scales count as this where M is made
 
 struct Rows8Params {
-  const __nv_bfloat16* q;
+  const void* q;
   long ldq;
-  __nv_bfloat16* out;
+  void* out;
   long ldo;
   const uint8_t* k_codes;
   const float* k_scales;
@@ -47,17 +52,23 @@ struct Rows8Params {
   int* tickets;                 // [n_seqs * row_tiles * n_kv_heads], zero before and after
 };
 
-template <int D, int NT>
+// D: head size; NT: eighths of query rows; T: the type of q and out (float: two fp16 numbers each).
+template <int D, int NT, typename T>
 struct Rw8Cfg {
-  static constexpr int KC = 2048 / D;              // keys of a chunk
+  static constexpr int SP = std::is_same<T, float>::value ? 2 : 1;
+  static constexpr int KC = D == 64 && NT == 1 ? 32 : 16;          // keys of a chunk
   static constexpr int CPP = PAGE8 / KC;           // chunks of a page
   static constexpr int MT = KC / 16, KS = D / 16;  // key tiles of a chunk; 16-dim steps of a row
-  static constexpr int STAGE = 4096 + 8 * KC;
-  static constexpr int STAGES = 3;
-  static constexpr int OREGS = KS * NT * 4, REGS = OREGS + 4 * NT;
-  static constexpr int BLOCKS = REGS <= 44 ? 2 : 1;      // blocks a SM
+  static constexpr int CODES = KC * D;             // bytes of a chunk's key codes, and of its value codes
+  static constexpr int STAGE = 2 * CODES + 8 * KC;
+  static constexpr int PAIRS = KS * NT;            // tiles of 16 dims by 8 rows of an output
+  static constexpr int STATE = (PAIRS * 4 * 32 + 16 * NT) * 4;      // bytes of a state: outputs, then maxima and sums of the rows
+  static constexpr bool IN_RING = STATE <= STAGE;  // a warp's state fits the stage it has just read
+  static constexpr int BLOCKS = (SP == 1 && PAIRS <= 8) ? 2 : 1;    // blocks a SM
+  static constexpr int STAGES = STAGE < 4000 ? (BLOCKS == 2 ? 4 : 6) : (BLOCKS == 2 ? 3 : 4);
   static constexpr int RING = RW8_WARPS * STAGES * STAGE;
-  static constexpr int MERGE = 2 * REGS * 32 * 4;
+  static constexpr int MERGE = IN_RING ? 0 : RW8_WARPS * STATE;
+  static constexpr int SLOT = STATE / 4;           // floats of a block's partial result
 };
 
 __device__ __forceinline__ void mma_f16(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
@@ -85,6 +96,13 @@ __device__ __forceinline__ uint32_t transpose8x8(uint32_t v) {
 }
 __device__ __forceinline__ uint32_t pack_half2(float lo, float hi) { return as_u32(__floats2half2_rn(lo, hi)); }
 
+// How the line of units is cut.  In pages: what a (sequence, kv head) costs beside its pages (its queries, the join of the warps, its
+// output), as units of no page at the front of its own; the least a range has; how near a border of two (sequence, kv head)s a cut is
+// moved to it (a part of one costs its partial result's way through memory and a ticket).
+struct Rw8Cut {
+  int front, least, near;
+};
+
 // One (sequence, row tile): its rows and the pages that they see.
 struct Rw8Entry {
   int seq, q_start, row0, rows, pos0, last, lo, pg_first, n_pages;
@@ -107,25 +125,27 @@ __device__ __forceinline__ Rw8Entry rw8_entry(const Rows8Params& p, int e, int t
   return d;
 }
 
-template <int D, int NT, int HELD>
-__global__ void __launch_bounds__(RW8_WARPS * 32, (Rw8Cfg<D, NT>::BLOCKS)) attention_rows8_kernel(Rows8Params p, int n_entries, int min_units) {
-  using C = Rw8Cfg<D, NT>;
-  constexpr int KC = C::KC, CPP = C::CPP, MT = C::MT, KS = C::KS, STAGES = C::STAGES;
+template <int D, int NT, int HELD, typename T>
+__global__ void __launch_bounds__(RW8_WARPS * 32, (Rw8Cfg<D, NT, T>::BLOCKS)) attention_rows8_kernel(Rows8Params p, int n_entries, Rw8Cut cut) {
+  using C = Rw8Cfg<D, NT, T>;
+  constexpr int KC = C::KC, CPP = C::CPP, MT = C::MT, KS = C::KS, STAGES = C::STAGES, SP = C::SP, STEP = RW8_WARPS / C::CPP;
+  static_assert(RW8_WARPS % CPP == 0, "a warp keeps its place in a page");
   extern __shared__ __align__(128) uint8_t smem[];
-  float* merge_buf = reinterpret_cast<float*>(smem + C::RING);
-  int* prefix = reinterpret_cast<int*>(smem + C::RING + C::MERGE);      // [n_entries + 1] pages ahead of an entry
+  int* prefix = reinterpret_cast<int*>(smem + C::RING + C::MERGE);      // [n_entries + 1] units ahead of an entry
   __shared__ int s_scan[RW8_WARPS], s_last;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
   const int G = p.group, Hkv = p.kv.n_kv_heads;
   pdl_wait();
   pdl_launch_dependents();
 
-  // ---- the line of units: pages ahead of each entry ----
+  // ---- the line of units: units ahead of each entry ----
+  int pairs = 0;                           // (entry, kv head)s that have pages
   {
     int carry = 0;
     for (int e0 = 0; e0 < n_entries; e0 += RW8_WARPS * 32) {
       const int e = e0 + threadIdx.x;
-      const int n = e < n_entries ? rw8_entry(p, e, 8 * NT).n_pages : 0;
+      const int pages = e < n_entries ? rw8_entry(p, e, 8 * NT).n_pages : 0;
+      const int n = pages > 0 ? (pages + cut.front) * Hkv : 0;
       int x = n;
 #pragma unroll
       for (int o = 1; o < 32; o <<= 1) {
@@ -133,8 +153,9 @@ __global__ void __launch_bounds__(RW8_WARPS * 32, (Rw8Cfg<D, NT>::BLOCKS)) atten
         if (lane >= o) x += y;
       }
       if (lane == 31) s_scan[warp] = x;
-      __syncthreads();
+      pairs += __syncthreads_count(n > 0) * Hkv;
       int before = carry, all = carry;
+#pragma unroll
       for (int w = 0; w < RW8_WARPS; ++w) {
         if (w < warp) before += s_scan[w];
         all += s_scan[w];
@@ -146,160 +167,151 @@ __global__ void __launch_bounds__(RW8_WARPS * 32, (Rw8Cfg<D, NT>::BLOCKS)) atten
     if (threadIdx.x == 0) prefix[n_entries] = carry;
     __syncthreads();
   }
-  const int total = prefix[n_entries] * Hkv;
-  const int blocks = max(1, min((int)gridDim.x, total / min_units));
-  auto range_start = [&](int c) { return (int)((long)c * total / blocks); };
+  const int total = prefix[n_entries];
+  const int blocks = min((int)gridDim.x, max(total / cut.least, pairs));
   if (blockIdx.x >= blocks || total == 0) return;
-  const int u0 = range_start(blockIdx.x), u1 = range_start(blockIdx.x + 1);
-
-  // ---- the ring: this warp's chunks of the block's range, asked for in order ----
-  uint8_t* ring = smem + warp * STAGES * C::STAGE;
-  struct Cursor {
-    int unit, seg_end;       // the chunk's unit; where the units of its (entry, kv head) end
-    int sub, e, kvh, pages, pg_first, seq;
-  } in;
-  auto find_entry = [&](int unit) {        // the entry whose units hold `unit`
-    int a = 0, b = n_entries;              // prefix[a] * Hkv <= unit < prefix[b] * Hkv
+  const int per = total / blocks, longer = total - per * blocks;      // even ranges: the first `longer` have per + 1 units
+  auto find_entry = [&](int unit) {        // the entry that has the unit (the last one if they are all before it)
+    int a = 0, b = n_entries;              // prefix[a] <= unit < prefix[b]
     while (b - a > 1) {
       const int m = (a + b) >> 1;
-      if (prefix[m] * Hkv <= unit) a = m;
+      if (prefix[m] <= unit) a = m;
       else b = m;
     }
     return a;
   };
-  auto seek = [&](Cursor& c) {             // the (entry, kv head) of c.unit
-    c.e = find_entry(c.unit);
-    const Rw8Entry d = rw8_entry(p, c.e, 8 * NT);
-    c.pages = d.n_pages;
-    c.pg_first = d.pg_first;
-    c.seq = d.seq;
-    c.kvh = (c.unit - prefix[c.e] * Hkv) / d.n_pages;
-    c.seg_end = prefix[c.e] * Hkv + (c.kvh + 1) * d.n_pages;
+  const int near = min(cut.near, per / 2);
+  auto range_start = [&](int c) {          // an even cut, moved to the border of two (entry, kv head)s that is near
+    const int u = c * per + min(c, longer);
+    if (u >= total) return total;
+    const int e = find_entry(u), len = (prefix[e + 1] - prefix[e]) / Hkv, at = (u - prefix[e]) % len;
+    return at <= near ? u - at : len - at <= near ? u - at + len : u;
   };
-  in.unit = u0 + warp / CPP;
-  in.sub = warp % CPP;
-  static_assert(RW8_WARPS % CPP == 0, "a warp keeps its place in a page");
-  int next_page = 0;
+  auto block_of = [&](int u) {             // whose range holds unit u
+    int c = u < longer * (per + 1) ? u / (per + 1) : (u - longer) / per;
+    while (c + 1 < blocks && range_start(c + 1) <= u) ++c;
+    while (range_start(c) > u) --c;
+    return c;
+  };
+  const int u0 = range_start(blockIdx.x), u1 = range_start(blockIdx.x + 1);
+  if (u0 >= u1) return;
+  const int e_first = find_entry(u0);
+  // the block's part of the (entry, kv head) that has unit `at`, from there on
+  struct Segment {
+    Rw8Entry d;
+    int kvh, begin, end;                   // all units of the (entry, kv head)
+    int first, n;                          // of its pages: the block's first, and how many
+  };
+  auto segment_at = [&](int at, int& e) {
+    while (prefix[e + 1] <= at) ++e;
+    Segment s;
+    s.d = rw8_entry(p, e, 8 * NT);
+    const int len = s.d.n_pages + cut.front;
+    s.kvh = (at - prefix[e]) / len;
+    s.begin = prefix[e] + s.kvh * len;
+    s.end = s.begin + len;
+    s.first = max(at - s.begin - cut.front, 0);
+    s.n = max(min(s.end, u1) - s.begin - cut.front, 0) - s.first;
+    return s;
+  };
+
+  // ---- the ring: this warp's chunks of the block's pages, asked for in order ----
+  uint8_t* ring = smem + warp * STAGES * C::STAGE;
+  const int sub = warp % CPP;              // the warp's place in a page
+  struct {
+    int page, seg_page0, seg_page1;        // the page asked for next and the segment's, counted over the block's pages
+    int at, e, kvh, first, next_page;      // where the next segment begins; the segment's first page of its sequence
+    const int32_t* table;
+  } in;
+  in.page = warp / CPP;
+  in.seg_page0 = in.seg_page1 = 0;
+  in.at = u0;
+  in.e = e_first;
+  in.next_page = -1;
+  bool more = true;                        // there are chunks to ask for
   auto look_up = [&]() {                   // the page of the chunk that is asked for next
-    if (in.unit >= u1) return;
-    if (in.unit >= in.seg_end) seek(in);
-    const int i = in.pg_first + in.unit - (in.seg_end - in.pages);
-    next_page = i < p.kv.table_pages ? p.kv.seq_pages[(size_t)in.seq * p.kv.pages_stride + i] : -1;
+    while (in.page >= in.seg_page1) {
+      if (in.at >= u1) {
+        more = false;
+        return;
+      }
+      const Segment s = segment_at(in.at, in.e);
+      in.at = s.end;
+      in.seg_page0 = in.seg_page1;
+      in.seg_page1 += s.n;
+      in.kvh = s.kvh;
+      in.first = s.d.pg_first + s.first;
+      in.table = p.kv.seq_pages + (size_t)s.d.seq * p.kv.pages_stride;
+    }
+    const int i = in.first + in.page - in.seg_page0;
+    in.next_page = i < p.kv.table_pages ? in.table[i] : -1;
   };
-  int issued = 0;
+  // Where a 16-byte piece lies, so that no two lanes of a load meet in a bank.  Keys in the order of the rows of the product's tile
+  // (key r is row 2 (r & 3) + (r >> 2 & 1) of its eight), pieces of odd rows of 128 bytes exchanged; values row by row.  Piece i of a
+  // lane is piece lane + 32 i of the chunk: its row and place are the lane's (D = 128: the lane's for even and odd i) and a constant.
+  int k_at[2], v_at;
+  {
+    constexpr int UPR = D / 16;
+    const int r = lane / UPR, u = lane % UPR;
+    v_at = C::CODES + r * D + (D == 128 ? u ^ ((r & 3) << 1) : u ^ (((r >> 1) & 1) << 1)) * 16;
+    if (D == 128) {
+      k_at[0] = 2 * r * D + u * 16;
+      k_at[1] = (2 * r + 1) * D + (u ^ 4) * 16;
+    } else {
+      k_at[0] = k_at[1] = (((r & 3) << 1) | (r >> 2)) * D + u * 16;
+    }
+  }
+  int issued = 0;                          // the stage filled next
   auto issue = [&]() {
-    if (in.unit < u1) {
-      uint8_t* st = ring + (issued % STAGES) * C::STAGE;
-      const bool known = (unsigned)next_page < (unsigned)p.kv.n_pages;
-      const size_t row0 = ((size_t)(known ? next_page : 0) * Hkv + in.kvh) * PAGE8 + in.sub * KC;
-      const uint8_t* kc = p.k_codes + row0 * D;
-      const uint8_t* vc = p.v_codes + row0 * D;
+    if (more) {
+      uint8_t* st = ring + issued * C::STAGE;
+      const bool known = (unsigned)in.next_page < (unsigned)p.kv.n_pages;
+      const size_t row0 = ((size_t)(known ? in.next_page : 0) * Hkv + in.kvh) * PAGE8 + sub * KC;
+      const uint8_t* kc = p.k_codes + row0 * D + lane * 16;
+      const uint8_t* vc = p.v_codes + row0 * D + lane * 16;
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        constexpr int UPR = D / 16;        // 16-byte pieces of a row
-        const int x = lane + 32 * i, r = x / UPR, u = x % UPR;
-        // Where a piece lies, so that no two lanes of a load meet in a bank.  Keys in the order of the rows of the product's tile
-        // (key r is row 2 (r & 3) + (r >> 2 & 1) of its eight), pieces of odd rows of 128 bytes exchanged; values row by row.
-        const int kr = (r & ~7) | ((r & 3) << 1) | ((r >> 2) & 1);
-        const int ku = D == 128 ? u ^ ((kr & 1) << 2) : u;
-        const int vu = D == 128 ? u ^ ((r & 3) << 1) : u ^ (((r >> 1) & 1) << 1);
-        cp_async16(st + kr * D + ku * 16, kc + x * 16, 16);
-        cp_async16(st + 2048 + r * D + vu * 16, vc + x * 16, 16);
+      for (int i = 0; i < C::CODES / 512; ++i) {
+        cp_async16(st + (D == 128 ? k_at[i & 1] + 1024 * (i >> 1) : k_at[0] + 512 * i), kc + 512 * i, 16);
+        cp_async16(st + v_at + 512 * i, vc + 512 * i, 16);
       }
       if (known) {
-        if (lane < KC / 4) cp_async16(st + 4096 + lane * 16, p.k_scales + row0 + lane * 4, 16);
-        else if (lane < KC / 2) cp_async16(st + 4096 + lane * 16, p.v_scales + row0 + (lane - KC / 4) * 4, 16);
+        if (lane < KC / 2) cp_async16(st + 2 * C::CODES + lane * 16, (lane < KC / 4 ? p.k_scales : p.v_scales - KC) + row0 + lane * 4, 16);
       } else {                             // a page that the pool does not have reads as NaN
-        for (int i = lane; i < 2 * KC; i += 32) reinterpret_cast<float*>(st + 4096)[i] = __int_as_float(0x7fffffff);
+        for (int i = lane; i < 2 * KC; i += 32) reinterpret_cast<float*>(st + 2 * C::CODES)[i] = __int_as_float(0x7fffffff);
       }
-      in.unit += RW8_WARPS / CPP;
+      in.page += STEP;
       look_up();
     }
     cp_async_commit();
-    ++issued;
+    issued = issued + 1 == STAGES ? 0 : issued + 1;
   };
-  in.seg_end = 0;
   look_up();
 #pragma unroll
   for (int i = 0; i < STAGES - 1; ++i) issue();
 
-  float O[KS][NT][4], M[NT][2], L[NT][2];
-  // lanes' registers <-> 32 consecutive floats a register: the state of a (range, entry, kv head)
-  auto put = [&](float* at) {
-#pragma unroll
-    for (int i = 0; i < KS; ++i)
-#pragma unroll
-      for (int n = 0; n < NT; ++n)
-#pragma unroll
-        for (int j = 0; j < 4; ++j) at[((i * NT + n) * 4 + j) * 32 + lane] = O[i][n][j];
-#pragma unroll
-    for (int n = 0; n < NT; ++n)
-#pragma unroll
-      for (int j = 0; j < 2; ++j) {
-        at[(C::OREGS + 2 * n + j) * 32 + lane] = M[n][j];
-        at[(C::OREGS + 2 * NT + 2 * n + j) * 32 + lane] = L[n][j];
-      }
-  };
-  // this state and another one, each relative to its own maximum (a state without one is zeros, or NaN, as it is)
-  auto join = [&](auto value) {
-    float mine[NT][2], other[NT][2];
-#pragma unroll
-    for (int n = 0; n < NT; ++n)
-#pragma unroll
-      for (int j = 0; j < 2; ++j) {
-        const float mo = value(C::OREGS + 2 * n + j), m = fmaxf(M[n][j], mo);
-        mine[n][j] = M[n][j] == -INFINITY ? 1.f : fast_exp2(M[n][j] - m);
-        other[n][j] = mo == -INFINITY ? 1.f : fast_exp2(mo - m);
-        M[n][j] = m;
-        L[n][j] = L[n][j] * mine[n][j] + value(C::OREGS + 2 * NT + 2 * n + j) * other[n][j];
-      }
-#pragma unroll
-    for (int i = 0; i < KS; ++i)
-#pragma unroll
-      for (int n = 0; n < NT; ++n)
-#pragma unroll
-        for (int j = 0; j < 4; ++j) O[i][n][j] = O[i][n][j] * mine[n][j & 1] + value((i * NT + n) * 4 + j) * other[n][j & 1];
-  };
-  auto clear = [&]() {
+  // ---- segments: the block's part of one (entry, kv head) after the other ----
+  int taken = 0;                           // the stage read next
+  int page = warp / CPP, seg_page0 = 0;    // the page of the chunk in it and the segment's first, counted over the block's pages
+  int e = e_first;
+  for (int at_unit = u0; at_unit < u1;) {
+    const Segment s = segment_at(at_unit, e);
+    const Rw8Entry& d = s.d;
+    const int kvh = s.kvh;
+    at_unit = s.end;
+    if (s.n <= 0) continue;                // (the range ends among the units of no page)
+
+    float O[KS][NT][4], M[NT][2], neg[NT][2], L[NT][2];      // neg: -M, 0 while there is no M
 #pragma unroll
     for (int n = 0; n < NT; ++n) {
 #pragma unroll
-      for (int j = 0; j < 2; ++j) M[n][j] = -INFINITY, L[n][j] = 0.f;
+      for (int j = 0; j < 2; ++j) M[n][j] = -INFINITY, neg[n][j] = 0.f, L[n][j] = 0.f;
 #pragma unroll
       for (int i = 0; i < KS; ++i)
 #pragma unroll
         for (int j = 0; j < 4; ++j) O[i][n][j] = 0.f;
     }
-  };
-  // the eight warps' states into warp 0's, two at a time
-  auto join_warps = [&]() {
-#pragma unroll
-    for (int from = RW8_WARPS - 2; from >= 0; from -= 2) {
-      const int n = from == 0 ? 1 : 2, to = from == 0 ? 0 : from - 2;      // warps from .. to warps to .. (last: warp 1 to warp 0)
-      const int first = from == 0 ? 1 : from;
-      if (warp >= first && warp < first + n) put(merge_buf + (warp - first) * C::REGS * 32);
-      __syncthreads();
-      if (warp >= to && warp < to + n) {
-        const float* at = merge_buf + (warp - to) * C::REGS * 32 + lane;
-        join([&](int i) { return at[i * 32]; });
-      }
-      __syncthreads();
-    }
-  };
-
-  // ---- segments: the block's part of one (entry, kv head) after the other ----
-  int taken = 0;                           // chunks that this warp has worked through
-  int unit = u0 + warp / CPP;              // and its next one's unit
-  const int key_sub = (warp % CPP) * KC;
-  for (int seg = u0; seg < u1;) {
-    const int e = find_entry(seg);
-    const Rw8Entry d = rw8_entry(p, e, 8 * NT);
-    const int kvh = (seg - prefix[e] * Hkv) / d.n_pages;
-    const int begin = prefix[e] * Hkv + kvh * d.n_pages, end = begin + d.n_pages;
-    const int seg_end = min(end, u1);
-
     // queries: row n * 8 + g, its dims in the order in which a lane has the keys' codes
-    uint32_t qf[NT][KS][2];
+    uint32_t qf[SP][NT][KS][2];
     float fac[NT][2];                      // of the columns 2t, 2t + 1: scale * log2(e) * the row's power of two
     int col_pos[NT][2];
 #pragma unroll
@@ -308,23 +320,33 @@ __global__ void __launch_bounds__(RW8_WARPS * 32, (Rw8Cfg<D, NT>::BLOCKS)) atten
       float x[D / 4];
       float a = 0.f;
 #pragma unroll
-      for (int c = 0; c < D / 64; ++c)
+      for (int c = 0; c < D / 64; ++c) {
+        const int row = d.row0 + r;
+        const T* src = (const T*)p.q + (size_t)(d.q_start + row / G) * p.ldq + (size_t)(kvh * G + row % G) * D + 64 * c + 16 * t;
+        if (SP == 1) {
 #pragma unroll
-        for (int h = 0; h < 2; ++h) {
-          uint4 raw = make_uint4(0u, 0u, 0u, 0u);
-          if (r < d.rows) {
-            const int row = d.row0 + r;
-            raw = *reinterpret_cast<const uint4*>(p.q + (size_t)(d.q_start + row / G) * p.ldq + (size_t)(kvh * G + row % G) * D + 64 * c + 16 * t + 8 * h);
+          for (int h = 0; h < 2; ++h) {
+            uint4 raw = make_uint4(0u, 0u, 0u, 0u);
+            if (r < d.rows) raw = *reinterpret_cast<const uint4*>(src + 8 * h);
+            const __nv_bfloat162* b = reinterpret_cast<const __nv_bfloat162*>(&raw);
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+              const float2 f = __bfloat1622float2(b[i]);
+              x[c * 16 + h * 8 + 2 * i] = f.x;
+              x[c * 16 + h * 8 + 2 * i + 1] = f.y;
+            }
           }
-          const __nv_bfloat162* b = reinterpret_cast<const __nv_bfloat162*>(&raw);
+        } else {
 #pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            const float2 f = __bfloat1622float2(b[i]);
-            x[c * 16 + h * 8 + 2 * i] = f.x;
-            x[c * 16 + h * 8 + 2 * i + 1] = f.y;
-            a = fmaxf(a, fmaxf(fabsf(f.x), fabsf(f.y)));
+          for (int h = 0; h < 4; ++h) {
+            float4 f = make_float4(0.f, 0.f, 0.f, 0.f);
+            if (r < d.rows) f = *reinterpret_cast<const float4*>(src + 4 * h);
+            x[c * 16 + 4 * h] = f.x, x[c * 16 + 4 * h + 1] = f.y, x[c * 16 + 4 * h + 2] = f.z, x[c * 16 + 4 * h + 3] = f.w;
           }
         }
+      }
+#pragma unroll
+      for (int i = 0; i < D / 4; ++i) a = fmaxf(a, fabsf(x[i]));
       a = fmaxf(a, __shfl_xor_sync(0xffffffffu, a, 1));
       a = fmaxf(a, __shfl_xor_sync(0xffffffffu, a, 2));
       // the power of two above the row's largest entry (a row that is zero or not finite: 1)
@@ -334,7 +356,12 @@ __global__ void __launch_bounds__(RW8_WARPS * 32, (Rw8Cfg<D, NT>::BLOCKS)) atten
 #pragma unroll
       for (int s = 0; s < KS; ++s)
 #pragma unroll
-        for (int h = 0; h < 2; ++h) qf[n][s][h] = pack_half2(x[4 * s + 2 * h] * down * down2, x[4 * s + 2 * h + 1] * down * down2);
+        for (int h = 0; h < 2; ++h) {
+          const float y0 = x[4 * s + 2 * h] * down * down2, y1 = x[4 * s + 2 * h + 1] * down * down2;
+          const __half2 hi = __floats2half2_rn(y0, y1);
+          qf[0][n][s][h] = as_u32(hi);
+          if (SP == 2) qf[SP - 1][n][s][h] = pack_half2(y0 - __low2float(hi), y1 - __high2float(hi));
+        }
       const float f = ldexpf(p.scale_log2, ex);
 #pragma unroll
       for (int j = 0; j < 2; ++j) {
@@ -344,18 +371,14 @@ __global__ void __launch_bounds__(RW8_WARPS * 32, (Rw8Cfg<D, NT>::BLOCKS)) atten
       }
     }
     const int first_pos = d.pos0 + d.row0 / G;
-    clear();
     bool unset = true;                     // some column has no maximum yet
-    for (; unit < seg_end; unit += RW8_WARPS / CPP) {
-      cp_async_wait<STAGES - 2>();
-      __syncwarp();                        // every lane's copies are here, and every lane is done with the stage before
-      issue();
-      const uint8_t* st = ring + (taken % STAGES) * C::STAGE;
-      const float* ks_s = reinterpret_cast<const float*>(st + 4096);
+
+    auto chunk = [&](auto masked_c, const uint8_t* st, int key0) {
+      constexpr bool MASKED = decltype(masked_c)::value;
+      const float* ks_s = reinterpret_cast<const float*>(st + 2 * C::CODES);
       const float* vs_s = ks_s + KC;
-      const int key0 = (d.pg_first + unit - begin) * PAGE8 + key_sub;
-      const bool masked = key0 + KC - 1 > first_pos || (p.window > 0 && key0 <= d.last - p.window);
-      float x[MT][NT][4], vs[MT][2];
+      float S[MT][NT][4], vs[MT][2], ks[MT][2];
+      uint32_t hidden = 0u;                // bit (m * NT + n) * 4 + j: that score's key is not seen
 #pragma unroll
       for (int m = 0; m < MT; ++m) {
         uint32_t ka[KS], kb[KS];
@@ -370,48 +393,64 @@ __global__ void __launch_bounds__(RW8_WARPS * 32, (Rw8Cfg<D, NT>::BLOCKS)) atten
 #pragma unroll
         for (int n = 0; n < NT; ++n)
 #pragma unroll
-          for (int j = 0; j < 4; ++j) x[m][n][j] = 0.f;
+          for (int j = 0; j < 4; ++j) S[m][n][j] = 0.f;
 #pragma unroll
         for (int s = 0; s < KS; ++s) {
           uint32_t a[4];
           halves4<HELD>(ka[s], a[0], a[2]);
           halves4<HELD>(kb[s], a[1], a[3]);
 #pragma unroll
-          for (int n = 0; n < NT; ++n) mma_f16(x[m][n], a, qf[n][s][0], qf[n][s][1]);
+          for (int n = 0; n < NT; ++n)
+#pragma unroll
+            for (int z = 0; z < SP; ++z) mma_f16(S[m][n], a, qf[z][n][s][0], qf[z][n][s][1]);
         }
         // rows g and g + 8 of the tile are the keys pk and pk + 8
         const int pk = m * 16 + (g >> 1) + 4 * (g & 1);
-        const float ks0 = ks_s[pk], ks1 = ks_s[pk + 8];
+        ks[m][0] = ks_s[pk], ks[m][1] = ks_s[pk + 8];
         vs[m][0] = vs_s[pk], vs[m][1] = vs_s[pk + 8];
+        if (MASKED) {
 #pragma unroll
-        for (int n = 0; n < NT; ++n)
+          for (int n = 0; n < NT; ++n)
 #pragma unroll
-          for (int j = 0; j < 4; ++j) {
-            x[m][n][j] *= (j < 2 ? ks0 : ks1) * fac[n][j & 1];
-            if (masked) {
+            for (int j = 0; j < 4; ++j) {
               const int key = key0 + pk + (j < 2 ? 0 : 8);
-              if (key > col_pos[n][j & 1] || (p.window > 0 && key <= col_pos[n][j & 1] - p.window)) x[m][n][j] = -INFINITY;
+              if (key > col_pos[n][j & 1] || (p.window > 0 && key <= col_pos[n][j & 1] - p.window)) hidden |= 1u << ((m * NT + n) * 4 + j);
             }
-          }
+        }
       }
-      float ex[MT][NT][4];
-      auto weigh = [&]() {                 // -> the largest weight times value scale
-        float top = 0.f;
+      auto is_hidden = [&](int m, int n, int j) { return MASKED && ((hidden >> ((m * NT + n) * 4 + j)) & 1u); };
+      uint32_t pb[SP][MT][NT][2];
+      float sum[NT][2];
+      auto weigh = [&]() {                 // weights, packed for the second product, and their sums; -> whether they are in range
+        __half2 top = __halves2half2(__ushort_as_half(0), __ushort_as_half(0));
+        bool fine = true;
 #pragma unroll
-        for (int n = 0; n < NT; ++n)
+        for (int n = 0; n < NT; ++n) {
+          sum[n][0] = L[n][0], sum[n][1] = L[n][1];
 #pragma unroll
-          for (int j = 0; j < 4; ++j) {
-            const float neg = M[n][j & 1] == -INFINITY ? 0.f : -M[n][j & 1];
+          for (int m = 0; m < MT; ++m) {
+            float w[4];
 #pragma unroll
-            for (int m = 0; m < MT; ++m) {
-              ex[m][n][j] = fast_exp2(x[m][n][j] + neg);
-              top = fmaxf(top, ex[m][n][j] * fmaxf(vs[m][j >> 1], RW8_TINY));
+            for (int j = 0; j < 4; ++j) {
+              float x = fast_exp2(fmaf(S[m][n][j], ks[m][j >> 1] * fac[n][j & 1], neg[n][j & 1]));
+              w[j] = x * vs[m][j >> 1];
+              if (is_hidden(m, n, j)) x = 0.f, w[j] = 0.f;               // (the key's scales may be anything)
+              sum[n][j & 1] += x;
+            }
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+              const __half2 hi = __floats2half2_rn(w[2 * h], w[2 * h + 1]);
+              top = __hmax2(top, hi);
+              pb[0][m][n][h] = as_u32(hi);
+              if (SP == 2) pb[SP - 1][m][n][h] = pack_half2(w[2 * h] - __low2float(hi), w[2 * h + 1] - __high2float(hi));
             }
           }
-        return top;
+          fine = fine && !(sum[n][0] > RW8_SUM) && !(sum[n][1] > RW8_SUM);
+        }
+        return fine && !(fmaxf(__low2float(top), __high2float(top)) > RW8_LAZY);
       };
-      float top = unset ? INFINITY : weigh();
-      if (__any_sync(0xffffffffu, top > RW8_LAZY)) {
+      const bool fine = weigh();
+      if (__any_sync(0xffffffffu, unset || !fine)) {
         unset = false;
 #pragma unroll
         for (int n = 0; n < NT; ++n)
@@ -420,7 +459,9 @@ __global__ void __launch_bounds__(RW8_WARPS * 32, (Rw8Cfg<D, NT>::BLOCKS)) atten
             float mx = -INFINITY;
 #pragma unroll
             for (int m = 0; m < MT; ++m)
-              mx = fmaxf(mx, fmaxf(x[m][n][j] + fast_log2(fmaxf(vs[m][0], RW8_TINY)), x[m][n][j + 2] + fast_log2(fmaxf(vs[m][1], RW8_TINY))));
+#pragma unroll
+              for (int h = 0; h < 2; ++h)
+                if (!is_hidden(m, n, j + 2 * h)) mx = fmaxf(mx, S[m][n][j + 2 * h] * (ks[m][h] * fac[n][j]) + fast_log2(fmaxf(vs[m][h], RW8_TINY)));
 #pragma unroll
             for (int o = 4; o < 32; o <<= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, o));
             const float m_new = fmaxf(M[n][j], mx), f = M[n][j] == -INFINITY ? 1.f : fast_exp2(M[n][j] - m_new);
@@ -428,154 +469,264 @@ __global__ void __launch_bounds__(RW8_WARPS * 32, (Rw8Cfg<D, NT>::BLOCKS)) atten
 #pragma unroll
             for (int i = 0; i < KS; ++i) O[i][n][j] *= f, O[i][n][j + 2] *= f;
             M[n][j] = m_new;
+            neg[n][j] = m_new == -INFINITY ? 0.f : -m_new;
             unset = unset || m_new == -INFINITY;
           }
         unset = __any_sync(0xffffffffu, unset);
         weigh();
       }
+      float Oc[SP == 2 ? KS : 1][SP == 2 ? NT : 1][4];
+      if (SP == 2) {
+#pragma unroll
+        for (int i = 0; i < KS; ++i)
+#pragma unroll
+          for (int n = 0; n < NT; ++n)
+#pragma unroll
+            for (int j = 0; j < 4; ++j) Oc[SP == 2 ? i : 0][SP == 2 ? n : 0][j] = 0.f;
+      }
+#pragma unroll
+      for (int n = 0; n < NT; ++n) L[n][0] = sum[n][0], L[n][1] = sum[n][1];
       const int seen0 = max(d.lo - key0, 0), seen1 = d.last - key0;      // rows of the chunk that some query sees
 #pragma unroll
       for (int m = 0; m < MT; ++m) {
-        uint32_t pb[NT][2];
 #pragma unroll
-        for (int n = 0; n < NT; ++n) {
-          float w[4];
+        for (int z = 0; z < SP; ++z)
 #pragma unroll
-          for (int j = 0; j < 4; ++j) {
-            L[n][j & 1] += ex[m][n][j];
-            w[j] = ex[m][n][j] * vs[m][j >> 1];
-            if (masked && x[m][n][j] == -INFINITY) w[j] = 0.f;           // (its scale may be anything)
-          }
-          pb[n][0] = transpose8x8(pack_half2(w[0], w[1]));
-          pb[n][1] = transpose8x8(pack_half2(w[2], w[3]));
-        }
+          for (int n = 0; n < NT; ++n) pb[z][m][n][0] = transpose8x8(pb[z][m][n][0]), pb[z][m][n][1] = transpose8x8(pb[z][m][n][1]);
         // values: keys 2t, 2t + 1 (+ 8) of the tile are the rows t, t + 4 (+ 8); a lane has the dims g * D / 8 ..
         uint32_t vw[4][D / 32];
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
           const int r = m * 16 + t + 4 * (j & 1) + 8 * (j >> 1);
           if (D == 128) {
-            const uint4 v = *reinterpret_cast<const uint4*>(st + 2048 + r * D + ((g ^ ((r & 3) << 1)) * 16));
+            const uint4 v = *reinterpret_cast<const uint4*>(st + C::CODES + r * D + ((g ^ ((r & 3) << 1)) * 16));
             vw[j][0] = v.x, vw[j][1] = v.y, vw[j][D / 32 - 2] = v.z, vw[j][D / 32 - 1] = v.w;
           } else {
-            const uint2 v = *reinterpret_cast<const uint2*>(st + 2048 + r * D + (((g >> 1) ^ (((r >> 1) & 1) << 1)) * 16) + (g & 1) * 8);
+            const uint2 v = *reinterpret_cast<const uint2*>(st + C::CODES + r * D + (((g >> 1) ^ (((r >> 1) & 1) << 1)) * 16) + (g & 1) * 8);
             vw[j][0] = v.x, vw[j][1] = v.y;
           }
-          if (masked && (r < seen0 || r > seen1)) {                      // (what lies there may be no number)
+          if (MASKED && (r < seen0 || r > seen1)) {                      // (what lies there may be no number)
 #pragma unroll
             for (int i = 0; i < D / 32; ++i) vw[j][i] = 0u;
           }
         }
 #pragma unroll
         for (int w = 0; w < D / 32; ++w) {       // four dims: two tiles of dims
-          uint32_t z[4], a01[4], a23[4];
-          asm("prmt.b32 %0, %1, %2, 0x5140;" : "=r"(z[0]) : "r"(vw[0][w]), "r"(vw[1][w]));
-          asm("prmt.b32 %0, %1, %2, 0x7362;" : "=r"(z[1]) : "r"(vw[0][w]), "r"(vw[1][w]));
-          asm("prmt.b32 %0, %1, %2, 0x5140;" : "=r"(z[2]) : "r"(vw[2][w]), "r"(vw[3][w]));
-          asm("prmt.b32 %0, %1, %2, 0x7362;" : "=r"(z[3]) : "r"(vw[2][w]), "r"(vw[3][w]));
-          halves4<HELD>(z[0], a01[0], a01[1]);
-          halves4<HELD>(z[2], a01[2], a01[3]);
-          halves4<HELD>(z[1], a23[0], a23[1]);
-          halves4<HELD>(z[3], a23[2], a23[3]);
+          uint32_t z4[4], a01[4], a23[4];
+          asm("prmt.b32 %0, %1, %2, 0x5140;" : "=r"(z4[0]) : "r"(vw[0][w]), "r"(vw[1][w]));
+          asm("prmt.b32 %0, %1, %2, 0x7362;" : "=r"(z4[1]) : "r"(vw[0][w]), "r"(vw[1][w]));
+          asm("prmt.b32 %0, %1, %2, 0x5140;" : "=r"(z4[2]) : "r"(vw[2][w]), "r"(vw[3][w]));
+          asm("prmt.b32 %0, %1, %2, 0x7362;" : "=r"(z4[3]) : "r"(vw[2][w]), "r"(vw[3][w]));
+          halves4<HELD>(z4[0], a01[0], a01[1]);
+          halves4<HELD>(z4[2], a01[2], a01[3]);
+          halves4<HELD>(z4[1], a23[0], a23[1]);
+          halves4<HELD>(z4[3], a23[2], a23[3]);
 #pragma unroll
-          for (int n = 0; n < NT; ++n) {
-            mma_f16(O[2 * w][n], a01, pb[n][0], pb[n][1]);
-            mma_f16(O[2 * w + 1][n], a23, pb[n][0], pb[n][1]);
-          }
+          for (int n = 0; n < NT; ++n)
+#pragma unroll
+            for (int z = 0; z < SP; ++z) {
+              mma_f16(SP == 2 ? Oc[SP == 2 ? 2 * w : 0][SP == 2 ? n : 0] : O[2 * w][n], a01, pb[z][m][n][0], pb[z][m][n][1]);
+              mma_f16(SP == 2 ? Oc[SP == 2 ? 2 * w + 1 : 0][SP == 2 ? n : 0] : O[2 * w + 1][n], a23, pb[z][m][n][0], pb[z][m][n][1]);
+            }
         }
       }
-      ++taken;
+      if (SP == 2) {
+#pragma unroll
+        for (int i = 0; i < KS; ++i)
+#pragma unroll
+          for (int n = 0; n < NT; ++n)
+#pragma unroll
+            for (int j = 0; j < 4; ++j) O[i][n][j] += Oc[SP == 2 ? i : 0][SP == 2 ? n : 0][j];
+      }
+    };
+
+    for (; page < seg_page0 + s.n; page += STEP) {
+      cp_async_wait<STAGES - 2>();
+      __syncwarp();                        // every lane's copies are here, and every lane is done with the stage before
+      issue();
+      const uint8_t* st = ring + taken * C::STAGE;
+      taken = taken + 1 == STAGES ? 0 : taken + 1;
+      const int key0 = (d.pg_first + s.first + page - seg_page0) * PAGE8 + sub * KC;
+      if (key0 + KC - 1 > first_pos || (p.window > 0 && key0 <= d.last - p.window)) chunk(std::true_type{}, st, key0);
+      else chunk(std::false_type{}, st, key0);
     }
+    seg_page0 += s.n;
 #pragma unroll
     for (int n = 0; n < NT; ++n)
 #pragma unroll
       for (int j = 0; j < 2; ++j)
 #pragma unroll
         for (int o = 4; o < 32; o <<= 1) L[n][j] += __shfl_xor_sync(0xffffffffu, L[n][j], o);
-    join_warps();
-    bool whole = true;
-    if (begin < u0 || end > u1) {          // other blocks have units of it too
-      auto block_of = [&](int u) {         // the block whose range holds unit u
-        int c = (int)((long)u * blocks / total);
-        while (range_start(c + 1) <= u) ++c;
-        while (range_start(c) > u) --c;
-        return c;
-      };
-      const int c_first = block_of(begin), c_last = block_of(end - 1);
-      auto slot = [&](int c) { return p.slots + (size_t)(2 * c + (range_start(c) < begin ? 1 : 0)) * C::REGS * 32; };
+
+    // ---- the warps' states meet: each leaves its own where nothing is being copied to (the stage read last; `issue` fills the one
+    // before it first), then a warp has some tiles of the output from all eight ----
+    auto state_of = [&](int w, int stage) { return reinterpret_cast<float*>(C::IN_RING ? smem + (w * STAGES + stage) * C::STAGE : smem + C::RING + w * C::STATE); };
+    __shared__ uint8_t s_stage[RW8_WARPS];
+    {
+      __syncwarp();
+      const int free_stage = taken == 0 ? STAGES - 1 : taken - 1;
+      if (lane == 0) s_stage[warp] = (uint8_t)free_stage;
+      float* at = state_of(warp, free_stage);
+#pragma unroll
+      for (int i = 0; i < KS; ++i)
+#pragma unroll
+        for (int n = 0; n < NT; ++n)
+#pragma unroll
+          for (int j = 0; j < 4; ++j) at[((i * NT + n) * 4 + j) * 32 + lane] = O[i][n][j];
+      if (g == 0) {
+#pragma unroll
+        for (int n = 0; n < NT; ++n)
+#pragma unroll
+          for (int j = 0; j < 2; ++j) at[C::PAIRS * 128 + n * 8 + 2 * t + j] = M[n][j], at[C::PAIRS * 128 + 8 * NT + n * 8 + 2 * t + j] = L[n][j];
+      }
+    }
+    __syncthreads();
+    // other blocks have pages of it too: partial results, a block's of its first segment and of its last apart
+    const bool shared_out = s.n < d.n_pages;
+    int c_first = 0, c_last = 0, first_slot = 0;
+    float* my_slot = nullptr;
+    if (shared_out) {
+      c_first = block_of(s.begin + cut.front), c_last = block_of(s.end - 1);
+      first_slot = 2 * c_first + (range_start(c_first) < s.begin ? 1 : 0);
+      my_slot = p.slots + (size_t)((int)blockIdx.x == c_first ? first_slot : 2 * (int)blockIdx.x) * C::SLOT;
+    }
+    // one tile of the output out of several states (a state without a maximum is zeros, or NaN, as it is), eight at a time
+    struct Tile {
+      float o[4], m[2], l[2];
+    };
+    auto gather = [&](int pair, int first, int n_states, int step, auto state, auto load) {
+      const int n = pair % NT;
+      Tile r;
+      r.m[0] = r.m[1] = -INFINITY;
+      r.l[0] = r.l[1] = r.o[0] = r.o[1] = r.o[2] = r.o[3] = 0.f;
+      for (int w0 = first; w0 < n_states; w0 += 8 * step) {
+        Tile x[8];
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+          const int w = w0 + i * step;
+          const float* at = state(min(w, n_states - 1));
+          const float* m = at + C::PAIRS * 128 + n * 8 + 2 * t;
+#pragma unroll
+          for (int j = 0; j < 2; ++j) x[i].m[j] = load(m + j), x[i].l[j] = load(m + 8 * NT + j);
+#pragma unroll
+          for (int j = 0; j < 4; ++j) x[i].o[j] = load(at + (pair * 4 + j) * 32 + lane);
+        }
+        float f[2], top[2] = {r.m[0], r.m[1]};
+#pragma unroll
+        for (int i = 0; i < 8; ++i)
+#pragma unroll
+          for (int j = 0; j < 2; ++j) top[j] = fmaxf(top[j], x[i].m[j]);
+#pragma unroll
+        for (int j = 0; j < 2; ++j) f[j] = r.m[j] == -INFINITY ? 1.f : fast_exp2(r.m[j] - top[j]), r.m[j] = top[j], r.l[j] *= f[j];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) r.o[j] *= f[j & 1];
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+          if (w0 + i * step >= n_states) break;
+#pragma unroll
+          for (int j = 0; j < 2; ++j) f[j] = x[i].m[j] == -INFINITY ? 1.f : fast_exp2(x[i].m[j] - top[j]), r.l[j] = fmaf(x[i].l[j], f[j], r.l[j]);
+#pragma unroll
+          for (int j = 0; j < 4; ++j) r.o[j] = fmaf(x[i].o[j], f[j & 1], r.o[j]);
+        }
+      }
+      return r;
+    };
+    auto write_out = [&](int pair, const Tile& r) {
+#pragma unroll
+      for (int j = 0; j < 2; ++j) {
+        const int r8 = (pair % NT) * 8 + 2 * t + j;
+        if (r8 >= d.rows) continue;
+        const int row = d.row0 + r8;
+        const float inv = r.l[j] == 0.f ? 0.f : 1.f / r.l[j];
+        T* at = (T*)p.out + (size_t)(d.q_start + row / G) * p.ldo + (size_t)(kvh * G + row % G) * D + g * (D / 8) + 2 * (pair / NT);
+        if (SP == 2) *reinterpret_cast<float2*>(at) = make_float2(r.o[j] * inv, r.o[j + 2] * inv);
+        else *reinterpret_cast<__nv_bfloat162*>(at) = __floats2bfloat162_rn(r.o[j] * inv, r.o[j + 2] * inv);
+      }
+    };
+    auto store = [&](float* slot, int pair, const Tile& r) {
+#pragma unroll
+      for (int j = 0; j < 4; ++j) __stcg(slot + (pair * 4 + j) * 32 + lane, r.o[j]);
+      if (pair < NT && g == 0) {
+#pragma unroll
+        for (int j = 0; j < 2; ++j) __stcg(slot + C::PAIRS * 128 + pair * 8 + 2 * t + j, r.m[j]), __stcg(slot + C::PAIRS * 128 + 8 * NT + pair * 8 + 2 * t + j, r.l[j]);
+      }
+    };
+    for (int pair = warp; pair < C::PAIRS; pair += RW8_WARPS) {
+      const Tile r = gather(pair, 0, RW8_WARPS, 1, [&](int w) { return (const float*)state_of(w, s_stage[w]); }, [](const float* x) { return *x; });
+      if (shared_out) store(my_slot, pair, r);
+      else write_out(pair, r);
+    }
+    if (shared_out) {
+      __threadfence();
+      __syncthreads();
       int* ticket = p.tickets + (size_t)e * Hkv + kvh;
-      if (warp == 0) {
-        put(slot(blockIdx.x));
+      if (threadIdx.x == 0) {
+        s_last = atomicAdd(ticket, 1) == c_last - c_first;
         __threadfence();
-        __syncwarp();
-        if (lane == 0) s_last = atomicAdd(ticket, 1) == c_last - c_first;
       }
       __syncthreads();
-      whole = s_last != 0;
-      if (whole) {
-        __threadfence();
-        clear();
-        for (int c = c_first + warp; c <= c_last; c += RW8_WARPS) {
-          const float* at = slot(c) + lane;
-          join([&](int i) { return __ldcg(at + i * 32); });
+      if (s_last) {
+        // the parts in order, a tile's shared by the warps that have no tile of their own (past L1: a line of it may hold the
+        // neighbour of a slot that was read before the neighbour was written)
+        constexpr int SHARE = C::PAIRS < RW8_WARPS ? RW8_WARPS / C::PAIRS : 1;
+        const int n_parts = c_last - c_first + 1;
+        for (int pair = warp / SHARE; pair < C::PAIRS; pair += RW8_WARPS / SHARE) {
+          Tile r = gather(pair, warp % SHARE, n_parts, SHARE,
+                          [&](int i) { return (const float*)(p.slots + (size_t)(i == 0 ? first_slot : 2 * (c_first + i)) * C::SLOT); },
+                          [](const float* x) { return __ldcg(x); });
+          if (SHARE > 1) {
+            float* mine = state_of(warp, s_stage[warp]);
+            mine[lane] = r.o[0], mine[32 + lane] = r.o[1], mine[64 + lane] = r.o[2], mine[96 + lane] = r.o[3];
+            mine[128 + lane] = r.m[0], mine[160 + lane] = r.m[1], mine[192 + lane] = r.l[0], mine[224 + lane] = r.l[1];
+            __syncthreads();
+            if (warp % SHARE) break;
+#pragma unroll
+            for (int w = 1; w < SHARE; ++w) {
+              const float* x = state_of(warp + w, s_stage[warp + w]) + lane;
+#pragma unroll
+              for (int j = 0; j < 2; ++j) {
+                const float m = x[128 + 32 * j], top = fmaxf(r.m[j], m);
+                const float f = r.m[j] == -INFINITY ? 1.f : fast_exp2(r.m[j] - top), h = m == -INFINITY ? 1.f : fast_exp2(m - top);
+                r.m[j] = top;
+                r.l[j] = r.l[j] * f + x[192 + 32 * j] * h;
+                r.o[j] = r.o[j] * f + x[32 * j] * h;
+                r.o[j + 2] = r.o[j + 2] * f + x[64 + 32 * j] * h;
+              }
+            }
+          }
+          write_out(pair, r);
         }
-        join_warps();
         if (threadIdx.x == 0) *ticket = 0;
       }
-      __syncthreads();                     // (s_last is free again)
     }
-    if (whole && warp == 0) {
-#pragma unroll
-      for (int n = 0; n < NT; ++n)
-#pragma unroll
-        for (int j = 0; j < 2; ++j) {
-          const int r = n * 8 + 2 * t + j;
-          if (r >= d.rows) continue;
-          const int row = d.row0 + r;
-          const float inv = L[n][j] == 0.f ? 0.f : 1.f / L[n][j];
-          __nv_bfloat16* o = p.out + (size_t)(d.q_start + row / G) * p.ldo + (size_t)(kvh * G + row % G) * D + g * (D / 8);
-#pragma unroll
-          for (int w = 0; w < D / 64; ++w) {     // eight dims
-            uint32_t v[4];
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-              __nv_bfloat162 h = __floats2bfloat162_rn(O[4 * w + i][n][j] * inv, O[4 * w + i][n][j + 2] * inv);
-              v[i] = *reinterpret_cast<uint32_t*>(&h);
-            }
-            *reinterpret_cast<uint4*>(o + 8 * w) = make_uint4(v[0], v[1], v[2], v[3]);
-          }
-        }
-    }
-    seg = seg_end;
+    __syncthreads();                       // the stages may be filled again, s_last and s_stage written
   }
   cp_async_wait_all();
 }
 
-template <int D, int NT, int HELD> bool rw8_configured() {
-  static PerDevice<bool> done;
-  if (!done.here())
-    done.here() = cudaFuncSetAttribute(attention_rows8_kernel<D, NT, HELD>, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                       Rw8Cfg<D, NT>::RING + Rw8Cfg<D, NT>::MERGE + 4 * (RW8_MAX_ENTRIES + 1)) == cudaSuccess;
-  return done.here();
-}
-
-template <int D, int NT, int HELD> int launch_rows8(const Rows8Params& p, int n_entries, int grid, cudaStream_t stream) {
-  using C = Rw8Cfg<D, NT>;
-  if (!rw8_configured<D, NT, HELD>()) return LLMI_ERR_LAUNCH;
+template <int D, int NT, int HELD, typename T> int launch_rows8(const Rows8Params& p, int n_entries, int grid, cudaStream_t stream) {
+  using C = Rw8Cfg<D, NT, T>;
+  constexpr auto kernel = attention_rows8_kernel<D, NT, HELD, T>;
+  static PerDevice<bool> configured;
+  if (!configured.here()) {
+    if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, C::RING + C::MERGE + 4 * (RW8_MAX_ENTRIES + 1)) != cudaSuccess)
+      return LLMI_ERR_LAUNCH;
+    configured.here() = true;
+  }
   const size_t smem = C::RING + C::MERGE + 4 * ((size_t)n_entries + 1);
   // no more blocks than are resident: many entries' table may leave room for one a SM only (228 KB; a block's own 1 KB and its statics)
   const int fit = (int)((228 << 10) / (smem + 1280));
   const int resident = min(C::BLOCKS, max(1, fit)) * sm_count();
-  return launch_pdl(PDL_ATTENTION, attention_rows8_kernel<D, NT, HELD>, (unsigned)min(grid, resident), RW8_WARPS * 32, smem, stream, p, n_entries, RW8_WARPS / C::CPP);
+  static const Rw8Cut cut = {getenv("RW8_FRONT") ? atoi(getenv("RW8_FRONT")) : 2, getenv("RW8_LEAST") ? atoi(getenv("RW8_LEAST")) : 1024 / D, getenv("RW8_NEAR") ? atoi(getenv("RW8_NEAR")) : 512 / D};
+  return launch_pdl(PDL_ATTENTION, kernel, (unsigned)min(grid, resident), RW8_WARPS * 32, smem, stream, p, n_entries, cut);
 }
 
-// query rows of a tile, in eighths: the fewest that hold a sequence's rows, of those there are
-inline int rw8_tiles(int D, long rows) { return rows <= 8 ? 1 : (rows <= 16 || D == 128) ? 2 : 4; }
-inline int rw8_regs(int D, int nt) { return D / 16 * nt * 4 + 4 * nt; }
-inline int rw8_grid(int D, int nt, long units) {
-  const long n = (long)(rw8_regs(D, nt) <= 44 ? 2 : 1) * sm_count();
-  return (int)(units < n ? units : n);
+// Eighths of query rows in a tile: the fewest that hold a sequence's rows, of those there are.
+inline int rw8_tiles(int dtype, int D, long rows) {
+  if (dtype == LLMI_DTYPE_F32) return rows <= 8 || D == 128 ? 1 : 2;
+  return rows <= 8 ? 1 : (rows <= 16 || D == 128) ? 2 : 4;
 }
+inline int rw8_grid(long units) { return (int)(units < 2L * sm_count() ? units : 2L * sm_count()); }
 
 }  // namespace llmi
 
@@ -583,39 +734,44 @@ using namespace llmi;
 
 // What a call needs: *floats of scratch for the blocks' partial results, *ints tickets (zero before the first call; every call
 // leaves them zero).  `max_q`: most tokens that a sequence brings.
-LLMI_EXPORT int llmi_attention_rows8_workspace(int n_seqs, int max_q, int n_heads, int n_kv_heads, int head_dim, int table_pages, long* floats, long* ints) {
-  if (n_seqs <= 0 || max_q <= 0 || n_kv_heads <= 0 || n_heads % n_kv_heads || (head_dim != 64 && head_dim != 128) || table_pages <= 0) return LLMI_ERR_BAD_SIZE;
+LLMI_EXPORT int llmi_attention_rows8_workspace(int dtype, int n_seqs, int max_q, int n_heads, int n_kv_heads, int head_dim, int table_pages, long* floats,
+                                               long* ints) {
+  if (n_seqs <= 0 || max_q <= 0 || n_kv_heads <= 0 || n_heads <= 0 || n_heads % n_kv_heads || (head_dim != 64 && head_dim != 128) || table_pages <= 0)
+    return LLMI_ERR_BAD_SIZE;
   const long rows = (long)max_q * (n_heads / n_kv_heads);
-  const int nt = rw8_tiles(head_dim, rows);
+  const int nt = rw8_tiles(dtype, head_dim, rows);
   const long tiles = (rows + 8 * nt - 1) / (8 * nt);
-  if (n_seqs * tiles > RW8_MAX_ENTRIES || n_seqs * tiles * n_kv_heads * (long)table_pages > 0x7fffffffL) return LLMI_ERR_BAD_SIZE;
+  if (n_seqs * tiles > RW8_MAX_ENTRIES || n_seqs * tiles * n_kv_heads * ((long)table_pages + 64) > 0x7fffffffL) return LLMI_ERR_BAD_SIZE;
   *ints = n_seqs * tiles * n_kv_heads;
-  *floats = 2L * rw8_grid(head_dim, nt, n_seqs * tiles * n_kv_heads * (long)table_pages) * rw8_regs(head_dim, nt) * 32;
+  *floats = 2L * rw8_grid(n_seqs * tiles * n_kv_heads * (long)table_pages) * (head_dim / 16 * nt * 128 + 16 * nt);
   return LLMI_OK;
 }
 
-LLMI_EXPORT int llmi_attention_rows8(int held, const void* q, long ldq, void* out, long ldo, const void* k_codes, const float* k_scales,
+LLMI_EXPORT int llmi_attention_rows8(int dtype, int held, const void* q, long ldq, void* out, long ldo, const void* k_codes, const float* k_scales,
                                      const void* v_codes, const float* v_scales, const int32_t* seq_q_start, const int32_t* seq_kv_len,
                                      const int32_t* seq_pages, int pages_stride, int table_pages, int n_seqs, int n_pages, int max_q,
                                      int n_heads, int n_kv_heads, int head_dim, float scale, int window, float* slots, long n_floats, int* tickets,
                                      long n_ints, cudaStream_t stream) {
   long floats, ints;
-  const int rc = llmi_attention_rows8_workspace(n_seqs, max_q, n_heads, n_kv_heads, head_dim, table_pages, &floats, &ints);
+  if (dtype != LLMI_DTYPE_F32 && dtype != LLMI_DTYPE_BF16) return LLMI_ERR_BAD_DTYPE;
+  const int rc = llmi_attention_rows8_workspace(dtype, n_seqs, max_q, n_heads, n_kv_heads, head_dim, table_pages, &floats, &ints);
   if (rc != LLMI_OK) return rc;
   if (n_floats < floats || n_ints < ints || n_pages <= 0 || window < 0) return LLMI_ERR_BAD_SIZE;
   if (held != HELD_INT8 && held != HELD_E4M3) return LLMI_ERR_BAD_DTYPE;
-  if ((((uintptr_t)q | (uintptr_t)out | (uintptr_t)k_codes | (uintptr_t)v_codes | (uintptr_t)k_scales | (uintptr_t)v_scales) & 15) || (ldq & 7) || (ldo & 7))
+  const long even = dtype == LLMI_DTYPE_F32 ? 3 : 7;         // rows are whole 16-byte pieces
+  if ((((uintptr_t)q | (uintptr_t)out | (uintptr_t)k_codes | (uintptr_t)v_codes | (uintptr_t)k_scales | (uintptr_t)v_scales) & 15) || (ldq & even) || (ldo & even))
     return LLMI_ERR_ALIGN;
   const int group = n_heads / n_kv_heads;
   const long rows = (long)max_q * group;
-  const int nt = rw8_tiles(head_dim, rows), tiles = (int)((rows + 8 * nt - 1) / (8 * nt));
-  Rows8Params p{(const __nv_bfloat16*)q, ldq, (__nv_bfloat16*)out, ldo, (const uint8_t*)k_codes, k_scales, (const uint8_t*)v_codes, v_scales,
+  const int nt = rw8_tiles(dtype, head_dim, rows), tiles = (int)((rows + 8 * nt - 1) / (8 * nt));
+  Rows8Params p{q, ldq, out, ldo, (const uint8_t*)k_codes, k_scales, (const uint8_t*)v_codes, v_scales,
                 seq_q_start, seq_kv_len, Paged8{seq_pages, pages_stride, table_pages, n_pages, n_kv_heads, head_dim}, n_seqs, group, tiles,
                 scale * 1.4426950408889634f, window, slots, tickets};
-  const int n_entries = n_seqs * tiles, grid = rw8_grid(head_dim, nt, (long)n_entries * n_kv_heads * table_pages);
-#define LLMI_ROWS8(D_, NT_) \
-  (held == HELD_INT8 ? launch_rows8<D_, NT_, HELD_INT8>(p, n_entries, grid, stream) : launch_rows8<D_, NT_, HELD_E4M3>(p, n_entries, grid, stream))
-  if (head_dim == 64) return nt == 1 ? LLMI_ROWS8(64, 1) : nt == 2 ? LLMI_ROWS8(64, 2) : LLMI_ROWS8(64, 4);
-  return nt == 1 ? LLMI_ROWS8(128, 1) : LLMI_ROWS8(128, 2);
+  const int n_entries = n_seqs * tiles, grid = rw8_grid((long)n_entries * n_kv_heads * table_pages);
+#define LLMI_ROWS8(D_, NT_, T_) \
+  (held == HELD_INT8 ? launch_rows8<D_, NT_, HELD_INT8, T_>(p, n_entries, grid, stream) : launch_rows8<D_, NT_, HELD_E4M3, T_>(p, n_entries, grid, stream))
+  if (dtype == LLMI_DTYPE_F32) return head_dim == 128 ? LLMI_ROWS8(128, 1, float) : nt == 1 ? LLMI_ROWS8(64, 1, float) : LLMI_ROWS8(64, 2, float);
+  if (head_dim == 64) return nt == 1 ? LLMI_ROWS8(64, 1, __nv_bfloat16) : nt == 2 ? LLMI_ROWS8(64, 2, __nv_bfloat16) : LLMI_ROWS8(64, 4, __nv_bfloat16);
+  return nt == 1 ? LLMI_ROWS8(128, 1, __nv_bfloat16) : LLMI_ROWS8(128, 2, __nv_bfloat16);
 #undef LLMI_ROWS8
 }

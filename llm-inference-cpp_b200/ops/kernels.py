@@ -187,7 +187,7 @@ def lib():
         l.llmi_attention_prefill_tc.argtypes = [P, L, L, P, L, P, P, L, P, I, P, P, I, I, I, I, I, F, I, I, I, P, L, P, I, P, I, P, P, L, P, I, P, L, P, P, P, I, I, I, P, P]
         l.llmi_rope_store8.argtypes = [I, I, P, L, P, L, P, I, P, P, P, I, I, I, P, P, P, P, I, I, I, I, I, I, P]
         l.llmi_attention_any8.argtypes = [I, I, P, L, P, L, P, P, P, P, P, P, P, I, I, I, I, I, I, I, I, F, I, P]
-        l.llmi_attention_rows8.argtypes = [I, P, L, P, L, P, P, P, P, P, P, P, I, I, I, I, I, I, I, I, F, I, P, L, P, L, P]
+        l.llmi_attention_rows8.argtypes = [I, I, P, L, P, L, P, P, P, P, P, P, P, I, I, I, I, I, I, I, I, F, I, P, L, P, L, P]
         _configured = True
     return l
 
@@ -2207,9 +2207,9 @@ _sizes8: dict = {}
 _kept8: dict = {}
 
 
-def _rows8_sizes(n_seqs: int, max_q: int, n_heads: int, n_kv_heads: int, head_dim: int, table_pages: int) -> tuple | None:
+def _rows8_sizes(dtype: int, n_seqs: int, max_q: int, n_heads: int, n_kv_heads: int, head_dim: int, table_pages: int) -> tuple | None:
     """(floats of scratch, tickets) that attention_rows8 needs, None where it does not take the sizes."""
-    key = (n_seqs, max_q, n_heads, n_kv_heads, head_dim, table_pages)
+    key = (dtype, n_seqs, max_q, n_heads, n_kv_heads, head_dim, table_pages)
     if key not in _sizes8:
         floats, ints = c_long(0), c_long(0)
         rc = lib().llmi_attention_rows8_workspace(*map(c_int, key), ctypes.byref(floats), ctypes.byref(ints))
@@ -2236,24 +2236,25 @@ def _workspace8(q: torch.Tensor, rt, n_floats: int, n_ints: int) -> tuple:
 
 def _aligned8(q, out, k: Rows8, v: Rows8) -> bool:
     return ((q.data_ptr() | out.data_ptr() | k.codes.data_ptr() | v.codes.data_ptr() | k.scales.data_ptr() | v.scales.data_ptr()) % 16 == 0
-            and q.stride(0) % 8 == 0 and out.stride(0) % 8 == 0)
+            and q.stride(0) * q.element_size() % 16 == 0 and out.stride(0) * out.element_size() % 16 == 0)
 
 
 def attention_rows8(q: torch.Tensor, out: torch.Tensor, k: Rows8, v: Rows8, seq_q_start, seq_kv_len, max_q: int, seq_pages, n_heads: int,
                     n_kv_heads: int, head_dim: int, scale: float, window: int = 0, rt=None) -> None:
-    """:func:`attention8` by the kernel for few query rows a sequence (bf16, head size 64 or 128): ``seq_q_start`` [sequences + 1],
+    """:func:`attention8` by the kernel for few query rows a sequence (head size 64 or 128): ``seq_q_start`` [sequences + 1],
     ``seq_kv_len`` [sequences], ``max_q`` the most tokens that a sequence brings."""
     name = "attention_rows8"
     held = _check8(name, q, k, v, seq_pages, n_heads, n_kv_heads, head_dim, (out, seq_q_start, seq_kv_len))
     S, P = seq_pages.shape
-    _refuse(name, q.dtype != torch.bfloat16 or out.dtype != torch.bfloat16, "takes bf16 only")
+    _refuse(name, out.dtype != q.dtype, "out must have q's type")
     _check_index(name, "seq_q_start", seq_q_start, S + 1)
     _check_index(name, "seq_kv_len", seq_kv_len, S)
-    sizes = _rows8_sizes(S, max_q, n_heads, n_kv_heads, head_dim, P)
+    dtype = _dtype_code(q)
+    sizes = _rows8_sizes(dtype, S, max_q, n_heads, n_kv_heads, head_dim, P)
     _refuse(name, sizes is None, "a size is out of the range this kernel takes")
     slots, tickets = _workspace8(q, rt, *sizes)
     _check(name, lib().llmi_attention_rows8(
-        held, q.data_ptr(), q.stride(0), out.data_ptr(), out.stride(0), k.codes.data_ptr(), k.scales.data_ptr(), v.codes.data_ptr(),
+        dtype, held, q.data_ptr(), q.stride(0), out.data_ptr(), out.stride(0), k.codes.data_ptr(), k.scales.data_ptr(), v.codes.data_ptr(),
         v.scales.data_ptr(), seq_q_start.data_ptr(), seq_kv_len.data_ptr(), seq_pages.data_ptr(), seq_pages.stride(0), P, S, k.codes.shape[0],
         max_q, n_heads, n_kv_heads, head_dim, scale, window, slots.data_ptr(), slots.numel(), tickets.data_ptr(), tickets.numel(), _stream8(q)))
 
@@ -2293,8 +2294,8 @@ def attention8(q: torch.Tensor, out: torch.Tensor, k: Rows8, v: Rows8, ctx, seq_
         rope_store8(q, rotated, inv_freq, rotary_dim, ctx.tok_seq, ctx.tok_pos, seq_pages, k, v, n_heads, n_kv_heads, head_dim, write_kv)
         q = rotated
     max_q = _most_new(ctx)
-    if (q.dtype == torch.bfloat16 and head_dim in (64, 128) and _aligned8(q, out, k, v)
-            and _rows8_sizes(seq_pages.shape[0], max_q, n_heads, n_kv_heads, head_dim, seq_pages.shape[1]) is not None):
+    if (head_dim in (64, 128) and _aligned8(q, out, k, v)
+            and _rows8_sizes(_dtype_code(q), seq_pages.shape[0], max_q, n_heads, n_kv_heads, head_dim, seq_pages.shape[1]) is not None):
         attention_rows8(q, out, k, v, ctx.seq_q_start, ctx.seq_kv_len, max_q, seq_pages, n_heads, n_kv_heads, head_dim, scale, window, rt)
         return
     attention_any8(q, out, k, v, ctx.tok_seq, ctx.tok_pos, seq_pages, n_heads, n_kv_heads, head_dim, scale, window)

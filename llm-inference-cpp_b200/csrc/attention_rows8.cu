@@ -717,7 +717,7 @@ template <int D, int NT, int HELD, typename T> int launch_rows8(const Rows8Param
   // no more blocks than are resident: many entries' table may leave room for one a SM only (228 KB; a block's own 1 KB and its statics)
   const int fit = (int)((228 << 10) / (smem + 1280));
   const int resident = min(C::BLOCKS, max(1, fit)) * sm_count();
-  static const Rw8Cut cut = {getenv("RW8_FRONT") ? atoi(getenv("RW8_FRONT")) : 2, getenv("RW8_LEAST") ? atoi(getenv("RW8_LEAST")) : 1024 / D, getenv("RW8_NEAR") ? atoi(getenv("RW8_NEAR")) : 512 / D};
+  const Rw8Cut cut = {4, 1024 / D, 512 / D};
   return launch_pdl(PDL_ATTENTION, kernel, (unsigned)min(grid, resident), RW8_WARPS * 32, smem, stream, p, n_entries, cut);
 }
 

@@ -1,0 +1,621 @@
+// Attention of prompts over the paged cache held in 8 bits (rows8.cuh) on the 5th-generation tensor cores (tcgen05), bf16 queries,
+// head size 64 or 128.  For a row at position p of kv head g, over the keys j of its sequence it sees:
+//     s_j = scale * k_scale[j] * (q . k_code[j]),   w = softmax(s),   out = sum_j w_j * v_scale[j] * v_code[j]
+// (reference loop: src/model/transformer.cpp:263-282.)
+//
+// A block takes 256 query rows of one sequence and kv head — tokens times the heads of the group, token by token, so that a page
+// serves the whole group — as two tiles of 128 rows, and walks the pages (64 keys) that they see:
+//
+//   raw pages     one thread copies a page's codes and scales (4 bulk copies) into a ring
+//   codes -> fp16 four warps make K' = code * (k_scale / kmax) and V' = code * (v_scale / vmax) of a page, kmax and vmax its largest
+//                 scales, rounded to fp16 once (half a step is 2^-11 of a number; a bf16 cache's is 2^-8), in the swizzled layout
+//                 that the products read; so the scales cost the softmax nothing per key: kmax joins its scale, log2 vmax its offset.
+//                 (A page whose scales are more than 2^12 apart would lose bits of its small rows, which may be all that a query
+//                 sees: there K' and V' are the codes themselves and the softmax takes each key's scales.)
+//   S = Q' K'^T   tcgen05.mma, Q' the queries divided by a power of two per row (fp16, exact but for entries 2^-14 of the largest)
+//   softmax       a thread owns a row: tcgen05.ld, mask, maximum, exp2, sum; P = 2^(s + log2 vmax - m) goes back to tensor memory
+//                 as fp16 over the S it has read; the sum of w is that of P / vmax
+//   O += P V'     tcgen05.mma with A in tensor memory, accumulating in fp32; m follows the running maximum (of s + log2 vmax) only
+//                 when that has grown by more than 8, so O is rescaled a few times per row
+//
+// What bounds it: the exponentials at head size 64 (16 a clock and SM; 64 x 128 of them a page and tile, 512 clocks), the products at
+// 128.  Two tiles share a converted page: the conversion, 2 x 64 x D codes, costs a sixth of their softmax.
+//
+// A step of few blocks leaves SMs idle: then a block's pages are cut into parts, each a block of its own that leaves (m, sum, O) per
+// row in a workspace; a second kernel joins them in order.  Waits are bounded (sm100.cuh).
+#include <math.h>
+
+#include "rows8.cuh"
+#include "tc_common.cuh"
+
+namespace llmi {
+
+constexpr int P8_ROWS = 256, P8_TILE = 128;
+constexpr int P8_THREADS = 14 * 32;       // copies, products, 2 x 4 softmax warps, 4 converting warps
+constexpr int P8_TMEM = 512;              // per tile of rows 256 columns: S of even and odd pages (64 each), O (D)
+constexpr float P8_LAZY = 8.0f;
+constexpr float P8_APART = 2.44140625e-4f;             // 2^-12
+constexpr float P8_TINY = 7.888609052210118e-31f;      // 2^-100: smaller scales of a page count as this
+
+struct Prompt8Params {
+  const __nv_bfloat16* q;
+  long ldq;
+  __nv_bfloat16* out;
+  long ldo;
+  const uint8_t* k_codes;
+  const float* k_scales;
+  const uint8_t* v_codes;
+  const float* v_scales;
+  const int32_t* seq_q_start;   // [n_seqs + 1]
+  const int32_t* seq_kv_len;    // [n_seqs]
+  Paged8 kv;
+  int n_seqs, group;
+  float scale_log2;
+  int window;
+  int parts, part_pages;        // most parts of a block's pages; the least pages of a part
+  float* partials;              // [block][kv head][part][256][D + 2] when parts > 1
+  int* error_flag;
+};
+
+template <int D>
+struct P8Cfg {
+  static constexpr int SUBS = D / 64;                     // 64-column sub-tiles of a row
+  static constexpr int Q_TILE = SUBS * P8_TILE * 128;     // bytes of a tile's queries
+  static constexpr int KV_TILE = SUBS * PAGE8 * 128;      // bytes of a page's K' or V'
+  static constexpr int STAGE = 2 * KV_TILE, STAGES = 3;
+  static constexpr int RAW = 2 * PAGE8 * D + 2 * PAGE8 * 4, RAWS = D == 64 ? 5 : 3;
+  static constexpr int SMEM = 1024 + 2 * Q_TILE + STAGES * STAGE + RAWS * RAW + 256;
+};
+
+// Block b of the step's blocks of 256 rows, counted from the last block of the last sequence backwards (late blocks see more keys and
+// come first).  A whole warp calls this.
+struct P8Block {
+  int seq, q_start, row0, rows, pos0, first, last, lo, pg_first, n_pages;      // rows 0: there is no such block
+};
+__device__ __forceinline__ P8Block prompt8_block(const Prompt8Params& p, int b) {
+  const int lane = threadIdx.x & 31;
+  P8Block d;
+  d.rows = d.n_pages = 0;
+  for (int s0 = p.n_seqs - 1; s0 >= 0; s0 -= 32) {
+    const int s = s0 - lane;
+    int n = 0;
+    if (s >= 0 && p.seq_kv_len[s] > 0) n = ((p.seq_q_start[s + 1] - p.seq_q_start[s]) * p.group + P8_ROWS - 1) / P8_ROWS;
+    int x = n;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const int y = __shfl_up_sync(0xffffffffu, x, o);
+      if (lane >= o) x += y;
+    }
+    const int all = __shfl_sync(0xffffffffu, x, 31);
+    if (b < all) {
+      const int src = __ffs(__ballot_sync(0xffffffffu, x > b)) - 1;
+      d.seq = s0 - src;
+      const int mb = __shfl_sync(0xffffffffu, x, src) - 1 - b;
+      d.q_start = p.seq_q_start[d.seq];
+      const int q_len = p.seq_q_start[d.seq + 1] - d.q_start, kv_len = p.seq_kv_len[d.seq];
+      d.row0 = mb * P8_ROWS;
+      d.rows = min(P8_ROWS, q_len * p.group - d.row0);
+      d.pos0 = kv_len - q_len;
+      d.first = d.pos0 + d.row0 / p.group;
+      d.last = d.pos0 + (d.row0 + d.rows - 1) / p.group;
+      d.lo = (p.window > 0 && d.first - p.window + 1 > 0) ? d.first - p.window + 1 : 0;
+      d.pg_first = d.lo / PAGE8;
+      if (d.last >= 0) d.n_pages = d.last / PAGE8 - d.pg_first + 1;
+      return d;
+    }
+    b -= all;
+  }
+  return d;
+}
+// Its pages in parts of equal size: (parts, pages of one).
+__device__ __forceinline__ int2 prompt8_parts(const Prompt8Params& p, int n_pages) {
+  const int n = max(1, min(p.parts, n_pages / p.part_pages));
+  const int per = max(1, (n_pages + n - 1) / n);
+  return make_int2(max(1, (n_pages + per - 1) / per), per);
+}
+
+// 16 columns of this thread's TMEM lane; no wait
+__device__ __forceinline__ void p8_ld16(uint32_t taddr, float* v) {
+  uint32_t r[16];
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15}, [%16];"
+      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]),
+        "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
+      : "r"(taddr));
+#pragma unroll
+  for (int i = 0; i < 16; ++i) v[i] = __uint_as_float(r[i]);
+}
+__device__ __forceinline__ void p8_ld_wait() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
+__device__ __forceinline__ void p8_st16(uint32_t taddr, const uint32_t* v) {
+  asm volatile(
+      "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16};"
+      ::"r"(taddr), "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7]), "r"(v[8]), "r"(v[9]),
+        "r"(v[10]), "r"(v[11]), "r"(v[12]), "r"(v[13]), "r"(v[14]), "r"(v[15])
+      : "memory");
+}
+__device__ __forceinline__ void p8_st_wait() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
+__device__ __forceinline__ void p8_mma_ts(uint32_t d, uint32_t a_tmem, uint64_t b, uint32_t idesc, uint32_t acc) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}"
+      ::"r"(d), "r"(a_tmem), "l"(b), "r"(idesc), "r"(acc)
+      : "memory");
+}
+__device__ __forceinline__ uint32_t half2_bits(__half2 h) { return *reinterpret_cast<uint32_t*>(&h); }
+
+template <int D, int HELD>
+__global__ void __launch_bounds__(P8_THREADS, 1) attention_prompt8_kernel(Prompt8Params p) {
+  using C = P8Cfg<D>;
+  constexpr int SUBS = C::SUBS, STAGES = C::STAGES, RAWS = C::RAWS;
+  extern __shared__ uint8_t smem_raw[];
+  const uint32_t base = (smem_u32(smem_raw) + 1023u) & ~1023u;
+  uint8_t* const base_p = smem_raw + (base - smem_u32(smem_raw));
+  const uint32_t q_smem = base, kv_smem = q_smem + 2 * C::Q_TILE, raw_smem = kv_smem + STAGES * C::STAGE, bars = raw_smem + RAWS * C::RAW;
+  const uint32_t q_full = bars, tmem_slot = bars + 248;
+  auto raw_full = [&](int s) { return bars + 8u * (1 + s); };
+  auto raw_empty = [&](int s) { return bars + 8u * (1 + RAWS + s); };
+  auto kv_full = [&](int s) { return bars + 8u * (1 + 2 * RAWS + s); };
+  auto kv_empty = [&](int s) { return bars + 8u * (1 + 2 * RAWS + STAGES + s); };
+  auto s_full = [&](int tile, int b) { return bars + 8u * (1 + 2 * RAWS + 2 * STAGES + 2 * tile + b); };
+  auto p_ready = [&](int tile, int b) { return bars + 8u * (5 + 2 * RAWS + 2 * STAGES + 2 * tile + b); };
+  auto o_done = [&](int tile) { return bars + 8u * (9 + 2 * RAWS + 2 * STAGES + tile); };
+  static_assert(8 * (11 + 2 * RAWS + 2 * STAGES) <= 248, "barriers fit");
+  __shared__ int s_known[RAWS];                          // the raw page is one of the pool
+  __shared__ float s_page[STAGES][4];                    // kmax, log2 vmax, 1 / vmax
+  __shared__ uint32_t s_poison[STAGES][2];               // keys whose values are no numbers
+  __shared__ int s_wide[STAGES];                         // the page's scales are far apart: its keys' own
+  __shared__ float s_key[STAGES][2][PAGE8];              // k_scale, log2 v_scale
+
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int kvh = blockIdx.x, G = p.group, Hkv = p.kv.n_kv_heads;
+  const int blk = blockIdx.y / p.parts, part = blockIdx.y % p.parts;
+  pdl_wait();
+  const P8Block d = prompt8_block(p, blk);
+  if (d.rows <= 0) return;
+  const int2 cut = prompt8_parts(p, d.n_pages);
+  if (part >= cut.x) return;
+  const int v0 = part * cut.y, n_pg = min(cut.y, d.n_pages - v0);
+  if (n_pg <= 0) return;                                 // (positions below 0 only: nothing to see)
+  const int pg0 = d.pg_first + v0;                       // this part's first page
+  // pages of this part that a tile's rows see the first key of
+  int n_tile[2];
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {
+    const int rows = min(P8_TILE, d.rows - i * P8_TILE);
+    n_tile[i] = 0;
+    if (rows > 0) {
+      const int last = d.pos0 + (d.row0 + i * P8_TILE + rows - 1) / G;
+      if (last >= 0) n_tile[i] = max(0, min(n_pg, last / PAGE8 - pg0 + 1));
+    }
+  }
+
+  if (threadIdx.x == 0) {
+    mbar_init(q_full, 8);
+    for (int s = 0; s < RAWS; ++s) mbar_init(raw_full(s), 1), mbar_init(raw_empty(s), 4);
+    for (int s = 0; s < STAGES; ++s) mbar_init(kv_full(s), 4), mbar_init(kv_empty(s), 1);
+    for (int i = 0; i < 2; ++i) {
+      for (int b = 0; b < 2; ++b) mbar_init(s_full(i, b), 1), mbar_init(p_ready(i, b), 4);
+      mbar_init(o_done(i), 1);
+    }
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+  }
+  if (warp == 1) {
+    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(tmem_slot), "r"(P8_TMEM));
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::);
+  }
+  asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+  __syncthreads();
+  asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+  uint32_t tmem;
+  asm volatile("ld.shared.u32 %0, [%1];" : "=r"(tmem) : "r"(tmem_slot));
+  pdl_launch_dependents();      // (not ahead of the tensor memory: a kernel behind this one could take it and wait for this block)
+
+  if (warp == 0) {
+    if (lane == 0) {
+      // ---- raw pages ----
+      const int32_t* pages = p.kv.seq_pages + (size_t)d.seq * p.kv.pages_stride;
+      for (int j = 0; j < n_pg; ++j) {
+        const int s = j % RAWS, at = pg0 + j;
+        const int page = at < p.kv.table_pages ? pages[at] : -1;
+        if (j >= RAWS && !mbar_wait(raw_empty(s), ((j / RAWS) - 1) & 1, p.error_flag, 101)) break;
+        const bool known = (unsigned)page < (unsigned)p.kv.n_pages;
+        s_known[s] = known;
+        if (known) {
+          const uint32_t st = raw_smem + s * C::RAW;
+          const size_t row = ((size_t)page * Hkv + kvh) * PAGE8;
+          mbar_expect_tx(raw_full(s), C::RAW);
+          bulk_load(st, p.k_codes + row * D, PAGE8 * D, raw_full(s));
+          bulk_load(st + PAGE8 * D, p.v_codes + row * D, PAGE8 * D, raw_full(s));
+          bulk_load(st + 2 * PAGE8 * D, p.k_scales + row, PAGE8 * 4, raw_full(s));
+          bulk_load(st + 2 * PAGE8 * D + PAGE8 * 4, p.v_scales + row, PAGE8 * 4, raw_full(s));
+        } else {
+          mbar_arrive(raw_full(s));
+        }
+      }
+    }
+  } else if (warp == 1) {
+    if (lane == 0) {
+      // ---- products ----
+      // S: A = Q' (K-major), B = K' (K-major), 64 columns; O: A = P (tensor memory, 32 columns of fp16 pairs), B = V' (MN-major).
+      // MMAs of one thread run in issue order: S_{j+1} may be issued into the buffer that P_{j-1} lies in once O += P_{j-1} V_{j-1} was.
+      const uint32_t idesc_s = (1u << 4) | ((uint32_t)(64 >> 3) << 17) | ((uint32_t)(128 >> 4) << 24), idesc_o = idesc_s | (1u << 16);
+      auto issue_s = [&](int tile, int j) {
+        const uint32_t dst = tmem + 256u * tile + 64u * (j & 1);
+#pragma unroll
+        for (int k = 0; k < D / 16; ++k)
+          umma_bf16(dst, umma_desc(q_smem + tile * C::Q_TILE + (k / 4) * (P8_TILE * 128)) + 2 * (k % 4),
+                    umma_desc(kv_smem + (j % STAGES) * C::STAGE + (k / 4) * (PAGE8 * 128)) + 2 * (k % 4), idesc_s, k > 0);
+        umma_commit(s_full(tile, j & 1));
+      };
+      auto issue_o = [&](int tile, int j) {
+        const uint32_t a = tmem + 256u * tile + 64u * (j & 1), o = tmem + 256u * tile + 128u;
+        const uint32_t v = kv_smem + (j % STAGES) * C::STAGE + C::KV_TILE;
+#pragma unroll
+        for (int k = 0; k < 4; ++k)
+#pragma unroll
+          for (int u = 0; u < SUBS; ++u)
+            p8_mma_ts(o + 64u * u, a + 8u * k, umma_desc(v + u * (PAGE8 * 128)) + (uint64_t)(k * ((16 * 128) >> 4)), idesc_o, (j > 0 || k > 0) ? 1u : 0u);
+        umma_commit(o_done(tile));
+      };
+      bool ok = mbar_wait(q_full, 0, p.error_flag, 102);
+      for (int j = 0; j <= n_pg && ok; ++j) {
+        if (j < n_pg) {
+          ok = mbar_wait(kv_full(j % STAGES), (j / STAGES) & 1, p.error_flag, 103);
+          if (!ok) break;
+          asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+          for (int tile = 0; tile < 2; ++tile)
+            if (j < n_tile[tile]) issue_s(tile, j);
+        }
+        if (j >= 1) {
+          for (int tile = 0; tile < 2 && ok; ++tile) {
+            if (j - 1 >= n_tile[tile]) continue;
+            ok = mbar_wait(p_ready(tile, (j - 1) & 1), ((j - 1) >> 1) & 1, p.error_flag, 104);
+            if (!ok) break;
+            asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+            issue_o(tile, j - 1);
+          }
+          if (j - 1 + STAGES < n_pg) umma_commit(kv_empty((j - 1) % STAGES));      // (where the stage is filled again)
+        }
+      }
+    }
+  } else if (warp < 10) {
+    // ---- softmax and output: a thread a row ----
+    const int tile = (warp - 2) >> 2, quad = warp & 3;
+    const int r = tile * P8_TILE + quad * 32 + lane;               // row of the block; quad * 32 + lane is its TMEM lane
+    const int row = d.row0 + r, tok = row / G, head = kvh * G + row % G;
+    const bool row_ok = r < d.rows;
+    const int qpos = d.pos0 + (d.row0 + min(r, d.rows - 1)) / G;
+    const int pos_a = __shfl_sync(0xffffffffu, qpos, 0), pos_b = __shfl_sync(0xffffffffu, qpos, 31);      // the warp's first and last
+    // the row's queries, divided by a power of two above the largest
+    float row_fac;
+    {
+      const uint4* src = reinterpret_cast<const uint4*>(p.q + (size_t)(d.q_start + (row_ok ? tok : 0)) * p.ldq + (size_t)head * D);
+      float a = 0.f;
+#pragma unroll
+      for (int c = 0; c < D / 8; ++c) {
+        const uint4 raw = row_ok ? src[c] : make_uint4(0u, 0u, 0u, 0u);
+        const __nv_bfloat162* b = reinterpret_cast<const __nv_bfloat162*>(&raw);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const float2 f = __bfloat1622float2(b[i]);
+          a = fmaxf(a, fmaxf(fabsf(f.x), fabsf(f.y)));
+        }
+      }
+      int ex = 0;
+      if (a > 0.f && a <= FLT_MAX) ex = max(-100, (int)((__float_as_uint(a) >> 23) & 255) - 126);
+      float down = __uint_as_float((uint32_t)(127 - min(ex, 126)) << 23);
+      const float down2 = ex > 126 ? 1.f / (float)(1 << (ex - 126)) : 1.f;
+      if (p.scale_log2 < 0.f) down = -down;                        // the factor of the scores below is positive
+      row_fac = fmaxf(ldexpf(fabsf(p.scale_log2), ex), 1e-30f);    // (never quite 0: 0 times a masked key's -inf is no number)
+      const uint32_t at = q_smem + tile * C::Q_TILE + (quad * 32 + lane) * 128;
+#pragma unroll
+      for (int c = 0; c < D / 8; ++c) {
+        const uint4 raw = row_ok ? src[c] : make_uint4(0u, 0u, 0u, 0u);
+        const __nv_bfloat162* b = reinterpret_cast<const __nv_bfloat162*>(&raw);
+        uint32_t h[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const float2 f = __bfloat1622float2(b[i]);
+          h[i] = half2_bits(__floats2half2_rn(f.x * down * down2, f.y * down * down2));
+        }
+        asm volatile("st.shared.v4.u32 [%0], {%1, %2, %3, %4};"
+                     ::"r"(at + (c / 8) * (P8_TILE * 128) + (((c % 8) ^ (lane & 7)) << 4)), "r"(h[0]), "r"(h[1]), "r"(h[2]), "r"(h[3]) : "memory");
+      }
+      asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+      __syncwarp();
+      if (lane == 0) mbar_arrive(q_full);
+    }
+    const int n = n_tile[tile];
+    const uint32_t t_lane = (uint32_t)(quad * 32) << 16, t_tile = tmem + 256u * tile + t_lane, t_o = t_tile + 128u;
+    float m_run = -INFINITY, m_ref = -INFINITY, l_run = 0.f;       // of s + log2 vmax, base 2; the sum of 2^(s - m_ref)
+    bool ok = true;
+    for (int j = 0; j < n && ok; ++j) {
+      ok = mbar_wait(s_full(tile, j & 1), (j >> 1) & 1, p.error_flag, 105);
+      if (!ok) break;
+      asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+      const uint32_t t_s = t_tile + 64u * (j & 1);
+      float sc[64];
+#pragma unroll
+      for (int c = 0; c < 64; c += 16) p8_ld16(t_s + (uint32_t)c, sc + c);
+      const float to_log2 = s_wide[j % STAGES] ? 1.f : row_fac * s_page[j % STAGES][0], lv = s_page[j % STAGES][1], inv_v = s_page[j % STAGES][2];
+      const uint32_t bad0 = s_poison[j % STAGES][0], bad1 = s_poison[j % STAGES][1];
+      const bool wide = s_wide[j % STAGES] != 0;
+      const int key0 = (pg0 + j) * PAGE8;
+      p8_ld_wait();
+      if (wide) {                                                  // (kmax 1 / row_fac, vmax 1: the scores are final)
+#pragma unroll
+        for (int c = 0; c < 64; ++c) sc[c] = fmaf(sc[c], row_fac * s_key[j % STAGES][0][c], s_key[j % STAGES][1][c]);
+      }
+      if (key0 + PAGE8 - 1 > pos_a || (p.window > 0 && key0 <= pos_b - p.window)) {
+        const int a = p.window > 0 ? qpos - p.window + 1 - key0 : 0, b = qpos - key0;      // the keys a .. b of the page are seen
+#pragma unroll
+        for (int c = 0; c < 64; ++c)
+          if (c > b || c < a) sc[c] = -INFINITY;
+      }
+      float mx4[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+#pragma unroll
+      for (int c = 0; c < 64; c += 8)
+#pragma unroll
+        for (int u = 0; u < 4; ++u) mx4[u] = fmaxf(mx4[u], fmaxf(sc[c + 2 * u], sc[c + 2 * u + 1]));
+      const float top = fmaf(fmaxf(fmaxf(mx4[0], mx4[1]), fmaxf(mx4[2], mx4[3])), to_log2, lv);
+      m_run = fmaxf(m_run, top);
+      float corr = 1.f;
+      if (m_run > m_ref + P8_LAZY || m_ref == -INFINITY) {         // (both -inf: nothing seen yet)
+        corr = m_ref == -INFINITY ? 0.f : fast_exp2(m_ref - m_run);
+        if (m_ref != -INFINITY) l_run = rescale8(l_run, m_ref - m_run);
+        m_ref = m_run;
+      }
+      const float off = m_ref == -INFINITY ? 0.f : lv - m_ref;
+      float2 sum2[4] = {{0.f, 0.f}, {0.f, 0.f}, {0.f, 0.f}, {0.f, 0.f}};
+      const float2 scale2 = make_float2(to_log2, to_log2), off2 = make_float2(off, off);
+      uint32_t packed[32];
+#pragma unroll
+      for (int c = 0; c < 64; c += 2) {
+        const float2 x = __ffma2_rn(make_float2(sc[c], sc[c + 1]), scale2, off2);
+        const float2 e = make_float2(fast_exp2(x.x), fast_exp2(x.y));
+        sum2[(c >> 1) & 3] = __fadd2_rn(sum2[(c >> 1) & 3], e);
+        packed[c >> 1] = half2_bits(__floats2half2_rn(e.x, e.y));
+      }
+      // The sum of w is that of P / vmax, unless all of P is so small that it may have lost some of it (values far smaller than those of
+      // another page, zeros for instance, say nothing about their weights).
+      if (!__any_sync(0xffffffffu, wide || top < m_ref - 64.f)) {
+        const float2 s = __fadd2_rn(__fadd2_rn(sum2[0], sum2[1]), __fadd2_rn(sum2[2], sum2[3]));
+        l_run = fmaf(s.x + s.y, inv_v, l_run);
+      } else {
+#pragma unroll
+        for (int c = 0; c < 64; ++c) l_run += fast_exp2(fmaf(sc[c], to_log2, off) - (wide ? s_key[j % STAGES][1][c] : lv));
+      }
+      if (bad0 | bad1) {                                           // values that are no numbers: for the rows that see them
+        const int a = p.window > 0 ? max(qpos - p.window + 1 - key0, 0) : 0, b = min(qpos - key0, 63);
+        const uint64_t bad = ((uint64_t)bad1 << 32) | bad0;
+        if (a <= b && ((bad >> a) << (63 - (b - a)))) l_run = __int_as_float(0x7fffffff);
+      }
+      if (j >= 1) {
+        // (waited for on every page: a wait on a phase's parity is right only for a thread at most one phase behind)
+        ok = mbar_wait(o_done(tile), (j - 1) & 1, p.error_flag, 106);
+        if (!ok) break;
+        if (__any_sync(0xffffffffu, corr != 1.f)) {
+          asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+#pragma unroll
+          for (int c = 0; c < D; c += 16) {
+            float t[16];
+            uint32_t u[16];
+            p8_ld16(t_o + (uint32_t)c, t);
+            p8_ld_wait();
+#pragma unroll
+            for (int e = 0; e < 16; ++e) u[e] = __float_as_uint(t[e] * corr);
+            p8_st16(t_o + (uint32_t)c, u);
+          }
+        }
+      }
+      p8_st16(t_s, packed);
+      p8_st16(t_s + 16u, packed + 16);
+      p8_st_wait();
+      asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+      __syncwarp();
+      if (lane == 0) mbar_arrive(p_ready(tile, j & 1));
+    }
+    // (`fine` is the same in all lanes: the TMEM loads are the whole warp's)
+    const bool fine = __all_sync(0xffffffffu, ok && (n == 0 || mbar_wait(o_done(tile), (n - 1) & 1, p.error_flag, 107)));
+    asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+    if (fine) {
+      if (cut.x > 1) {
+        float* slot = p.partials + (((size_t)blk * Hkv + kvh) * p.parts + part) * (P8_ROWS * (D + 2));
+        if (row_ok) slot[r] = m_ref, slot[P8_ROWS + r] = l_run;
+        float* dst = slot + 2 * P8_ROWS + (size_t)r * D;
+#pragma unroll 1
+        for (int c = 0; c < D; c += 16) {
+          float o[16];
+          if (n > 0) p8_ld16(t_o + (uint32_t)c, o), p8_ld_wait();
+#pragma unroll
+          for (int e = 0; e < 16; e += 4)
+            if (row_ok) *reinterpret_cast<float4*>(dst + c + e) = n > 0 ? make_float4(o[e], o[e + 1], o[e + 2], o[e + 3]) : make_float4(0.f, 0.f, 0.f, 0.f);
+        }
+      } else {
+        const float inv = l_run == 0.f ? 0.f : 1.f / l_run;
+        __nv_bfloat16* dst = p.out + (size_t)(d.q_start + tok) * p.ldo + (size_t)head * D;
+#pragma unroll 1
+        for (int c = 0; c < D; c += 16) {
+          float o[16];
+          if (n > 0) p8_ld16(t_o + (uint32_t)c, o), p8_ld_wait();
+          uint32_t w[8];
+#pragma unroll
+          for (int e = 0; e < 8; ++e) {
+            // (without a page, or with weights that are all zero, the row sees nothing)
+            __nv_bfloat162 h = __floats2bfloat162_rn(n > 0 ? o[2 * e] * inv : 0.f, n > 0 ? o[2 * e + 1] * inv : 0.f);
+            w[e] = *reinterpret_cast<uint32_t*>(&h);
+          }
+          if (row_ok) {
+            *reinterpret_cast<uint4*>(dst + c) = make_uint4(w[0], w[1], w[2], w[3]);
+            *reinterpret_cast<uint4*>(dst + c + 8) = make_uint4(w[4], w[5], w[6], w[7]);
+          }
+        }
+      }
+    }
+  } else {
+    // ---- codes to fp16 ----
+    const int id = threadIdx.x - 10 * 32;                          // 0 .. 127
+    constexpr int UPR = D / 16, UNITS = PAGE8 * UPR / 128;         // 16-byte pieces of a row, and of a tile per thread
+    for (int j = 0; j < n_pg; ++j) {
+      const int s = j % RAWS, st = j % STAGES;
+      if (!mbar_wait(raw_full(s), (j / RAWS) & 1, p.error_flag, 108)) break;
+      if (j >= STAGES && !mbar_wait(kv_empty(st), ((j / STAGES) - 1) & 1, p.error_flag, 109)) break;
+      const uint8_t* raw = base_p + (raw_smem - base) + s * C::RAW;
+      const float* ks = reinterpret_cast<const float*>(raw + 2 * PAGE8 * D);
+      const float* vs = ks + PAGE8;
+      const bool known = s_known[s] != 0;
+      const int a = max(d.lo - (pg0 + j) * PAGE8, 0), b = min(d.last - (pg0 + j) * PAGE8, 63);      // rows that some query sees
+      // the page's largest scales (of rows that are numbers) and its rows that are not
+      float km = 0.f, vm = 0.f, kn = INFINITY, vn = INFINITY;              // largest, and least but zeros
+      uint32_t bad[2];
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        const int r = lane + 32 * h;
+        const bool in = r >= a && r <= b;
+        const float x = in && known ? ks[r] : 0.f, y = in ? (known ? vs[r] : __int_as_float(0x7fffffff)) : 0.f;
+        km = fmaxf(km, finite8(x) ? fabsf(x) : 0.f);
+        vm = fmaxf(vm, finite8(y) ? fabsf(y) : 0.f);
+        if (x != 0.f) kn = fminf(kn, fabsf(x));
+        if (y != 0.f) vn = fminf(vn, fabsf(y));
+        bad[h] = __ballot_sync(0xffffffffu, !finite8(y));
+      }
+      km = fmaxf(warp_max(km), P8_TINY);
+      vm = fmaxf(warp_max(vm), P8_TINY);
+      const bool wide = __any_sync(0xffffffffu, kn < km * P8_APART || vn < vm * P8_APART);
+      if (id == 0) {
+        s_page[st][0] = km;
+        s_page[st][1] = wide ? 0.f : log2f(vm);
+        s_page[st][2] = 1.f / vm;
+        s_poison[st][0] = bad[0];
+        s_poison[st][1] = bad[1];
+        s_wide[st] = wide;
+      }
+      if (wide) {
+        if (id < PAGE8) {
+          const bool in = id >= a && id <= b && known;
+          const float y = in ? fmaxf(vs[id], P8_TINY) : 1.f;               // (a NaN's values are zeros here: its bit is in s_poison)
+          s_key[st][0][id] = in ? ks[id] : 0.f;
+          s_key[st][1][id] = log2f(y);
+        }
+      }
+      const uint32_t k_dst = kv_smem + st * C::STAGE, v_dst = k_dst + C::KV_TILE;
+      const float k_inv = 1.f / km, v_inv = 1.f / vm;
+#pragma unroll
+      for (int i = 0; i < UNITS; ++i) {
+        const int x = id + 128 * i, r = x / UPR, u = x % UPR;
+        const bool in = r >= a && r <= b && known;
+        const uint4 kw = *reinterpret_cast<const uint4*>(raw + x * 16), vw = *reinterpret_cast<const uint4*>(raw + PAGE8 * D + x * 16);
+        // the row's factor as the sum of two fp16 numbers, so that a product is rounded once
+        const float kf = in ? (wide ? 1.f : ks[r] * k_inv) : 0.f, vf = in && finite8(vs[r]) ? vs[r] * (wide ? 1.f / fmaxf(vs[r], P8_TINY) : v_inv) : 0.f;
+        const __half kh = __float2half_rn(kf), vh = __float2half_rn(vf);
+        const __half2 kh2 = __half2half2(kh), vh2 = __half2half2(vh);
+        const __half2 kl2 = __half2half2(__float2half_rn(kf - __half2float(kh))), vl2 = __half2half2(__float2half_rn(vf - __half2float(vh)));
+        const bool zero_v = !(in && finite8(vs[r])), zero_k = !in;          // (codes there may be no numbers)
+        const uint32_t* kp = &kw.x;
+        const uint32_t* vp = &vw.x;
+        const uint32_t at = (u / 4) * (PAGE8 * 128) + r * 128;
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {                                       // eight codes: 16 bytes of fp16
+          uint32_t kx[4], vx[4];
+#pragma unroll
+          for (int w = 0; w < 2; ++w) {
+            const uint32_t kc = zero_k ? 0u : kp[2 * h + w], vc = zero_v ? 0u : vp[2 * h + w];
+            __half2 k0, k1, v0h, v1h;
+            k0 = halves8<HELD>(kc & 0xffffu), k1 = halves8<HELD>(kc >> 16);
+            v0h = halves8<HELD>(vc & 0xffffu), v1h = halves8<HELD>(vc >> 16);
+            kx[2 * w] = half2_bits(__hfma2(k0, kh2, __hmul2(k0, kl2)));
+            kx[2 * w + 1] = half2_bits(__hfma2(k1, kh2, __hmul2(k1, kl2)));
+            vx[2 * w] = half2_bits(__hfma2(v0h, vh2, __hmul2(v0h, vl2)));
+            vx[2 * w + 1] = half2_bits(__hfma2(v1h, vh2, __hmul2(v1h, vl2)));
+          }
+          const uint32_t o = at + (((2 * (u % 4) + h) ^ (r & 7)) << 4);
+          asm volatile("st.shared.v4.u32 [%0], {%1, %2, %3, %4};" ::"r"(k_dst + o), "r"(kx[0]), "r"(kx[1]), "r"(kx[2]), "r"(kx[3]) : "memory");
+          asm volatile("st.shared.v4.u32 [%0], {%1, %2, %3, %4};" ::"r"(v_dst + o), "r"(vx[0]), "r"(vx[1]), "r"(vx[2]), "r"(vx[3]) : "memory");
+        }
+      }
+      asm volatile("fence.proxy.async.shared::cta;" ::: "memory");        // the products read what was written, and the raw page may be overwritten
+      __syncwarp();
+      if (lane == 0) {
+        mbar_arrive(kv_full(st));
+        mbar_arrive(raw_empty(s));
+      }
+    }
+  }
+  asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+  __syncthreads();
+  if (warp == 1) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(P8_TMEM));
+}
+
+// The parts of a block's rows, in order: a warp a row.
+template <int D>
+__global__ void __launch_bounds__(256) prompt8_join_kernel(Prompt8Params p) {
+  pdl_wait();
+  pdl_launch_dependents();
+  const int kvh = blockIdx.x, blk = blockIdx.y / 8, lane = threadIdx.x & 31, G = p.group;
+  const P8Block d = prompt8_block(p, blk);
+  const int2 cut = prompt8_parts(p, d.n_pages);
+  if (d.rows <= 0 || d.n_pages <= 0 || cut.x <= 1) return;
+  for (int r = (blockIdx.y % 8) * 8 + (threadIdx.x >> 5); r < d.rows; r += 64) {
+    const float* slot = p.partials + ((size_t)blk * p.kv.n_kv_heads + kvh) * p.parts * (P8_ROWS * (D + 2));
+    const size_t step = P8_ROWS * (D + 2);
+    float m = -INFINITY, l = 0.f, o[D / 32];
+    for (int z = lane; z < cut.x; z += 32) m = fmaxf(m, slot[z * step + r]);
+    m = warp_max(m);
+#pragma unroll
+    for (int i = 0; i < D / 32; ++i) o[i] = 0.f;
+#pragma unroll 4
+    for (int z = 0; z < cut.x; ++z) {
+      const float mz = slot[z * step + r], f = mz == -INFINITY ? 1.f : fast_exp2(mz - m);
+      l += rescale8(slot[z * step + P8_ROWS + r], mz == -INFINITY ? 0.f : mz - m);
+      const float* src = slot + z * step + 2 * P8_ROWS + (size_t)r * D + lane * (D / 32);
+#pragma unroll
+      for (int i = 0; i < D / 32; ++i) o[i] = fmaf(src[i], f, o[i]);
+    }
+    const int row = d.row0 + r;
+    const float inv = l == 0.f ? 0.f : 1.f / l;
+    __nv_bfloat162* dst = reinterpret_cast<__nv_bfloat162*>(p.out + (size_t)(d.q_start + row / G) * p.ldo + (size_t)(kvh * G + row % G) * D + lane * (D / 32));
+#pragma unroll
+    for (int i = 0; i < D / 32; i += 2) dst[i / 2] = __floats2bfloat162_rn(o[i] * inv, o[i + 1] * inv);
+  }
+}
+
+template <int D, int HELD> int launch_prompt8(const Prompt8Params& p, int n_blocks, cudaStream_t stream) {
+  static PerDevice<bool> configured;
+  if (!configured.here()) {
+    if (cudaFuncSetAttribute(attention_prompt8_kernel<D, HELD>, cudaFuncAttributeMaxDynamicSharedMemorySize, P8Cfg<D>::SMEM) != cudaSuccess)
+      return LLMI_ERR_LAUNCH;
+    configured.here() = true;
+  }
+  const int rc = launch_pdl(PDL_ATTENTION, attention_prompt8_kernel<D, HELD>, dim3((unsigned)p.kv.n_kv_heads, (unsigned)(n_blocks * p.parts)), P8_THREADS,
+                            P8Cfg<D>::SMEM, stream, p);
+  if (rc != LLMI_OK || p.parts <= 1) return rc;
+  return launch_pdl(PDL_ATTENTION, prompt8_join_kernel<D>, dim3((unsigned)p.kv.n_kv_heads, (unsigned)(n_blocks * 8)), 256, 0, stream, p);
+}
+
+}  // namespace llmi
+
+using namespace llmi;
+
+// `n_blocks`: at least the blocks of 256 rows over all sequences (n_tokens * group / 256 + n_seqs are enough).  `parts` > 1: a block's
+// pages in up to so many parts of at least `part_pages` pages, over `partials` of n_blocks * n_kv_heads * parts * 256 * (head_dim + 2)
+// floats.
+LLMI_EXPORT int llmi_attention_prompt8(int held, const void* q, long ldq, void* out, long ldo, const void* k_codes, const float* k_scales,
+                                       const void* v_codes, const float* v_scales, const int32_t* seq_q_start, const int32_t* seq_kv_len,
+                                       const int32_t* seq_pages, int pages_stride, int table_pages, int n_seqs, int n_pages, int n_blocks,
+                                       int n_heads, int n_kv_heads, int head_dim, float scale, int window, int parts, int part_pages,
+                                       float* partials, long n_floats, int* error_flag, cudaStream_t stream) {
+  if (n_seqs <= 0 || n_blocks <= 0 || n_kv_heads <= 0 || n_heads <= 0 || n_heads % n_kv_heads || (head_dim != 64 && head_dim != 128) ||
+      table_pages <= 0 || n_pages <= 0 || window < 0 || parts <= 0 || part_pages <= 0)
+    return LLMI_ERR_BAD_SIZE;
+  if ((long)n_blocks * parts > 65535 || n_blocks > 8191) return LLMI_ERR_BAD_SIZE;
+  if (parts > 1 && (!partials || n_floats < (long)n_blocks * n_kv_heads * parts * P8_ROWS * (head_dim + 2))) return LLMI_ERR_BAD_SIZE;
+  if (held != HELD_INT8 && held != HELD_E4M3) return LLMI_ERR_BAD_DTYPE;
+  if ((((uintptr_t)q | (uintptr_t)out | (uintptr_t)k_codes | (uintptr_t)v_codes | (uintptr_t)k_scales | (uintptr_t)v_scales | (uintptr_t)partials) & 15) ||
+      (ldq & 7) || (ldo & 7))
+    return LLMI_ERR_ALIGN;
+  Prompt8Params p{(const __nv_bfloat16*)q, ldq, (__nv_bfloat16*)out, ldo, (const uint8_t*)k_codes, k_scales, (const uint8_t*)v_codes, v_scales,
+                  seq_q_start, seq_kv_len, Paged8{seq_pages, pages_stride, table_pages, n_pages, n_kv_heads, head_dim}, n_seqs, n_heads / n_kv_heads,
+                  scale * 1.4426950408889634f, window, parts, part_pages, partials, error_flag};
+  if (head_dim == 64) return held == HELD_INT8 ? launch_prompt8<64, HELD_INT8>(p, n_blocks, stream) : launch_prompt8<64, HELD_E4M3>(p, n_blocks, stream);
+  return held == HELD_INT8 ? launch_prompt8<128, HELD_INT8>(p, n_blocks, stream) : launch_prompt8<128, HELD_E4M3>(p, n_blocks, stream);
+}

@@ -465,7 +465,7 @@ __global__ void __launch_bounds__(RW8_WARPS * 32, (Rw8Cfg<D, NT, T>::BLOCKS)) at
 #pragma unroll
             for (int o = 4; o < 32; o <<= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, o));
             const float m_new = fmaxf(M[n][j], mx), f = M[n][j] == -INFINITY ? 1.f : fast_exp2(M[n][j] - m_new);
-            L[n][j] *= f;
+            if (M[n][j] != -INFINITY) L[n][j] = rescale8(L[n][j], M[n][j] - m_new);
 #pragma unroll
             for (int i = 0; i < KS; ++i) O[i][n][j] *= f, O[i][n][j + 2] *= f;
             M[n][j] = m_new;
@@ -617,14 +617,14 @@ __global__ void __launch_bounds__(RW8_WARPS * 32, (Rw8Cfg<D, NT, T>::BLOCKS)) at
 #pragma unroll
           for (int j = 0; j < 2; ++j) top[j] = fmaxf(top[j], x[i].m[j]);
 #pragma unroll
-        for (int j = 0; j < 2; ++j) f[j] = r.m[j] == -INFINITY ? 1.f : fast_exp2(r.m[j] - top[j]), r.m[j] = top[j], r.l[j] *= f[j];
+        for (int j = 0; j < 2; ++j) f[j] = r.m[j] == -INFINITY ? 1.f : fast_exp2(r.m[j] - top[j]), r.l[j] = r.m[j] == -INFINITY ? r.l[j] : rescale8(r.l[j], r.m[j] - top[j]), r.m[j] = top[j];
 #pragma unroll
         for (int j = 0; j < 4; ++j) r.o[j] *= f[j & 1];
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
           if (w0 + i * step >= n_states) break;
 #pragma unroll
-          for (int j = 0; j < 2; ++j) f[j] = x[i].m[j] == -INFINITY ? 1.f : fast_exp2(x[i].m[j] - top[j]), r.l[j] = fmaf(x[i].l[j], f[j], r.l[j]);
+          for (int j = 0; j < 2; ++j) f[j] = x[i].m[j] == -INFINITY ? 1.f : fast_exp2(x[i].m[j] - top[j]), r.l[j] += rescale8(x[i].l[j], x[i].m[j] == -INFINITY ? 0.f : x[i].m[j] - top[j]);
 #pragma unroll
           for (int j = 0; j < 4; ++j) r.o[j] = fmaf(x[i].o[j], f[j & 1], r.o[j]);
         }
@@ -687,8 +687,8 @@ __global__ void __launch_bounds__(RW8_WARPS * 32, (Rw8Cfg<D, NT, T>::BLOCKS)) at
               for (int j = 0; j < 2; ++j) {
                 const float m = x[128 + 32 * j], top = fmaxf(r.m[j], m);
                 const float f = r.m[j] == -INFINITY ? 1.f : fast_exp2(r.m[j] - top), h = m == -INFINITY ? 1.f : fast_exp2(m - top);
+                r.l[j] = rescale8(r.l[j], r.m[j] == -INFINITY ? 0.f : r.m[j] - top) + rescale8(x[192 + 32 * j], m == -INFINITY ? 0.f : m - top);
                 r.m[j] = top;
-                r.l[j] = r.l[j] * f + x[192 + 32 * j] * h;
                 r.o[j] = r.o[j] * f + x[32 * j] * h;
                 r.o[j + 2] = r.o[j + 2] * f + x[64 + 32 * j] * h;
               }

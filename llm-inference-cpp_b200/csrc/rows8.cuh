@@ -82,6 +82,12 @@ template <int HELD> __device__ __forceinline__ __half2 halves8(uint32_t w) {
   asm("cvt.rn.f16x2.e4m3x2 %0, %1;" : "=r"(r) : "h"((uint16_t)w));
   return *reinterpret_cast<__half2*>(&r);
 }
+// A sum of weights relative to a maximum that is `down` >= 0 below the new one (base 2).  In two steps: the maxima are those of score +
+// log2 of a value's scale, so the factor alone may be below what fp32 has where the sum times it is not.
+__device__ __forceinline__ float rescale8(float sum, float down) {
+  const float h = fast_exp2(0.5f * down);
+  return sum * h * h;
+}
 template <int HELD> __device__ __forceinline__ float code8(uint32_t byte) { return __low2float(halves8<HELD>(byte)); }
 
 }  // namespace llmi

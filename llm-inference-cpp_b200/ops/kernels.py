@@ -170,7 +170,7 @@ def lib():
                      "llmi_normed_pair", "llmi_stream_axpy_norm", "llmi_stream_postnorm", "llmi_softcap_rows", "llmi_moe_table",
                      "llmi_qkv_unit_prepare", "llmi_latent_prepare_direct", "llmi_channel_token_supported",
                      "llmi_channel_token_prepare", "llmi_channel_token_step", "llmi_cast_rows", "llmi_heads_token", "llmi_heads_token_supported",
-                     "llmi_rope_store8", "llmi_attention_any8", "llmi_attention_rows8", "llmi_attention_rows8_workspace"):
+                     "llmi_rope_store8", "llmi_attention_any8", "llmi_attention_rows8", "llmi_attention_rows8_workspace", "llmi_attention_prompt8"):
             getattr(l, name).restype = c_int
         l.llmi_gemm_tc_workspace.restype = c_long
         l.llmi_delta_state_floats.restype = c_long
@@ -188,6 +188,7 @@ def lib():
         l.llmi_rope_store8.argtypes = [I, I, P, L, P, L, P, I, P, P, P, I, I, I, P, P, P, P, I, I, I, I, I, I, P]
         l.llmi_attention_any8.argtypes = [I, I, P, L, P, L, P, P, P, P, P, P, P, I, I, I, I, I, I, I, I, F, I, P]
         l.llmi_attention_rows8.argtypes = [I, I, P, L, P, L, P, P, P, P, P, P, P, I, I, I, I, I, I, I, I, F, I, P, L, P, L, P]
+        l.llmi_attention_prompt8.argtypes = [I, P, L, P, L, P, P, P, P, P, P, P, I, I, I, I, I, I, I, I, F, I, I, I, P, L, P, P]
         _configured = True
     return l
 
@@ -2259,6 +2260,41 @@ def attention_rows8(q: torch.Tensor, out: torch.Tensor, k: Rows8, v: Rows8, seq_
         max_q, n_heads, n_kv_heads, head_dim, scale, window, slots.data_ptr(), slots.numel(), tickets.data_ptr(), tickets.numel(), _stream8(q)))
 
 
+_ROWS8_MOST = int(os.environ.get("ROWS8_MOST", "32"))
+_PROMPT8_PART_PAGES = 8       # the least pages of a part of a block of 256 query rows
+
+
+def prompt8_parts(n_blocks: int, n_kv_heads: int, table_pages: int) -> int:
+    """In how many parts at most the prompt kernel of 8-bit rows cuts the pages of a block of 256 query rows: while there are
+    fewer blocks than two waves of the device's SMs (one block each), as many as make four."""
+    jobs = n_blocks * n_kv_heads
+    if jobs >= 2 * sm_count():
+        return 1
+    return max(1, min(16, table_pages // _PROMPT8_PART_PAGES, -(-4 * sm_count() // jobs)))
+
+
+def attention_prompt8(q: torch.Tensor, out: torch.Tensor, k: Rows8, v: Rows8, seq_q_start, seq_kv_len, n_blocks: int, seq_pages, n_heads: int,
+                      n_kv_heads: int, head_dim: int, scale: float, window: int = 0, rt=None) -> None:
+    """:func:`attention8` on the tcgen05 tensor cores (bf16, head size 64 or 128): arguments as :func:`attention_rows8`; ``n_blocks``:
+    at least the blocks of 256 rows (tokens times heads of a kv head) over all sequences."""
+    name = "attention_prompt8"
+    held = _check8(name, q, k, v, seq_pages, n_heads, n_kv_heads, head_dim, (out, seq_q_start, seq_kv_len))
+    S, P = seq_pages.shape
+    _refuse(name, q.dtype != torch.bfloat16 or out.dtype != torch.bfloat16, "takes bf16 only")
+    _check_index(name, "seq_q_start", seq_q_start, S + 1)
+    _check_index(name, "seq_kv_len", seq_kv_len, S)
+    parts = prompt8_parts(n_blocks, n_kv_heads, P)
+    partials = None
+    if parts > 1:
+        n = n_blocks * n_kv_heads * parts * 256 * (head_dim + 2)
+        partials = rt.scratch("attn8_parts", (n,), torch.float32) if rt is not None else torch.empty(n, dtype=torch.float32, device=q.device)
+    _check(name, lib().llmi_attention_prompt8(
+        held, q.data_ptr(), q.stride(0), out.data_ptr(), out.stride(0), k.codes.data_ptr(), k.scales.data_ptr(), v.codes.data_ptr(),
+        v.scales.data_ptr(), seq_q_start.data_ptr(), seq_kv_len.data_ptr(), seq_pages.data_ptr(), seq_pages.stride(0), P, S, k.codes.shape[0],
+        n_blocks, n_heads, n_kv_heads, head_dim, scale, window, parts, _PROMPT8_PART_PAGES, _addr(partials), partials.numel() if parts > 1 else 0,
+        tc_scratch(q.device).error.data_ptr(), _stream8(q)))
+
+
 def _most_new(ctx) -> int:
     """A bound on the tokens that a sequence of the step brings, the same for every step that a recorded one is replayed for: a
     prompt step may be padded to a shape, whose recording is told apart by ``short_message`` (the bound itself, or 0)."""
@@ -2293,9 +2329,14 @@ def attention8(q: torch.Tensor, out: torch.Tensor, k: Rows8, v: Rows8, ctx, seq_
         rotated = rt.scratch("attn_q8", (T, width)) if rt is not None else torch.empty((T, width), dtype=q.dtype, device=q.device)
         rope_store8(q, rotated, inv_freq, rotary_dim, ctx.tok_seq, ctx.tok_pos, seq_pages, k, v, n_heads, n_kv_heads, head_dim, write_kv)
         q = rotated
-    max_q = _most_new(ctx)
-    if (head_dim in (64, 128) and _aligned8(q, out, k, v)
-            and _rows8_sizes(_dtype_code(q), seq_pages.shape[0], max_q, n_heads, n_kv_heads, head_dim, seq_pages.shape[1]) is not None):
+    max_q, group = _most_new(ctx), n_heads // n_kv_heads
+    fast = head_dim in (64, 128) and _aligned8(q, out, k, v)
+    if fast and q.dtype == torch.bfloat16 and max_q * group > _ROWS8_MOST:
+        n_blocks = T * group // 256 + seq_pages.shape[0]
+        if n_blocks <= 4095:
+            attention_prompt8(q, out, k, v, ctx.seq_q_start, ctx.seq_kv_len, n_blocks, seq_pages, n_heads, n_kv_heads, head_dim, scale, window, rt)
+            return
+    if (fast and _rows8_sizes(_dtype_code(q), seq_pages.shape[0], max_q, n_heads, n_kv_heads, head_dim, seq_pages.shape[1]) is not None):
         attention_rows8(q, out, k, v, ctx.seq_q_start, ctx.seq_kv_len, max_q, seq_pages, n_heads, n_kv_heads, head_dim, scale, window, rt)
         return
     attention_any8(q, out, k, v, ctx.tok_seq, ctx.tok_pos, seq_pages, n_heads, n_kv_heads, head_dim, scale, window)

@@ -7,6 +7,7 @@
 // serves the whole group — as two tiles of 128 rows, and walks the pages (64 keys) that they see:
 //
 //   raw pages     one thread copies a page's codes and scales (4 bulk copies) into a ring
+//   scales        one warp makes each row's factor of the page
 //   codes -> fp16 four warps make K' = code * (k_scale / kmax) and V' = code * (v_scale / vmax) of a page, kmax and vmax its largest
 //                 scales, rounded to fp16 once (half a step is 2^-11 of a number; a bf16 cache's is 2^-8), in the swizzled layout
 //                 that the products read; so the scales cost the softmax nothing per key: kmax joins its scale, log2 vmax its offset.
@@ -31,7 +32,7 @@
 namespace llmi {
 
 constexpr int P8_ROWS = 256, P8_TILE = 128;
-constexpr int P8_THREADS = 14 * 32;       // copies, products, 2 x 4 softmax warps, 4 converting warps
+constexpr int P8_THREADS = 15 * 32;       // copies, products, 2 x 4 softmax warps, 4 converting warps, scales
 constexpr int P8_TMEM = 512;              // per tile of rows 256 columns: S of even and odd pages (64 each), O (D)
 constexpr float P8_LAZY = 8.0f;
 constexpr float P8_APART = 2.44140625e-4f;             // 2^-12
@@ -64,7 +65,7 @@ struct P8Cfg {
   static constexpr int KV_TILE = SUBS * PAGE8 * 128;      // bytes of a page's K' or V'
   static constexpr int STAGE = 2 * KV_TILE, STAGES = 3;
   static constexpr int RAW = 2 * PAGE8 * D + 2 * PAGE8 * 4, RAWS = D == 64 ? 5 : 3;
-  static constexpr int SMEM = 1024 + 2 * Q_TILE + STAGES * STAGE + RAWS * RAW + 256;
+  static constexpr int SMEM = 1024 + 2 * Q_TILE + STAGES * STAGE + RAWS * RAW + 272;
 };
 
 // Block b of the step's blocks of 256 rows, counted from the last block of the last sequence backwards (late blocks see more keys and
@@ -151,7 +152,7 @@ __global__ void __launch_bounds__(P8_THREADS, 1) attention_prompt8_kernel(Prompt
   const uint32_t base = (smem_u32(smem_raw) + 1023u) & ~1023u;
   uint8_t* const base_p = smem_raw + (base - smem_u32(smem_raw));
   const uint32_t q_smem = base, kv_smem = q_smem + 2 * C::Q_TILE, raw_smem = kv_smem + STAGES * C::STAGE, bars = raw_smem + RAWS * C::RAW;
-  const uint32_t q_full = bars, tmem_slot = bars + 248;
+  const uint32_t q_full = bars, tmem_slot = bars + 264;
   auto raw_full = [&](int s) { return bars + 8u * (1 + s); };
   auto raw_empty = [&](int s) { return bars + 8u * (1 + RAWS + s); };
   auto kv_full = [&](int s) { return bars + 8u * (1 + 2 * RAWS + s); };
@@ -159,7 +160,10 @@ __global__ void __launch_bounds__(P8_THREADS, 1) attention_prompt8_kernel(Prompt
   auto s_full = [&](int tile, int b) { return bars + 8u * (1 + 2 * RAWS + 2 * STAGES + 2 * tile + b); };
   auto p_ready = [&](int tile, int b) { return bars + 8u * (5 + 2 * RAWS + 2 * STAGES + 2 * tile + b); };
   auto o_done = [&](int tile) { return bars + 8u * (9 + 2 * RAWS + 2 * STAGES + tile); };
-  static_assert(8 * (11 + 2 * RAWS + 2 * STAGES) <= 248, "barriers fit");
+  auto fac_full = [&](int s) { return bars + 8u * (11 + 2 * RAWS + 2 * STAGES + s); };
+  static_assert(8 * (11 + 3 * RAWS + 2 * STAGES) <= 264, "barriers fit");
+  __shared__ uint2 s_fac[RAWS][PAGE8];                   // a raw row's factors, each the sum of two fp16 numbers: of its keys, of its values
+  __shared__ uint32_t s_none[RAWS][4];                   // rows whose key codes, and whose value codes, may be no numbers
   __shared__ int s_known[RAWS];                          // the raw page is one of the pool
   __shared__ float s_page[STAGES][4];                    // kmax, log2 vmax, 1 / vmax
   __shared__ uint32_t s_poison[STAGES][2];               // keys whose values are no numbers
@@ -191,7 +195,7 @@ __global__ void __launch_bounds__(P8_THREADS, 1) attention_prompt8_kernel(Prompt
 
   if (threadIdx.x == 0) {
     mbar_init(q_full, 8);
-    for (int s = 0; s < RAWS; ++s) mbar_init(raw_full(s), 1), mbar_init(raw_empty(s), 4);
+    for (int s = 0; s < RAWS; ++s) mbar_init(raw_full(s), 1), mbar_init(raw_empty(s), 4), mbar_init(fac_full(s), 1);
     for (int s = 0; s < STAGES; ++s) mbar_init(kv_full(s), 4), mbar_init(kv_empty(s), 1);
     for (int i = 0; i < 2; ++i) {
       for (int b = 0; b < 2; ++b) mbar_init(s_full(i, b), 1), mbar_init(p_ready(i, b), 4);
@@ -452,65 +456,89 @@ __global__ void __launch_bounds__(P8_THREADS, 1) attention_prompt8_kernel(Prompt
         }
       }
     }
+  } else if (warp == 14) {
+    // ---- scales: what the softmax needs of a page, and its rows' factors ----
+    for (int j = 0; j < n_pg; ++j) {
+      const int s = j % RAWS, st = j % STAGES;
+      if (!mbar_wait(raw_full(s), (j / RAWS) & 1, p.error_flag, 108)) break;
+      const float* ks = reinterpret_cast<const float*>(base_p + (raw_smem - base) + s * C::RAW + 2 * PAGE8 * D);
+      const bool known = s_known[s] != 0;
+      const int a = max(d.lo - (pg0 + j) * PAGE8, 0), b = min(d.last - (pg0 + j) * PAGE8, 63);      // rows that some query sees
+      // the page's largest scales (of rows that are numbers), the least but zeros, and its rows that are no numbers
+      float x[2], y[2], km = 0.f, vm = 0.f, kn = INFINITY, vn = INFINITY;
+      uint32_t bad[2], out[2];
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        const int r = lane + 32 * h;
+        const bool in = r >= a && r <= b;
+        x[h] = in && known ? ks[r] : 0.f;
+        y[h] = in ? (known ? ks[PAGE8 + r] : __int_as_float(0x7fffffff)) : 0.f;
+        const float fx = finite8(x[h]) ? fabsf(x[h]) : 0.f, fy = finite8(y[h]) ? fabsf(y[h]) : 0.f;
+        km = fmaxf(km, fx), vm = fmaxf(vm, fy);
+        if (fx != 0.f) kn = fminf(kn, fx);
+        if (fy != 0.f) vn = fminf(vn, fy);
+        bad[h] = __ballot_sync(0xffffffffu, !finite8(y[h]));
+        out[h] = __ballot_sync(0xffffffffu, !(in && known));
+      }
+#pragma unroll
+      for (int o = 16; o > 0; o >>= 1) {
+        km = fmaxf(km, __shfl_xor_sync(0xffffffffu, km, o));
+        vm = fmaxf(vm, __shfl_xor_sync(0xffffffffu, vm, o));
+      }
+      km = fmaxf(km, P8_TINY);
+      vm = fmaxf(vm, P8_TINY);
+      const bool wide = __any_sync(0xffffffffu, kn < km * P8_APART || vn < vm * P8_APART);
+      const float k_inv = 1.f / km, v_inv = 1.f / vm;
+      // (the softmax is done with what is there of the page three before)
+      if (j >= STAGES && !mbar_wait(kv_empty(st), ((j / STAGES) - 1) & 1, p.error_flag, 109)) break;
+      if (lane == 0) {
+        s_page[st][0] = km;
+        s_page[st][1] = wide ? 0.f : log2f(vm);
+        s_page[st][2] = v_inv;
+        s_poison[st][0] = bad[0];
+        s_poison[st][1] = bad[1];
+        s_wide[st] = wide;
+        s_none[s][0] = out[0], s_none[s][1] = out[1], s_none[s][2] = out[0] | bad[0], s_none[s][3] = out[1] | bad[1];
+      }
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        const int r = lane + 32 * h;
+        float kf = x[h] * k_inv, vf = finite8(y[h]) ? y[h] * v_inv : 0.f;
+        if (wide) {
+          const float own = fmaxf(y[h], P8_TINY);                          // (a NaN's values are zeros here: its bit is in s_poison)
+          s_key[st][0][r] = x[h];
+          s_key[st][1][r] = log2f(own);
+          kf = 1.f;
+          vf = finite8(y[h]) ? y[h] / own : 0.f;
+        }
+        const __half kh = __float2half_rn(kf), vh = __float2half_rn(vf);
+        s_fac[s][r] = make_uint2(half2_bits(__halves2half2(kh, __float2half_rn(kf - __half2float(kh)))),
+                                 half2_bits(__halves2half2(vh, __float2half_rn(vf - __half2float(vh)))));
+      }
+      __syncwarp();
+      if (lane == 0) mbar_arrive(fac_full(s));
+    }
   } else {
     // ---- codes to fp16 ----
     const int id = threadIdx.x - 10 * 32;                          // 0 .. 127
     constexpr int UPR = D / 16, UNITS = PAGE8 * UPR / 128;         // 16-byte pieces of a row, and of a tile per thread
     for (int j = 0; j < n_pg; ++j) {
       const int s = j % RAWS, st = j % STAGES;
-      if (!mbar_wait(raw_full(s), (j / RAWS) & 1, p.error_flag, 108)) break;
-      if (j >= STAGES && !mbar_wait(kv_empty(st), ((j / STAGES) - 1) & 1, p.error_flag, 109)) break;
+      if (!mbar_wait(fac_full(s), (j / RAWS) & 1, p.error_flag, 110)) break;      // (the raw page is here, and the stage is free)
       const uint8_t* raw = base_p + (raw_smem - base) + s * C::RAW;
-      const float* ks = reinterpret_cast<const float*>(raw + 2 * PAGE8 * D);
-      const float* vs = ks + PAGE8;
-      const bool known = s_known[s] != 0;
-      const int a = max(d.lo - (pg0 + j) * PAGE8, 0), b = min(d.last - (pg0 + j) * PAGE8, 63);      // rows that some query sees
-      // the page's largest scales (of rows that are numbers) and its rows that are not
-      float km = 0.f, vm = 0.f, kn = INFINITY, vn = INFINITY;              // largest, and least but zeros
-      uint32_t bad[2];
-#pragma unroll
-      for (int h = 0; h < 2; ++h) {
-        const int r = lane + 32 * h;
-        const bool in = r >= a && r <= b;
-        const float x = in && known ? ks[r] : 0.f, y = in ? (known ? vs[r] : __int_as_float(0x7fffffff)) : 0.f;
-        km = fmaxf(km, finite8(x) ? fabsf(x) : 0.f);
-        vm = fmaxf(vm, finite8(y) ? fabsf(y) : 0.f);
-        if (x != 0.f) kn = fminf(kn, fabsf(x));
-        if (y != 0.f) vn = fminf(vn, fabsf(y));
-        bad[h] = __ballot_sync(0xffffffffu, !finite8(y));
-      }
-      km = fmaxf(warp_max(km), P8_TINY);
-      vm = fmaxf(warp_max(vm), P8_TINY);
-      const bool wide = __any_sync(0xffffffffu, kn < km * P8_APART || vn < vm * P8_APART);
-      if (id == 0) {
-        s_page[st][0] = km;
-        s_page[st][1] = wide ? 0.f : log2f(vm);
-        s_page[st][2] = 1.f / vm;
-        s_poison[st][0] = bad[0];
-        s_poison[st][1] = bad[1];
-        s_wide[st] = wide;
-      }
-      if (wide) {
-        if (id < PAGE8) {
-          const bool in = id >= a && id <= b && known;
-          const float y = in ? fmaxf(vs[id], P8_TINY) : 1.f;               // (a NaN's values are zeros here: its bit is in s_poison)
-          s_key[st][0][id] = in ? ks[id] : 0.f;
-          s_key[st][1][id] = log2f(y);
-        }
-      }
       const uint32_t k_dst = kv_smem + st * C::STAGE, v_dst = k_dst + C::KV_TILE;
-      const float k_inv = 1.f / km, v_inv = 1.f / vm;
+      const bool some = HELD == HELD_E4M3 && (s_none[s][2] | s_none[s][3]) != 0u;      // (any int8 code times 0 is 0)
 #pragma unroll
       for (int i = 0; i < UNITS; ++i) {
         const int x = id + 128 * i, r = x / UPR, u = x % UPR;
-        const bool in = r >= a && r <= b && known;
-        const uint4 kw = *reinterpret_cast<const uint4*>(raw + x * 16), vw = *reinterpret_cast<const uint4*>(raw + PAGE8 * D + x * 16);
-        // the row's factor as the sum of two fp16 numbers, so that a product is rounded once
-        const float kf = in ? (wide ? 1.f : ks[r] * k_inv) : 0.f, vf = in && finite8(vs[r]) ? vs[r] * (wide ? 1.f / fmaxf(vs[r], P8_TINY) : v_inv) : 0.f;
-        const __half kh = __float2half_rn(kf), vh = __float2half_rn(vf);
-        const __half2 kh2 = __half2half2(kh), vh2 = __half2half2(vh);
-        const __half2 kl2 = __half2half2(__float2half_rn(kf - __half2float(kh))), vl2 = __half2half2(__float2half_rn(vf - __half2float(vh)));
-        const bool zero_v = !(in && finite8(vs[r])), zero_k = !in;          // (codes there may be no numbers)
+        uint4 kw = *reinterpret_cast<const uint4*>(raw + x * 16), vw = *reinterpret_cast<const uint4*>(raw + PAGE8 * D + x * 16);
+        const uint2 f = s_fac[s][r];
+        if (some) {
+          if ((s_none[s][r >> 5] >> (r & 31)) & 1u) kw = make_uint4(0u, 0u, 0u, 0u);
+          if ((s_none[s][2 + (r >> 5)] >> (r & 31)) & 1u) vw = make_uint4(0u, 0u, 0u, 0u);
+        }
+        const __half2 kf = *reinterpret_cast<const __half2*>(&f.x), vf = *reinterpret_cast<const __half2*>(&f.y);
+        const __half2 kh2 = __low2half2(kf), kl2 = __high2half2(kf), vh2 = __low2half2(vf), vl2 = __high2half2(vf);
         const uint32_t* kp = &kw.x;
         const uint32_t* vp = &vw.x;
         const uint32_t at = (u / 4) * (PAGE8 * 128) + r * 128;
@@ -518,11 +546,9 @@ __global__ void __launch_bounds__(P8_THREADS, 1) attention_prompt8_kernel(Prompt
         for (int h = 0; h < 2; ++h) {                                       // eight codes: 16 bytes of fp16
           uint32_t kx[4], vx[4];
 #pragma unroll
-          for (int w = 0; w < 2; ++w) {
-            const uint32_t kc = zero_k ? 0u : kp[2 * h + w], vc = zero_v ? 0u : vp[2 * h + w];
-            __half2 k0, k1, v0h, v1h;
-            k0 = halves8<HELD>(kc & 0xffffu), k1 = halves8<HELD>(kc >> 16);
-            v0h = halves8<HELD>(vc & 0xffffu), v1h = halves8<HELD>(vc >> 16);
+          for (int w = 0; w < 2; ++w) {                                     // a product is rounded once
+            const __half2 k0 = halves8<HELD>(kp[2 * h + w] & 0xffffu), k1 = halves8<HELD>(kp[2 * h + w] >> 16);
+            const __half2 v0h = halves8<HELD>(vp[2 * h + w] & 0xffffu), v1h = halves8<HELD>(vp[2 * h + w] >> 16);
             kx[2 * w] = half2_bits(__hfma2(k0, kh2, __hmul2(k0, kl2)));
             kx[2 * w + 1] = half2_bits(__hfma2(k1, kh2, __hmul2(k1, kl2)));
             vx[2 * w] = half2_bits(__hfma2(v0h, vh2, __hmul2(v0h, vl2)));

@@ -75,7 +75,7 @@ template <int HELD> __device__ __forceinline__ __half2 halves8(uint32_t w) {
   uint32_t r;
   if (HELD == HELD_INT8) {
     // 0x6400 | u is 1024 + u in fp16; u = code + 128
-    asm("prmt.b32 %0, %1, %2, 0x4140;" : "=r"(r) : "r"(w ^ 0x8080u), "r"(0x64646464u));
+    asm("prmt.b32 %0, %1, %2, 0x4140;" : "=r"(r) : "r"(w ^ 0x80808080u), "r"(0x64646464u));
     const __half2 bias = __halves2half2(__ushort_as_half(0x6480), __ushort_as_half(0x6480));      // 1152
     return __hsub2(*reinterpret_cast<__half2*>(&r), bias);
   }

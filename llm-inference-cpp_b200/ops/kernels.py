@@ -2264,16 +2264,17 @@ _ROWS8_MOST = int(os.environ.get("ROWS8_MOST", "32"))
 _PROMPT8_PART_PAGES = 8       # the least pages of a part of a block of 256 query rows
 
 
-def prompt8_parts(n_blocks: int, n_kv_heads: int, table_pages: int) -> int:
-    """In how many parts at most the prompt kernel of 8-bit rows cuts the pages of a block of 256 query rows: while there are
-    fewer blocks than two waves of the device's SMs (one block each), as many as make four."""
-    jobs = n_blocks * n_kv_heads
-    if jobs >= 2 * sm_count():
+def prompt8_parts(n_blocks: int, n_kv_heads: int, table_pages: int, max_q: int) -> int:
+    """In how many parts at most the prompt kernel of 8-bit rows cuts the pages of a block of 256 query rows, with one block a SM.
+    Blocks of whole prompts differ in their pages and start with the longest, so that a wave of them fills the device evenly; blocks
+    of a message behind a long history all see nearly all of it, and are cut until there are four waves."""
+    jobs, sms = n_blocks * n_kv_heads, sm_count()
+    if jobs >= 3 * sms or (jobs >= sms and 2 * max_q >= 64 * table_pages):
         return 1
-    return max(1, min(16, table_pages // _PROMPT8_PART_PAGES, -(-4 * sm_count() // jobs)))
+    return max(1, min(16, table_pages // _PROMPT8_PART_PAGES, -(-4 * sms // jobs)))
 
 
-def attention_prompt8(q: torch.Tensor, out: torch.Tensor, k: Rows8, v: Rows8, seq_q_start, seq_kv_len, n_blocks: int, seq_pages, n_heads: int,
+def attention_prompt8(q: torch.Tensor, out: torch.Tensor, k: Rows8, v: Rows8, seq_q_start, seq_kv_len, n_blocks: int, max_q: int, seq_pages, n_heads: int,
                       n_kv_heads: int, head_dim: int, scale: float, window: int = 0, rt=None) -> None:
     """:func:`attention8` on the tcgen05 tensor cores (bf16, head size 64 or 128): arguments as :func:`attention_rows8`; ``n_blocks``:
     at least the blocks of 256 rows (tokens times heads of a kv head) over all sequences."""
@@ -2283,7 +2284,7 @@ def attention_prompt8(q: torch.Tensor, out: torch.Tensor, k: Rows8, v: Rows8, se
     _refuse(name, q.dtype != torch.bfloat16 or out.dtype != torch.bfloat16, "takes bf16 only")
     _check_index(name, "seq_q_start", seq_q_start, S + 1)
     _check_index(name, "seq_kv_len", seq_kv_len, S)
-    parts = prompt8_parts(n_blocks, n_kv_heads, P)
+    parts = prompt8_parts(n_blocks, n_kv_heads, P, max_q)
     partials = None
     if parts > 1:
         n = n_blocks * n_kv_heads * parts * 256 * (head_dim + 2)
@@ -2334,7 +2335,7 @@ def attention8(q: torch.Tensor, out: torch.Tensor, k: Rows8, v: Rows8, ctx, seq_
     if fast and q.dtype == torch.bfloat16 and max_q * group > _ROWS8_MOST:
         n_blocks = T * group // 256 + seq_pages.shape[0]
         if n_blocks <= 4095:
-            attention_prompt8(q, out, k, v, ctx.seq_q_start, ctx.seq_kv_len, n_blocks, seq_pages, n_heads, n_kv_heads, head_dim, scale, window, rt)
+            attention_prompt8(q, out, k, v, ctx.seq_q_start, ctx.seq_kv_len, n_blocks, max_q, seq_pages, n_heads, n_kv_heads, head_dim, scale, window, rt)
             return
     if (fast and _rows8_sizes(_dtype_code(q), seq_pages.shape[0], max_q, n_heads, n_kv_heads, head_dim, seq_pages.shape[1]) is not None):
         attention_rows8(q, out, k, v, ctx.seq_q_start, ctx.seq_kv_len, max_q, seq_pages, n_heads, n_kv_heads, head_dim, scale, window, rt)

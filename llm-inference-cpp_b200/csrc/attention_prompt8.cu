@@ -14,7 +14,7 @@
 //                 (A page whose scales are more than 2^12 apart would lose bits of its small rows, which may be all that a query
 //                 sees: there K' and V' are the codes themselves and the softmax takes each key's scales.)
 //   S = Q' K'^T   tcgen05.mma, Q' the queries divided by a power of two per row (fp16, exact but for entries 2^-14 of the largest)
-//   softmax       a thread owns a row: tcgen05.ld, mask, maximum, exp2, sum; P = 2^(s + log2 vmax - m) goes back to tensor memory
+//   softmax       two threads own a row, 32 keys of a page each: tcgen05.ld, mask, maximum (exchanged), exp2, sum; P = 2^(s + log2 vmax - m) goes back to tensor memory
 //                 as fp16 over the S it has read; the sum of w is that of P / vmax
 //   O += P V'     tcgen05.mma with A in tensor memory, accumulating in fp32; m follows the running maximum (of s + log2 vmax) only
 //                 when that has grown by more than 8, so O is rescaled a few times per row
@@ -32,7 +32,10 @@
 namespace llmi {
 
 constexpr int P8_ROWS = 256, P8_TILE = 128;
-constexpr int P8_THREADS = 15 * 32;       // copies, products, 2 x 4 softmax warps, 4 converting warps, scales
+// Warps: 0 copies, 1 products, 2 scales, (3 none,) 4 .. 19 softmax (two tiles, two halves of a page's keys, four quarters of the rows),
+// 20 .. 23 codes to fp16.
+constexpr int P8_SOFTMAX = 4, P8_CONVERT = 20, P8_WARPS = 24;
+constexpr int P8_THREADS = P8_WARPS * 32;
 constexpr int P8_TMEM = 512;              // per tile of rows 256 columns: S of even and odd pages (64 each), O (D)
 constexpr float P8_LAZY = 8.0f;
 constexpr float P8_APART = 2.44140625e-4f;             // 2^-12
@@ -135,12 +138,30 @@ __device__ __forceinline__ void p8_st16(uint32_t taddr, const uint32_t* v) {
       : "memory");
 }
 __device__ __forceinline__ void p8_st_wait() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
-__device__ __forceinline__ void p8_mma_ts(uint32_t d, uint32_t a_tmem, uint64_t b, uint32_t idesc, uint32_t acc) {
+// Products and commits by the one lane of a warp that has `one` set; the whole warp comes here, so that descriptors and addresses stay
+// in uniform registers (in a branch of one lane each product's way there took 65 clocks, 2.4 of the 3.5 thousand a page at D = 128).
+__device__ __forceinline__ void p8_mma(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t acc, uint32_t one) {
   asm volatile(
-      "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
-      "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}"
-      ::"r"(d), "r"(a_tmem), "l"(b), "r"(idesc), "r"(acc)
+      "{\n\t.reg .pred p, q;\n\tsetp.ne.b32 p, %4, 0;\n\tsetp.ne.b32 q, %5, 0;\n\t"
+      "@q tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}"
+      ::"r"(d), "l"(a), "l"(b), "r"(idesc), "r"(acc), "r"(one)
       : "memory");
+}
+__device__ __forceinline__ void p8_mma_ts(uint32_t d, uint32_t a_tmem, uint64_t b, uint32_t idesc, uint32_t acc, uint32_t one) {
+  asm volatile(
+      "{\n\t.reg .pred p, q;\n\tsetp.ne.b32 p, %4, 0;\n\tsetp.ne.b32 q, %5, 0;\n\t"
+      "@q tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}"
+      ::"r"(d), "r"(a_tmem), "l"(b), "r"(idesc), "r"(acc), "r"(one)
+      : "memory");
+}
+__device__ __forceinline__ void p8_commit(uint32_t bar, uint32_t one) {
+  asm volatile("{\n\t.reg .pred q;\n\tsetp.ne.b32 q, %1, 0;\n\t@q tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];\n\t}"
+               ::"r"(bar), "r"(one) : "memory");
+}
+__device__ __forceinline__ uint32_t elect_one() {
+  uint32_t one;
+  asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(one));
+  return one;
 }
 __device__ __forceinline__ uint32_t half2_bits(__half2 h) { return *reinterpret_cast<uint32_t*>(&h); }
 
@@ -167,6 +188,8 @@ __global__ void __launch_bounds__(P8_THREADS, 1) attention_prompt8_kernel(Prompt
   __shared__ int s_known[RAWS];                          // the raw page is one of the pool
   __shared__ float s_page[STAGES][4];                    // kmax, log2 vmax, 1 / vmax
   __shared__ uint32_t s_poison[STAGES][2];               // keys whose values are no numbers
+  __shared__ float s_top[2][2][2][P8_TILE];              // [page parity][tile][half][row]: the largest score of a row's half
+  __shared__ float s_sum[2][2][P8_TILE];
   __shared__ int s_wide[STAGES];                         // the page's scales are far apart: its keys' own
   __shared__ float s_key[STAGES][2][PAGE8];              // k_scale, log2 v_scale
 
@@ -194,11 +217,11 @@ __global__ void __launch_bounds__(P8_THREADS, 1) attention_prompt8_kernel(Prompt
   }
 
   if (threadIdx.x == 0) {
-    mbar_init(q_full, 8);
+    mbar_init(q_full, 16);
     for (int s = 0; s < RAWS; ++s) mbar_init(raw_full(s), 1), mbar_init(raw_empty(s), 4), mbar_init(fac_full(s), 1);
     for (int s = 0; s < STAGES; ++s) mbar_init(kv_full(s), 4), mbar_init(kv_empty(s), 1);
     for (int i = 0; i < 2; ++i) {
-      for (int b = 0; b < 2; ++b) mbar_init(s_full(i, b), 1), mbar_init(p_ready(i, b), 4);
+      for (int b = 0; b < 2; ++b) mbar_init(s_full(i, b), 1), mbar_init(p_ready(i, b), 8);
       mbar_init(o_done(i), 1);
     }
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
@@ -238,58 +261,69 @@ __global__ void __launch_bounds__(P8_THREADS, 1) attention_prompt8_kernel(Prompt
       }
     }
   } else if (warp == 1) {
-    if (lane == 0) {
-      // ---- products ----
-      // S: A = Q' (K-major), B = K' (K-major), 64 columns; O: A = P (tensor memory, 32 columns of fp16 pairs), B = V' (MN-major).
-      // MMAs of one thread run in issue order: S_{j+1} may be issued into the buffer that P_{j-1} lies in once O += P_{j-1} V_{j-1} was.
-      const uint32_t idesc_s = (1u << 4) | ((uint32_t)(64 >> 3) << 17) | ((uint32_t)(128 >> 4) << 24), idesc_o = idesc_s | (1u << 16);
-      auto issue_s = [&](int tile, int j) {
-        const uint32_t dst = tmem + 256u * tile + 64u * (j & 1);
+    // ---- products ----
+    // S: A = Q' (K-major), B = K' (K-major), 64 columns; O: A = P (tensor memory, 32 columns of fp16 pairs), B = V' (MN-major, sub-tiles
+    // of 64 dims KV_TILE / SUBS apart).  MMAs of one thread run in issue order: S_{j+1} may be issued into the buffer that P_{j-1} lies in
+    // once O += P_{j-1} V_{j-1} was.  Everything here is the same in all lanes.
+    const uint32_t idesc_s = (1u << 4) | ((uint32_t)(64 >> 3) << 17) | ((uint32_t)(128 >> 4) << 24);
+    const uint32_t idesc_o = (1u << 4) | (1u << 16) | ((uint32_t)(D >> 3) << 17) | ((uint32_t)(128 >> 4) << 24);
+    const uint32_t one = elect_one(), tm = __shfl_sync(0xffffffffu, tmem, 0);
+    const int pages = __shfl_sync(0xffffffffu, n_pg, 0);
+    const int in_tile[2] = {__shfl_sync(0xffffffffu, n_tile[0], 0), __shfl_sync(0xffffffffu, n_tile[1], 0)};
+    const uint64_t desc_q = umma_desc(q_smem);
+    const uint64_t desc_k = umma_desc(kv_smem);
+    const uint64_t desc_v = umma_desc(kv_smem + C::KV_TILE) + ((uint64_t)((PAGE8 * 128 >> 4) - 1) << 16);      // leading offset: to the next 64 dims
+    auto issue_s = [&](int tile, int j, int st) {
+      const uint32_t dst = tm + 256u * tile + 64u * (j & 1);
 #pragma unroll
-        for (int k = 0; k < D / 16; ++k)
-          umma_bf16(dst, umma_desc(q_smem + tile * C::Q_TILE + (k / 4) * (P8_TILE * 128)) + 2 * (k % 4),
-                    umma_desc(kv_smem + (j % STAGES) * C::STAGE + (k / 4) * (PAGE8 * 128)) + 2 * (k % 4), idesc_s, k > 0);
-        umma_commit(s_full(tile, j & 1));
-      };
-      auto issue_o = [&](int tile, int j) {
-        const uint32_t a = tmem + 256u * tile + 64u * (j & 1), o = tmem + 256u * tile + 128u;
-        const uint32_t v = kv_smem + (j % STAGES) * C::STAGE + C::KV_TILE;
+      for (int k = 0; k < D / 16; ++k)
+        p8_mma(dst, desc_q + (uint32_t)((tile * C::Q_TILE + (k / 4) * (P8_TILE * 128)) >> 4) + 2 * (k % 4),
+               desc_k + (uint32_t)(st * (C::STAGE >> 4)) + ((k / 4) * (PAGE8 * 128) >> 4) + 2 * (k % 4), idesc_s, k > 0, one);
+      p8_commit(s_full(tile, j & 1), one);
+    };
+    auto issue_o = [&](int tile, int j, int st) {
+      const uint32_t a = tm + 256u * tile + 64u * (j & 1), o = tm + 256u * tile + 128u;
 #pragma unroll
-        for (int k = 0; k < 4; ++k)
+      for (int k = 0; k < 4; ++k)
+        p8_mma_ts(o, a + 32u * (k / 2) + 8u * (k % 2), desc_v + (uint32_t)(st * (C::STAGE >> 4)) + (k * (16 * 128) >> 4), idesc_o, (j > 0 || k > 0) ? 1u : 0u, one);
+      p8_commit(o_done(tile), one);
+    };
+    bool ok = __all_sync(0xffffffffu, mbar_wait(q_full, 0, p.error_flag, 102));
+    int st = 0, before = 0;              // the stage of page j, of page j - 1
+    uint32_t phase = 0;
+    for (int j = 0; j <= pages && ok; ++j) {
+      if (j < pages) {
+        ok = __all_sync(0xffffffffu, mbar_wait(kv_full(st), phase, p.error_flag, 103));
+        if (!ok) break;
+        asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
 #pragma unroll
-          for (int u = 0; u < SUBS; ++u)
-            p8_mma_ts(o + 64u * u, a + 8u * k, umma_desc(v + u * (PAGE8 * 128)) + (uint64_t)(k * ((16 * 128) >> 4)), idesc_o, (j > 0 || k > 0) ? 1u : 0u);
-        umma_commit(o_done(tile));
-      };
-      bool ok = mbar_wait(q_full, 0, p.error_flag, 102);
-      for (int j = 0; j <= n_pg && ok; ++j) {
-        if (j < n_pg) {
-          ok = mbar_wait(kv_full(j % STAGES), (j / STAGES) & 1, p.error_flag, 103);
-          if (!ok) break;
-          asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-          for (int tile = 0; tile < 2; ++tile)
-            if (j < n_tile[tile]) issue_s(tile, j);
-        }
-        if (j >= 1) {
-          for (int tile = 0; tile < 2 && ok; ++tile) {
-            if (j - 1 >= n_tile[tile]) continue;
-            ok = mbar_wait(p_ready(tile, (j - 1) & 1), ((j - 1) >> 1) & 1, p.error_flag, 104);
-            if (!ok) break;
-            asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-            issue_o(tile, j - 1);
-          }
-          if (j - 1 + STAGES < n_pg) umma_commit(kv_empty((j - 1) % STAGES));      // (where the stage is filled again)
-        }
+        for (int tile = 0; tile < 2; ++tile)
+          if (j < in_tile[tile]) issue_s(tile, j, st);
       }
+      if (j >= 1) {
+#pragma unroll
+        for (int tile = 0; tile < 2; ++tile) {
+          if (j - 1 >= in_tile[tile] || !ok) continue;
+          ok = __all_sync(0xffffffffu, mbar_wait(p_ready(tile, (j - 1) & 1), ((j - 1) >> 1) & 1, p.error_flag, 104));
+          asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+          if (ok) issue_o(tile, j - 1, before);
+        }
+        if (j - 1 + STAGES < pages) p8_commit(kv_empty(before), one);      // (where the stage is filled again)
+      }
+      before = st;
+      if (++st == STAGES) st = 0, phase ^= 1u;
     }
-  } else if (warp < 10) {
-    // ---- softmax and output: a thread a row ----
-    const int tile = (warp - 2) >> 2, quad = warp & 3;
-    const int r = tile * P8_TILE + quad * 32 + lane;               // row of the block; quad * 32 + lane is its TMEM lane
+  } else if (warp >= P8_SOFTMAX && warp < P8_CONVERT) {
+    // ---- softmax and output: two threads a row, each with 32 keys of every page and half of the row's output ----
+    constexpr int HD = D / 2;
+    const int tile = (warp - P8_SOFTMAX) >> 3, half = ((warp - P8_SOFTMAX) >> 2) & 1, quad = warp & 3;
+    const int in_tile = quad * 32 + lane, r = tile * P8_TILE + in_tile;       // the row's TMEM lane, the row of the block
     const int row = d.row0 + r, tok = row / G, head = kvh * G + row % G;
     const bool row_ok = r < d.rows;
     const int qpos = d.pos0 + (d.row0 + min(r, d.rows - 1)) / G;
     const int pos_a = __shfl_sync(0xffffffffu, qpos, 0), pos_b = __shfl_sync(0xffffffffu, qpos, 31);      // the warp's first and last
+    // what the two threads of a row tell each other: 64 threads meet
+    auto meet = [&]() { asm volatile("bar.sync %0, 64;" ::"r"(1 + tile * 4 + quad) : "memory"); };
     // the row's queries, divided by a power of two above the largest
     float row_fac;
     {
@@ -311,16 +345,17 @@ __global__ void __launch_bounds__(P8_THREADS, 1) attention_prompt8_kernel(Prompt
       const float down2 = ex > 126 ? 1.f / (float)(1 << (ex - 126)) : 1.f;
       if (p.scale_log2 < 0.f) down = -down;                        // the factor of the scores below is positive
       row_fac = fmaxf(ldexpf(fabsf(p.scale_log2), ex), 1e-30f);    // (never quite 0: 0 times a masked key's -inf is no number)
-      const uint32_t at = q_smem + tile * C::Q_TILE + (quad * 32 + lane) * 128;
+      const uint32_t at = q_smem + tile * C::Q_TILE + in_tile * 128;
 #pragma unroll
-      for (int c = 0; c < D / 8; ++c) {
+      for (int i = 0; i < HD / 8; ++i) {
+        const int c = half * (HD / 8) + i;
         const uint4 raw = row_ok ? src[c] : make_uint4(0u, 0u, 0u, 0u);
         const __nv_bfloat162* b = reinterpret_cast<const __nv_bfloat162*>(&raw);
         uint32_t h[4];
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          const float2 f = __bfloat1622float2(b[i]);
-          h[i] = half2_bits(__floats2half2_rn(f.x * down * down2, f.y * down * down2));
+        for (int e = 0; e < 4; ++e) {
+          const float2 f = __bfloat1622float2(b[e]);
+          h[e] = half2_bits(__floats2half2_rn(f.x * down * down2, f.y * down * down2));
         }
         asm volatile("st.shared.v4.u32 [%0], {%1, %2, %3, %4};"
                      ::"r"(at + (c / 8) * (P8_TILE * 128) + (((c % 8) ^ (lane & 7)) << 4)), "r"(h[0]), "r"(h[1]), "r"(h[2]), "r"(h[3]) : "memory");
@@ -330,38 +365,43 @@ __global__ void __launch_bounds__(P8_THREADS, 1) attention_prompt8_kernel(Prompt
       if (lane == 0) mbar_arrive(q_full);
     }
     const int n = n_tile[tile];
-    const uint32_t t_lane = (uint32_t)(quad * 32) << 16, t_tile = tmem + 256u * tile + t_lane, t_o = t_tile + 128u;
-    float m_run = -INFINITY, m_ref = -INFINITY, l_run = 0.f;       // of s + log2 vmax, base 2; the sum of 2^(s - m_ref)
+    const uint32_t t_lane = (uint32_t)(quad * 32) << 16, t_tile = tmem + 256u * tile + t_lane, t_o = t_tile + 128u + (uint32_t)(HD * half);
+    float m_run = -INFINITY, m_ref = -INFINITY, l_run = 0.f;       // of s + log2 vmax, base 2; the sum of 2^(s - m_ref) over this half
     bool ok = true;
-    for (int j = 0; j < n && ok; ++j) {
-      ok = mbar_wait(s_full(tile, j & 1), (j >> 1) & 1, p.error_flag, 105);
-      if (!ok) break;
+    int st = 0;                                                    // j % STAGES
+    // (after a wait that gave up the pages are gone through without waiting: the two threads of a row go on meeting)
+    for (int j = 0; j < n; ++j, st = st + 1 == STAGES ? 0 : st + 1) {
+      ok = ok && mbar_wait(s_full(tile, j & 1), (j >> 1) & 1, p.error_flag, 105);
+      __syncwarp();
       asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-      const uint32_t t_s = t_tile + 64u * (j & 1);
-      float sc[64];
-#pragma unroll
-      for (int c = 0; c < 64; c += 16) p8_ld16(t_s + (uint32_t)c, sc + c);
-      const float to_log2 = s_wide[j % STAGES] ? 1.f : row_fac * s_page[j % STAGES][0], lv = s_page[j % STAGES][1], inv_v = s_page[j % STAGES][2];
-      const uint32_t bad0 = s_poison[j % STAGES][0], bad1 = s_poison[j % STAGES][1];
-      const bool wide = s_wide[j % STAGES] != 0;
-      const int key0 = (pg0 + j) * PAGE8;
+      const uint32_t t_s = t_tile + 64u * (j & 1) + 32u * half;    // this half's scores, then its weights
+      float sc[32];
+      p8_ld16(t_s, sc);
+      p8_ld16(t_s + 16u, sc + 16);
+      const bool wide = s_wide[st] != 0;
+      const float to_log2 = wide ? 1.f : row_fac * s_page[st][0], lv = s_page[st][1], inv_v = s_page[st][2];
+      const uint32_t bad = s_poison[st][half];
+      const int key0 = (pg0 + j) * PAGE8 + 32 * half;
       p8_ld_wait();
       if (wide) {                                                  // (kmax 1 / row_fac, vmax 1: the scores are final)
 #pragma unroll
-        for (int c = 0; c < 64; ++c) sc[c] = fmaf(sc[c], row_fac * s_key[j % STAGES][0][c], s_key[j % STAGES][1][c]);
+        for (int c = 0; c < 32; ++c) sc[c] = fmaf(sc[c], row_fac * s_key[st][0][32 * half + c], s_key[st][1][32 * half + c]);
       }
-      if (key0 + PAGE8 - 1 > pos_a || (p.window > 0 && key0 <= pos_b - p.window)) {
-        const int a = p.window > 0 ? qpos - p.window + 1 - key0 : 0, b = qpos - key0;      // the keys a .. b of the page are seen
+      if (key0 + 31 > pos_a || (p.window > 0 && key0 <= pos_b - p.window)) {
+        const int a = p.window > 0 ? qpos - p.window + 1 - key0 : 0, b = qpos - key0;      // the keys a .. b are seen
 #pragma unroll
-        for (int c = 0; c < 64; ++c)
+        for (int c = 0; c < 32; ++c)
           if (c > b || c < a) sc[c] = -INFINITY;
       }
       float mx4[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
-      for (int c = 0; c < 64; c += 8)
+      for (int c = 0; c < 32; c += 8)
 #pragma unroll
         for (int u = 0; u < 4; ++u) mx4[u] = fmaxf(mx4[u], fmaxf(sc[c + 2 * u], sc[c + 2 * u + 1]));
-      const float top = fmaf(fmaxf(fmaxf(mx4[0], mx4[1]), fmaxf(mx4[2], mx4[3])), to_log2, lv);
+      float top = fmaf(fmaxf(fmaxf(mx4[0], mx4[1]), fmaxf(mx4[2], mx4[3])), to_log2, lv);
+      s_top[j & 1][tile][half][in_tile] = top;
+      meet();
+      top = fmaxf(top, s_top[j & 1][tile][half ^ 1][in_tile]);
       m_run = fmaxf(m_run, top);
       float corr = 1.f;
       if (m_run > m_ref + P8_LAZY || m_ref == -INFINITY) {         // (both -inf: nothing seen yet)
@@ -372,9 +412,9 @@ __global__ void __launch_bounds__(P8_THREADS, 1) attention_prompt8_kernel(Prompt
       const float off = m_ref == -INFINITY ? 0.f : lv - m_ref;
       float2 sum2[4] = {{0.f, 0.f}, {0.f, 0.f}, {0.f, 0.f}, {0.f, 0.f}};
       const float2 scale2 = make_float2(to_log2, to_log2), off2 = make_float2(off, off);
-      uint32_t packed[32];
+      uint32_t packed[16];
 #pragma unroll
-      for (int c = 0; c < 64; c += 2) {
+      for (int c = 0; c < 32; c += 2) {
         const float2 x = __ffma2_rn(make_float2(sc[c], sc[c + 1]), scale2, off2);
         const float2 e = make_float2(fast_exp2(x.x), fast_exp2(x.y));
         sum2[(c >> 1) & 3] = __fadd2_rn(sum2[(c >> 1) & 3], e);
@@ -387,21 +427,20 @@ __global__ void __launch_bounds__(P8_THREADS, 1) attention_prompt8_kernel(Prompt
         l_run = fmaf(s.x + s.y, inv_v, l_run);
       } else {
 #pragma unroll
-        for (int c = 0; c < 64; ++c) l_run += fast_exp2(fmaf(sc[c], to_log2, off) - (wide ? s_key[j % STAGES][1][c] : lv));
+        for (int c = 0; c < 32; ++c) l_run += fast_exp2(fmaf(sc[c], to_log2, off) - (wide ? s_key[st][1][32 * half + c] : lv));
       }
-      if (bad0 | bad1) {                                           // values that are no numbers: for the rows that see them
-        const int a = p.window > 0 ? max(qpos - p.window + 1 - key0, 0) : 0, b = min(qpos - key0, 63);
-        const uint64_t bad = ((uint64_t)bad1 << 32) | bad0;
-        if (a <= b && ((bad >> a) << (63 - (b - a)))) l_run = __int_as_float(0x7fffffff);
+      if (bad) {                                                   // values that are no numbers: for the rows that see them
+        const int a = p.window > 0 ? max(qpos - p.window + 1 - key0, 0) : 0, b = min(qpos - key0, 31);
+        if (a <= b && ((bad >> a) << (31 - (b - a)))) l_run = __int_as_float(0x7fffffff);
       }
       if (j >= 1) {
         // (waited for on every page: a wait on a phase's parity is right only for a thread at most one phase behind)
-        ok = mbar_wait(o_done(tile), (j - 1) & 1, p.error_flag, 106);
-        if (!ok) break;
+        ok = ok && mbar_wait(o_done(tile), (j - 1) & 1, p.error_flag, 106);
+        __syncwarp();
         if (__any_sync(0xffffffffu, corr != 1.f)) {
           asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
 #pragma unroll
-          for (int c = 0; c < D; c += 16) {
+          for (int c = 0; c < HD; c += 16) {
             float t[16];
             uint32_t u[16];
             p8_ld16(t_o + (uint32_t)c, t);
@@ -413,7 +452,6 @@ __global__ void __launch_bounds__(P8_THREADS, 1) attention_prompt8_kernel(Prompt
         }
       }
       p8_st16(t_s, packed);
-      p8_st16(t_s + 16u, packed + 16);
       p8_st_wait();
       asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
       __syncwarp();
@@ -422,13 +460,16 @@ __global__ void __launch_bounds__(P8_THREADS, 1) attention_prompt8_kernel(Prompt
     // (`fine` is the same in all lanes: the TMEM loads are the whole warp's)
     const bool fine = __all_sync(0xffffffffu, ok && (n == 0 || mbar_wait(o_done(tile), (n - 1) & 1, p.error_flag, 107)));
     asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+    s_sum[tile][half][in_tile] = l_run;
+    meet();
+    const float l_all = s_sum[tile][0][in_tile] + s_sum[tile][1][in_tile];
     if (fine) {
       if (cut.x > 1) {
         float* slot = p.partials + (((size_t)blk * Hkv + kvh) * p.parts + part) * (P8_ROWS * (D + 2));
-        if (row_ok) slot[r] = m_ref, slot[P8_ROWS + r] = l_run;
-        float* dst = slot + 2 * P8_ROWS + (size_t)r * D;
+        if (row_ok && half == 0) slot[r] = m_ref, slot[P8_ROWS + r] = l_all;
+        float* dst = slot + 2 * P8_ROWS + (size_t)r * D + HD * half;
 #pragma unroll 1
-        for (int c = 0; c < D; c += 16) {
+        for (int c = 0; c < HD; c += 16) {
           float o[16];
           if (n > 0) p8_ld16(t_o + (uint32_t)c, o), p8_ld_wait();
 #pragma unroll
@@ -436,10 +477,10 @@ __global__ void __launch_bounds__(P8_THREADS, 1) attention_prompt8_kernel(Prompt
             if (row_ok) *reinterpret_cast<float4*>(dst + c + e) = n > 0 ? make_float4(o[e], o[e + 1], o[e + 2], o[e + 3]) : make_float4(0.f, 0.f, 0.f, 0.f);
         }
       } else {
-        const float inv = l_run == 0.f ? 0.f : 1.f / l_run;
-        __nv_bfloat16* dst = p.out + (size_t)(d.q_start + tok) * p.ldo + (size_t)head * D;
+        const float inv = l_all == 0.f ? 0.f : 1.f / l_all;
+        __nv_bfloat16* dst = p.out + (size_t)(d.q_start + tok) * p.ldo + (size_t)head * D + HD * half;
 #pragma unroll 1
-        for (int c = 0; c < D; c += 16) {
+        for (int c = 0; c < HD; c += 16) {
           float o[16];
           if (n > 0) p8_ld16(t_o + (uint32_t)c, o), p8_ld_wait();
           uint32_t w[8];
@@ -456,7 +497,7 @@ __global__ void __launch_bounds__(P8_THREADS, 1) attention_prompt8_kernel(Prompt
         }
       }
     }
-  } else if (warp == 14) {
+  } else if (warp == 2) {
     // ---- scales: what the softmax needs of a page, and its rows' factors ----
     for (int j = 0; j < n_pg; ++j) {
       const int s = j % RAWS, st = j % STAGES;
@@ -518,9 +559,9 @@ __global__ void __launch_bounds__(P8_THREADS, 1) attention_prompt8_kernel(Prompt
       __syncwarp();
       if (lane == 0) mbar_arrive(fac_full(s));
     }
-  } else {
+  } else if (warp >= P8_CONVERT) {
     // ---- codes to fp16 ----
-    const int id = threadIdx.x - 10 * 32;                          // 0 .. 127
+    const int id = threadIdx.x - P8_CONVERT * 32;                          // 0 .. 127
     constexpr int UPR = D / 16, UNITS = PAGE8 * UPR / 128;         // 16-byte pieces of a row, and of a tile per thread
     for (int j = 0; j < n_pg; ++j) {
       const int s = j % RAWS, st = j % STAGES;

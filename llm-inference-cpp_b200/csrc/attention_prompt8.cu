@@ -6,9 +6,10 @@
 // A block takes 256 query rows of one sequence and kv head — tokens times the heads of the group, token by token, so that a page
 // serves the whole group — as two tiles of 128 rows, and walks the pages (64 keys) that they see:
 //
-//   raw pages     one thread copies a page's codes and scales (4 bulk copies) into a ring
 //   scales        one warp makes each row's factor of the page
-//   codes -> fp16 four warps make K' = code * (k_scale / kmax) and V' = code * (v_scale / vmax) of a page, kmax and vmax its largest
+//   codes -> fp16 four warps bring a page's codes into a ring with cp.async, each thread what it will read itself, so that nobody waits
+//                 for anybody (a thread that asks for bulk copies is busy half a microsecond with each: four a page were 2,000 clocks,
+//                 most of a page's time), and make K' = code * (k_scale / kmax) and V' = code * (v_scale / vmax) of a page, kmax and vmax its largest
 //                 scales, rounded to fp16 once (half a step is 2^-11 of a number; a bf16 cache's is 2^-8), in the swizzled layout
 //                 that the products read; so the scales cost the softmax nothing per key: kmax joins its scale, log2 vmax its offset.
 //                 (A page whose scales are more than 2^12 apart would lose bits of its small rows, which may be all that a query
@@ -26,18 +27,21 @@
 // row in a workspace; a second kernel joins them in order.  Waits are bounded (sm100.cuh).
 #include <math.h>
 
+#include "mma_sync.cuh"
 #include "rows8.cuh"
 #include "tc_common.cuh"
 
 namespace llmi {
 
 constexpr int P8_ROWS = 256, P8_TILE = 128;
-// Warps: 0 copies, 1 products, 2 scales, (3 none,) 4 .. 19 softmax (two tiles, two halves of a page's keys, four quarters of the rows),
+// Warps: 0 scales, 1 products, (2, 3 none,) 4 .. 19 softmax (two tiles, two halves of a page's keys, four quarters of the rows),
 // 20 .. 23 codes to fp16.
 constexpr int P8_SOFTMAX = 4, P8_CONVERT = 20, P8_WARPS = 24;
 constexpr int P8_THREADS = P8_WARPS * 32;
 constexpr int P8_TMEM = 512;              // per tile of rows 256 columns: S of even and odd pages (64 each), O (D)
-constexpr float P8_LAZY = 8.0f;
+constexpr float P8_LAZY = 1.0f, P8_MOST = 256.f;        // a weight beyond 2^8 moves the reference maximum where that is 1 behind
+constexpr uint32_t PG_WIDE = 1u, PG_POISON = 2u;       // the page's scales are far apart; it has values that are no numbers
+constexpr float P8_LIGHT = 8.077935669463161e-28f;     // 2^-90
 constexpr float P8_APART = 2.44140625e-4f;             // 2^-12
 constexpr float P8_TINY = 7.888609052210118e-31f;      // 2^-100: smaller scales of a page count as this
 
@@ -67,8 +71,8 @@ struct P8Cfg {
   static constexpr int Q_TILE = SUBS * P8_TILE * 128;     // bytes of a tile's queries
   static constexpr int KV_TILE = SUBS * PAGE8 * 128;      // bytes of a page's K' or V'
   static constexpr int STAGE = 2 * KV_TILE, STAGES = 3;
-  static constexpr int RAW = 2 * PAGE8 * D + 2 * PAGE8 * 4, RAWS = D == 64 ? 5 : 3;
-  static constexpr int SMEM = 1024 + 2 * Q_TILE + STAGES * STAGE + RAWS * RAW + 272;
+  static constexpr int RAW = 2 * PAGE8 * D, RAWS = D == 64 ? 4 : 3;      // codes of a page; pages under way
+  static constexpr int SMEM = 1024 + 2 * Q_TILE + STAGES * STAGE + RAWS * RAW + 176;
 };
 
 // Block b of the step's blocks of 256 rows, counted from the last block of the last sequence backwards (late blocks see more keys and
@@ -164,33 +168,31 @@ __device__ __forceinline__ uint32_t elect_one() {
   return one;
 }
 __device__ __forceinline__ uint32_t half2_bits(__half2 h) { return *reinterpret_cast<uint32_t*>(&h); }
+__device__ __forceinline__ __half2 bits_half2(uint32_t w) { return *reinterpret_cast<__half2*>(&w); }
 
 template <int D, int HELD>
 __global__ void __launch_bounds__(P8_THREADS, 1) attention_prompt8_kernel(Prompt8Params p) {
   using C = P8Cfg<D>;
-  constexpr int SUBS = C::SUBS, STAGES = C::STAGES, RAWS = C::RAWS;
+  constexpr int STAGES = C::STAGES, RAWS = C::RAWS;
   extern __shared__ uint8_t smem_raw[];
   const uint32_t base = (smem_u32(smem_raw) + 1023u) & ~1023u;
   uint8_t* const base_p = smem_raw + (base - smem_u32(smem_raw));
   const uint32_t q_smem = base, kv_smem = q_smem + 2 * C::Q_TILE, raw_smem = kv_smem + STAGES * C::STAGE, bars = raw_smem + RAWS * C::RAW;
-  const uint32_t q_full = bars, tmem_slot = bars + 264;
-  auto raw_full = [&](int s) { return bars + 8u * (1 + s); };
-  auto raw_empty = [&](int s) { return bars + 8u * (1 + RAWS + s); };
-  auto kv_full = [&](int s) { return bars + 8u * (1 + 2 * RAWS + s); };
-  auto kv_empty = [&](int s) { return bars + 8u * (1 + 2 * RAWS + STAGES + s); };
-  auto s_full = [&](int tile, int b) { return bars + 8u * (1 + 2 * RAWS + 2 * STAGES + 2 * tile + b); };
-  auto p_ready = [&](int tile, int b) { return bars + 8u * (5 + 2 * RAWS + 2 * STAGES + 2 * tile + b); };
-  auto o_done = [&](int tile) { return bars + 8u * (9 + 2 * RAWS + 2 * STAGES + tile); };
-  auto fac_full = [&](int s) { return bars + 8u * (11 + 2 * RAWS + 2 * STAGES + s); };
-  static_assert(8 * (11 + 3 * RAWS + 2 * STAGES) <= 264, "barriers fit");
-  __shared__ uint2 s_fac[RAWS][PAGE8];                   // a raw row's factors, each the sum of two fp16 numbers: of its keys, of its values
-  __shared__ uint32_t s_none[RAWS][4];                   // rows whose key codes, and whose value codes, may be no numbers
-  __shared__ int s_known[RAWS];                          // the raw page is one of the pool
-  __shared__ float s_page[STAGES][4];                    // kmax, log2 vmax, 1 / vmax
+  const uint32_t q_full = bars, tmem_slot = bars + 168;
+  auto fac_full = [&](int s) { return bars + 8u * (1 + s); };
+  auto kv_full = [&](int s) { return bars + 8u * (1 + STAGES + s); };
+  auto kv_empty = [&](int s) { return bars + 8u * (1 + 2 * STAGES + s); };
+  auto s_full = [&](int tile, int b) { return bars + 8u * (1 + 3 * STAGES + 2 * tile + b); };
+  auto p_ready = [&](int tile, int b) { return bars + 8u * (5 + 3 * STAGES + 2 * tile + b); };
+  auto o_done = [&](int tile) { return bars + 8u * (9 + 3 * STAGES + tile); };
+  static_assert(8 * (11 + 3 * STAGES) <= 168, "barriers fit");
+  __shared__ float s_scales[RAWS][2 * PAGE8];            // pages under way: scales of keys, of values
+  __shared__ uint2 s_fac[STAGES][PAGE8];                 // a row's factors, each the sum of two fp16 numbers: of its keys, of its values
+  __shared__ uint32_t s_none[STAGES][4];                 // rows whose key codes, and whose value codes, may be no numbers
+  __shared__ float4 s_page[STAGES];                      // kmax, log2 vmax, 1 / vmax, whether the page needs a look (PG_*, as bits)
   __shared__ uint32_t s_poison[STAGES][2];               // keys whose values are no numbers
-  __shared__ float s_top[2][2][2][P8_TILE];              // [page parity][tile][half][row]: the largest score of a row's half
+  __shared__ float s_top[2][2][P8_TILE];                 // [tile][half][row]: the largest score of a row's half
   __shared__ float s_sum[2][2][P8_TILE];
-  __shared__ int s_wide[STAGES];                         // the page's scales are far apart: its keys' own
   __shared__ float s_key[STAGES][2][PAGE8];              // k_scale, log2 v_scale
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -218,8 +220,7 @@ __global__ void __launch_bounds__(P8_THREADS, 1) attention_prompt8_kernel(Prompt
 
   if (threadIdx.x == 0) {
     mbar_init(q_full, 16);
-    for (int s = 0; s < RAWS; ++s) mbar_init(raw_full(s), 1), mbar_init(raw_empty(s), 4), mbar_init(fac_full(s), 1);
-    for (int s = 0; s < STAGES; ++s) mbar_init(kv_full(s), 4), mbar_init(kv_empty(s), 1);
+    for (int s = 0; s < STAGES; ++s) mbar_init(fac_full(s), 1), mbar_init(kv_full(s), 4), mbar_init(kv_empty(s), 1);
     for (int i = 0; i < 2; ++i) {
       for (int b = 0; b < 2; ++b) mbar_init(s_full(i, b), 1), mbar_init(p_ready(i, b), 8);
       mbar_init(o_done(i), 1);
@@ -237,29 +238,85 @@ __global__ void __launch_bounds__(P8_THREADS, 1) attention_prompt8_kernel(Prompt
   asm volatile("ld.shared.u32 %0, [%1];" : "=r"(tmem) : "r"(tmem_slot));
   pdl_launch_dependents();      // (not ahead of the tensor memory: a kernel behind this one could take it and wait for this block)
 
+  // the page of the pool that page j of this part is, or -1
+  const int32_t* table = p.kv.seq_pages + (size_t)d.seq * p.kv.pages_stride;
+  auto page_at = [&](int j) {
+    const int at = pg0 + j, page = j < n_pg && at < p.kv.table_pages ? table[at] : -1;
+    return (unsigned)page < (unsigned)p.kv.n_pages ? page : -1;
+  };
   if (warp == 0) {
-    if (lane == 0) {
-      // ---- raw pages ----
-      const int32_t* pages = p.kv.seq_pages + (size_t)d.seq * p.kv.pages_stride;
-      for (int j = 0; j < n_pg; ++j) {
-        const int s = j % RAWS, at = pg0 + j;
-        const int page = at < p.kv.table_pages ? pages[at] : -1;
-        if (j >= RAWS && !mbar_wait(raw_empty(s), ((j / RAWS) - 1) & 1, p.error_flag, 101)) break;
-        const bool known = (unsigned)page < (unsigned)p.kv.n_pages;
-        s_known[s] = known;
-        if (known) {
-          const uint32_t st = raw_smem + s * C::RAW;
-          const size_t row = ((size_t)page * Hkv + kvh) * PAGE8;
-          mbar_expect_tx(raw_full(s), C::RAW);
-          bulk_load(st, p.k_codes + row * D, PAGE8 * D, raw_full(s));
-          bulk_load(st + PAGE8 * D, p.v_codes + row * D, PAGE8 * D, raw_full(s));
-          bulk_load(st + 2 * PAGE8 * D, p.k_scales + row, PAGE8 * 4, raw_full(s));
-          bulk_load(st + 2 * PAGE8 * D + PAGE8 * 4, p.v_scales + row, PAGE8 * 4, raw_full(s));
-        } else {
-          mbar_arrive(raw_full(s));
-        }
+    // ---- scales: what the softmax needs of a page, and its rows' factors ----
+    int under_way[RAWS], next = page_at(0);
+    auto ask = [&](int j) {                                        // lanes 0 .. 15: the keys' scales, the others: the values'
+      const int page = next;
+      next = page_at(j + 1);
+      const size_t row = ((size_t)max(page, 0) * Hkv + kvh) * PAGE8 + (lane & 15) * 4;
+      cp_async16(&s_scales[j % RAWS][lane * 4], (lane < 16 ? p.k_scales : p.v_scales) + row, 16);
+      cp_async_commit();
+      return page;
+    };
+#pragma unroll
+    for (int i = 0; i < RAWS - 1; ++i) under_way[i] = ask(i);
+    int st = 0;
+    uint32_t phase = 1u;
+    for (int j = 0; j < n_pg; ++j) {
+      under_way[RAWS - 1] = ask(j + RAWS - 1);
+      cp_async_wait<RAWS - 1>();
+      __syncwarp();
+      const float* ks = s_scales[j % RAWS];
+      const bool known = under_way[0] >= 0;
+#pragma unroll
+      for (int i = 0; i < RAWS - 1; ++i) under_way[i] = under_way[i + 1];
+      const int a = max(d.lo - (pg0 + j) * PAGE8, 0), b = min(d.last - (pg0 + j) * PAGE8, 63);      // rows that some query sees
+      // the page's largest scales (of rows that are numbers), the least but zeros, and its rows that are no numbers
+      float x[2], y[2], km = 0.f, vm = 0.f, kn = INFINITY, vn = INFINITY;
+      uint32_t bad[2], out[2];
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        const int r = lane + 32 * h;
+        const bool in = r >= a && r <= b;
+        x[h] = in && known ? ks[r] : 0.f;
+        y[h] = in ? (known ? ks[PAGE8 + r] : __int_as_float(0x7fffffff)) : 0.f;
+        const float fx = finite8(x[h]) ? fabsf(x[h]) : 0.f, fy = finite8(y[h]) ? fabsf(y[h]) : 0.f;
+        km = fmaxf(km, fx), vm = fmaxf(vm, fy);
+        if (fx != 0.f) kn = fminf(kn, fx);
+        if (fy != 0.f) vn = fminf(vn, fy);
+        bad[h] = __ballot_sync(0xffffffffu, !finite8(y[h]));
+        out[h] = __ballot_sync(0xffffffffu, !(in && known));
       }
+      // (numbers that are not negative are ordered as their bits are)
+      km = fmaxf(__uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(km))), P8_TINY);
+      vm = fmaxf(__uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(vm))), P8_TINY);
+      const bool wide = __any_sync(0xffffffffu, kn < km * P8_APART || vn < vm * P8_APART);
+      const float k_inv = __frcp_rn(km), v_inv = __frcp_rn(vm), lv = wide ? 0.f : fast_log2(vm);
+      // (the softmax is done with what is there of the page three before)
+      if (j >= STAGES && !mbar_wait(kv_empty(st), phase, p.error_flag, 109)) break;
+      if (lane == 0) {
+        s_page[st] = make_float4(km, lv, v_inv, __uint_as_float((wide ? PG_WIDE : 0u) | ((bad[0] | bad[1]) ? PG_POISON : 0u)));
+        s_poison[st][0] = bad[0];
+        s_poison[st][1] = bad[1];
+        s_none[st][0] = out[0], s_none[st][1] = out[1], s_none[st][2] = out[0] | bad[0], s_none[st][3] = out[1] | bad[1];
+      }
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        const int r = lane + 32 * h;
+        float kf = x[h] * k_inv, vf = finite8(y[h]) ? y[h] * v_inv : 0.f;
+        if (wide) {
+          const float own = fmaxf(y[h], P8_TINY);                          // (a NaN's values are zeros here: its bit is in s_poison)
+          s_key[st][0][r] = x[h];
+          s_key[st][1][r] = log2f(own);
+          kf = 1.f;
+          vf = finite8(y[h]) ? y[h] / own : 0.f;
+        }
+        const __half kh = __float2half_rn(kf), vh = __float2half_rn(vf);
+        s_fac[st][r] = make_uint2(half2_bits(__halves2half2(kh, __float2half_rn(kf - __half2float(kh)))),
+                                 half2_bits(__halves2half2(vh, __float2half_rn(vf - __half2float(vh)))));
+      }
+      __syncwarp();
+      if (lane == 0) mbar_arrive(fac_full(st));
+      if (++st == STAGES) st = 0, phase ^= 1u;
     }
+    cp_async_wait_all();
   } else if (warp == 1) {
     // ---- products ----
     // S: A = Q' (K-major), B = K' (K-major), 64 columns; O: A = P (tensor memory, 32 columns of fp16 pairs), B = V' (MN-major, sub-tiles
@@ -324,6 +381,12 @@ __global__ void __launch_bounds__(P8_THREADS, 1) attention_prompt8_kernel(Prompt
     const int pos_a = __shfl_sync(0xffffffffu, qpos, 0), pos_b = __shfl_sync(0xffffffffu, qpos, 31);      // the warp's first and last
     // what the two threads of a row tell each other: 64 threads meet
     auto meet = [&]() { asm volatile("bar.sync %0, 64;" ::"r"(1 + tile * 4 + quad) : "memory"); };
+    auto any_of_pair = [&](bool x) {
+      uint32_t r;
+      asm volatile("{\n\t.reg .pred p, q;\n\tsetp.ne.b32 p, %2, 0;\n\tbarrier.cta.red.or.pred q, %1, 64, p;\n\tselp.u32 %0, 1, 0, q;\n\t}"
+                   : "=r"(r) : "r"(1 + tile * 4 + quad), "r"(x ? 1u : 0u) : "memory");
+      return r != 0u;
+    };
     // the row's queries, divided by a power of two above the largest
     float row_fac;
     {
@@ -366,7 +429,9 @@ __global__ void __launch_bounds__(P8_THREADS, 1) attention_prompt8_kernel(Prompt
     }
     const int n = n_tile[tile];
     const uint32_t t_lane = (uint32_t)(quad * 32) << 16, t_tile = tmem + 256u * tile + t_lane, t_o = t_tile + 128u + (uint32_t)(HD * half);
-    float m_run = -INFINITY, m_ref = -INFINITY, l_run = 0.f;       // of s + log2 vmax, base 2; the sum of 2^(s - m_ref) over this half
+    // the reference maximum (of s + log2 vmax, base 2) and 0 less it (0 while there is none); the sum of 2^(s - m_ref) over this half, and
+    // over the other one when they last met
+    float m_ref = -INFINITY, neg_ref = 0.f, l_run = 0.f, l_other = 0.f;
     bool ok = true;
     int st = 0;                                                    // j % STAGES
     // (after a wait that gave up the pages are gone through without waiting: the two threads of a row go on meeting)
@@ -378,12 +443,13 @@ __global__ void __launch_bounds__(P8_THREADS, 1) attention_prompt8_kernel(Prompt
       float sc[32];
       p8_ld16(t_s, sc);
       p8_ld16(t_s + 16u, sc + 16);
-      const bool wide = s_wide[st] != 0;
-      const float to_log2 = wide ? 1.f : row_fac * s_page[st][0], lv = s_page[st][1], inv_v = s_page[st][2];
-      const uint32_t bad = s_poison[st][half];
+      const float4 page = s_page[st];
+      const uint32_t look = __float_as_uint(page.w);
       const int key0 = (pg0 + j) * PAGE8 + 32 * half;
+      float to_log2 = row_fac * page.x, off = page.y + neg_ref;
       p8_ld_wait();
-      if (wide) {                                                  // (kmax 1 / row_fac, vmax 1: the scores are final)
+      if (look & PG_WIDE) {                                        // (kmax 1 / row_fac, vmax 1: the scores are final)
+        to_log2 = 1.f;
 #pragma unroll
         for (int c = 0; c < 32; ++c) sc[c] = fmaf(sc[c], row_fac * s_key[st][0][32 * half + c], s_key[st][1][32 * half + c]);
       }
@@ -393,45 +459,69 @@ __global__ void __launch_bounds__(P8_THREADS, 1) attention_prompt8_kernel(Prompt
         for (int c = 0; c < 32; ++c)
           if (c > b || c < a) sc[c] = -INFINITY;
       }
-      float mx4[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
-#pragma unroll
-      for (int c = 0; c < 32; c += 8)
-#pragma unroll
-        for (int u = 0; u < 4; ++u) mx4[u] = fmaxf(mx4[u], fmaxf(sc[c + 2 * u], sc[c + 2 * u + 1]));
-      float top = fmaf(fmaxf(fmaxf(mx4[0], mx4[1]), fmaxf(mx4[2], mx4[3])), to_log2, lv);
-      s_top[j & 1][tile][half][in_tile] = top;
-      meet();
-      top = fmaxf(top, s_top[j & 1][tile][half ^ 1][in_tile]);
-      m_run = fmaxf(m_run, top);
-      float corr = 1.f;
-      if (m_run > m_ref + P8_LAZY || m_ref == -INFINITY) {         // (both -inf: nothing seen yet)
-        corr = m_ref == -INFINITY ? 0.f : fast_exp2(m_ref - m_run);
-        if (m_ref != -INFINITY) l_run = rescale8(l_run, m_ref - m_run);
-        m_ref = m_run;
-      }
-      const float off = m_ref == -INFINITY ? 0.f : lv - m_ref;
-      float2 sum2[4] = {{0.f, 0.f}, {0.f, 0.f}, {0.f, 0.f}, {0.f, 0.f}};
-      const float2 scale2 = make_float2(to_log2, to_log2), off2 = make_float2(off, off);
       uint32_t packed[16];
+      float sum;
+      __half2 top2;
+      auto weigh = [&]() {
+        float2 sum2[4] = {{0.f, 0.f}, {0.f, 0.f}, {0.f, 0.f}, {0.f, 0.f}};
+        __half2 t2[2] = {__half2half2(__ushort_as_half(0)), __half2half2(__ushort_as_half(0))};
+        const float2 scale2 = make_float2(to_log2, to_log2), off2 = make_float2(off, off);
 #pragma unroll
-      for (int c = 0; c < 32; c += 2) {
-        const float2 x = __ffma2_rn(make_float2(sc[c], sc[c + 1]), scale2, off2);
-        const float2 e = make_float2(fast_exp2(x.x), fast_exp2(x.y));
-        sum2[(c >> 1) & 3] = __fadd2_rn(sum2[(c >> 1) & 3], e);
-        packed[c >> 1] = half2_bits(__floats2half2_rn(e.x, e.y));
-      }
-      // The sum of w is that of P / vmax, unless all of P is so small that it may have lost some of it (values far smaller than those of
-      // another page, zeros for instance, say nothing about their weights).
-      if (!__any_sync(0xffffffffu, wide || top < m_ref - 64.f)) {
+        for (int c = 0; c < 32; c += 2) {
+          const float2 x = __ffma2_rn(make_float2(sc[c], sc[c + 1]), scale2, off2);
+          const float2 e = make_float2(fast_exp2(x.x), fast_exp2(x.y));
+          sum2[(c >> 1) & 3] = __fadd2_rn(sum2[(c >> 1) & 3], e);
+          const __half2 h = __floats2half2_rn(e.x, e.y);
+          t2[(c >> 1) & 1] = __hmax2(t2[(c >> 1) & 1], h);
+          packed[c >> 1] = half2_bits(h);
+        }
         const float2 s = __fadd2_rn(__fadd2_rn(sum2[0], sum2[1]), __fadd2_rn(sum2[2], sum2[3]));
-        l_run = fmaf(s.x + s.y, inv_v, l_run);
-      } else {
+        sum = s.x + s.y;
+        top2 = __hmax2(t2[0], t2[1]);
+      };
+      weigh();
+      // The common page: no weight has outgrown the reference maximum, and the sum of w is that of P / vmax.  Otherwise both threads of
+      // every row of the two warps go the long way.
+      float corr = 1.f;
+      const bool rare = m_ref == -INFINITY || fmaxf(__low2float(top2), __high2float(top2)) > P8_MOST || page.z * P8_LIGHT > l_run + l_other || look != 0u;
+      if (any_of_pair(rare)) {
+        float mx = -INFINITY;
 #pragma unroll
-        for (int c = 0; c < 32; ++c) l_run += fast_exp2(fmaf(sc[c], to_log2, off) - (wide ? s_key[st][1][32 * half + c] : lv));
-      }
-      if (bad) {                                                   // values that are no numbers: for the rows that see them
-        const int a = p.window > 0 ? max(qpos - p.window + 1 - key0, 0) : 0, b = min(qpos - key0, 31);
-        if (a <= b && ((bad >> a) << (31 - (b - a)))) l_run = __int_as_float(0x7fffffff);
+        for (int c = 0; c < 32; ++c) mx = fmaxf(mx, sc[c]);
+        float top = fmaf(mx, to_log2, page.y);
+        s_top[tile][half][in_tile] = top;
+        s_sum[tile][half][in_tile] = l_run;
+        meet();
+        top = fmaxf(top, s_top[tile][half ^ 1][in_tile]);
+        l_other = s_sum[tile][half ^ 1][in_tile];
+        meet();
+        if (top > m_ref + P8_LAZY || m_ref == -INFINITY) {         // (both -inf: nothing seen yet)
+          if (m_ref != -INFINITY) {
+            corr = fast_exp2(m_ref - top);
+            l_run = rescale8(l_run, m_ref - top);
+            l_other = rescale8(l_other, m_ref - top);
+          }
+          m_ref = top;
+          neg_ref = top == -INFINITY ? 0.f : -top;
+        }
+        off = page.y + neg_ref;
+        weigh();
+        // The sum of w key by key where P may have lost some of it: in a page whose values are far smaller than another page's (zeros, for
+        // instance, say nothing about their weights).
+        if (__any_sync(0xffffffffu, look != 0u || page.z * P8_LIGHT > l_run + l_other)) {
+          const bool wide = (look & PG_WIDE) != 0u;
+#pragma unroll
+          for (int c = 0; c < 32; ++c) l_run += fast_exp2(fmaf(sc[c], to_log2, off) - (wide ? s_key[st][1][32 * half + c] : page.y));
+        } else {
+          l_run = fmaf(sum, page.z, l_run);
+        }
+        const uint32_t bad = s_poison[st][half];
+        if (bad) {                                                 // values that are no numbers: for the rows that see them
+          const int a = p.window > 0 ? max(qpos - p.window + 1 - key0, 0) : 0, b = min(qpos - key0, 31);
+          if (a <= b && ((bad >> a) << (31 - (b - a)))) l_run = __int_as_float(0x7fffffff);
+        }
+      } else {
+        l_run = fmaf(sum, page.z, l_run);
       }
       if (j >= 1) {
         // (waited for on every page: a wait on a phase's parity is right only for a thread at most one phase behind)
@@ -497,116 +587,84 @@ __global__ void __launch_bounds__(P8_THREADS, 1) attention_prompt8_kernel(Prompt
         }
       }
     }
-  } else if (warp == 2) {
-    // ---- scales: what the softmax needs of a page, and its rows' factors ----
-    for (int j = 0; j < n_pg; ++j) {
-      const int s = j % RAWS, st = j % STAGES;
-      if (!mbar_wait(raw_full(s), (j / RAWS) & 1, p.error_flag, 108)) break;
-      const float* ks = reinterpret_cast<const float*>(base_p + (raw_smem - base) + s * C::RAW + 2 * PAGE8 * D);
-      const bool known = s_known[s] != 0;
-      const int a = max(d.lo - (pg0 + j) * PAGE8, 0), b = min(d.last - (pg0 + j) * PAGE8, 63);      // rows that some query sees
-      // the page's largest scales (of rows that are numbers), the least but zeros, and its rows that are no numbers
-      float x[2], y[2], km = 0.f, vm = 0.f, kn = INFINITY, vn = INFINITY;
-      uint32_t bad[2], out[2];
-#pragma unroll
-      for (int h = 0; h < 2; ++h) {
-        const int r = lane + 32 * h;
-        const bool in = r >= a && r <= b;
-        x[h] = in && known ? ks[r] : 0.f;
-        y[h] = in ? (known ? ks[PAGE8 + r] : __int_as_float(0x7fffffff)) : 0.f;
-        const float fx = finite8(x[h]) ? fabsf(x[h]) : 0.f, fy = finite8(y[h]) ? fabsf(y[h]) : 0.f;
-        km = fmaxf(km, fx), vm = fmaxf(vm, fy);
-        if (fx != 0.f) kn = fminf(kn, fx);
-        if (fy != 0.f) vn = fminf(vn, fy);
-        bad[h] = __ballot_sync(0xffffffffu, !finite8(y[h]));
-        out[h] = __ballot_sync(0xffffffffu, !(in && known));
-      }
-#pragma unroll
-      for (int o = 16; o > 0; o >>= 1) {
-        km = fmaxf(km, __shfl_xor_sync(0xffffffffu, km, o));
-        vm = fmaxf(vm, __shfl_xor_sync(0xffffffffu, vm, o));
-      }
-      km = fmaxf(km, P8_TINY);
-      vm = fmaxf(vm, P8_TINY);
-      const bool wide = __any_sync(0xffffffffu, kn < km * P8_APART || vn < vm * P8_APART);
-      const float k_inv = 1.f / km, v_inv = 1.f / vm;
-      // (the softmax is done with what is there of the page three before)
-      if (j >= STAGES && !mbar_wait(kv_empty(st), ((j / STAGES) - 1) & 1, p.error_flag, 109)) break;
-      if (lane == 0) {
-        s_page[st][0] = km;
-        s_page[st][1] = wide ? 0.f : log2f(vm);
-        s_page[st][2] = v_inv;
-        s_poison[st][0] = bad[0];
-        s_poison[st][1] = bad[1];
-        s_wide[st] = wide;
-        s_none[s][0] = out[0], s_none[s][1] = out[1], s_none[s][2] = out[0] | bad[0], s_none[s][3] = out[1] | bad[1];
-      }
-#pragma unroll
-      for (int h = 0; h < 2; ++h) {
-        const int r = lane + 32 * h;
-        float kf = x[h] * k_inv, vf = finite8(y[h]) ? y[h] * v_inv : 0.f;
-        if (wide) {
-          const float own = fmaxf(y[h], P8_TINY);                          // (a NaN's values are zeros here: its bit is in s_poison)
-          s_key[st][0][r] = x[h];
-          s_key[st][1][r] = log2f(own);
-          kf = 1.f;
-          vf = finite8(y[h]) ? y[h] / own : 0.f;
-        }
-        const __half kh = __float2half_rn(kf), vh = __float2half_rn(vf);
-        s_fac[s][r] = make_uint2(half2_bits(__halves2half2(kh, __float2half_rn(kf - __half2float(kh)))),
-                                 half2_bits(__halves2half2(vh, __float2half_rn(vf - __half2float(vh)))));
-      }
-      __syncwarp();
-      if (lane == 0) mbar_arrive(fac_full(s));
-    }
   } else if (warp >= P8_CONVERT) {
     // ---- codes to fp16 ----
     const int id = threadIdx.x - P8_CONVERT * 32;                          // 0 .. 127
     constexpr int UPR = D / 16, UNITS = PAGE8 * UPR / 128;         // 16-byte pieces of a row, and of a tile per thread
-    for (int j = 0; j < n_pg; ++j) {
-      const int s = j % RAWS, st = j % STAGES;
-      if (!mbar_wait(fac_full(s), (j / RAWS) & 1, p.error_flag, 110)) break;      // (the raw page is here, and the stage is free)
-      const uint8_t* raw = base_p + (raw_smem - base) + s * C::RAW;
-      const uint32_t k_dst = kv_smem + st * C::STAGE, v_dst = k_dst + C::KV_TILE;
-      const bool some = HELD == HELD_E4M3 && (s_none[s][2] | s_none[s][3]) != 0u;      // (any int8 code times 0 is 0)
+    int next = page_at(0), slot = 0;                               // the slot of the ring filled next
+    auto ask = [&](int j) {
+      const int page = next;
+      next = page_at(j + 1);
+      uint8_t* raw = base_p + (raw_smem - base) + slot * C::RAW;
+      const size_t row = ((size_t)max(page, 0) * Hkv + kvh) * PAGE8 * D;
 #pragma unroll
       for (int i = 0; i < UNITS; ++i) {
-        const int x = id + 128 * i, r = x / UPR, u = x % UPR;
-        uint4 kw = *reinterpret_cast<const uint4*>(raw + x * 16), vw = *reinterpret_cast<const uint4*>(raw + PAGE8 * D + x * 16);
-        const uint2 f = s_fac[s][r];
-        if (some) {
-          if ((s_none[s][r >> 5] >> (r & 31)) & 1u) kw = make_uint4(0u, 0u, 0u, 0u);
-          if ((s_none[s][2 + (r >> 5)] >> (r & 31)) & 1u) vw = make_uint4(0u, 0u, 0u, 0u);
-        }
-        const __half2 kf = *reinterpret_cast<const __half2*>(&f.x), vf = *reinterpret_cast<const __half2*>(&f.y);
-        const __half2 kh2 = __low2half2(kf), kl2 = __high2half2(kf), vh2 = __low2half2(vf), vl2 = __high2half2(vf);
-        const uint32_t* kp = &kw.x;
-        const uint32_t* vp = &vw.x;
-        const uint32_t at = (u / 4) * (PAGE8 * 128) + r * 128;
+        const int x = (id + 128 * i) * 16;
+        cp_async16(raw + x, p.k_codes + row + x, page >= 0 ? 16 : 0);
+        cp_async16(raw + PAGE8 * D + x, p.v_codes + row + x, page >= 0 ? 16 : 0);
+      }
+      cp_async_commit();
+      slot = slot + 1 == RAWS ? 0 : slot + 1;
+    };
 #pragma unroll
-        for (int h = 0; h < 2; ++h) {                                       // eight codes: 16 bytes of fp16
-          uint32_t kx[4], vx[4];
+    for (int i = 0; i < RAWS - 1; ++i) ask(i);
+    int st = 0, s = 0;
+    uint32_t phase = 0;
+    for (int j = 0; j < n_pg; ++j) {
+      ask(j + RAWS - 1);                                           // (into the slot that this thread has read last)
+      cp_async_wait<RAWS - 1>();
+      if (!mbar_wait(fac_full(st), phase, p.error_flag, 110)) break;       // (the stage is free, too)
+      const uint8_t* raw = base_p + (raw_smem - base) + s * C::RAW;
+      s = s + 1 == RAWS ? 0 : s + 1;
+      const uint32_t k_dst = kv_smem + st * C::STAGE, v_dst = k_dst + C::KV_TILE;
+      const bool some = HELD == HELD_E4M3 && (s_none[st][2] | s_none[st][3]) != 0u;     // (any int8 code times 0 is 0)
 #pragma unroll
-          for (int w = 0; w < 2; ++w) {                                     // a product is rounded once
-            const __half2 k0 = halves8<HELD>(kp[2 * h + w] & 0xffffu), k1 = halves8<HELD>(kp[2 * h + w] >> 16);
-            const __half2 v0h = halves8<HELD>(vp[2 * h + w] & 0xffffu), v1h = halves8<HELD>(vp[2 * h + w] >> 16);
-            kx[2 * w] = half2_bits(__hfma2(k0, kh2, __hmul2(k0, kl2)));
-            kx[2 * w + 1] = half2_bits(__hfma2(k1, kh2, __hmul2(k1, kl2)));
-            vx[2 * w] = half2_bits(__hfma2(v0h, vh2, __hmul2(v0h, vl2)));
-            vx[2 * w + 1] = half2_bits(__hfma2(v1h, vh2, __hmul2(v1h, vl2)));
+      for (int i0 = 0; i0 < UNITS; i0 += 2) {                               // two pieces of keys and of values at a time
+        uint4 kw[2], vw[2];
+        uint2 f[2];
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+          const int x = id + 128 * (i0 + i), r = x / UPR;
+          kw[i] = *reinterpret_cast<const uint4*>(raw + x * 16), vw[i] = *reinterpret_cast<const uint4*>(raw + PAGE8 * D + x * 16);
+          f[i] = s_fac[st][r];
+          if (some) {
+            if ((s_none[st][r >> 5] >> (r & 31)) & 1u) kw[i] = make_uint4(0u, 0u, 0u, 0u);
+            if ((s_none[st][2 + (r >> 5)] >> (r & 31)) & 1u) vw[i] = make_uint4(0u, 0u, 0u, 0u);
           }
-          const uint32_t o = at + (((2 * (u % 4) + h) ^ (r & 7)) << 4);
-          asm volatile("st.shared.v4.u32 [%0], {%1, %2, %3, %4};" ::"r"(k_dst + o), "r"(kx[0]), "r"(kx[1]), "r"(kx[2]), "r"(kx[3]) : "memory");
-          asm volatile("st.shared.v4.u32 [%0], {%1, %2, %3, %4};" ::"r"(v_dst + o), "r"(vx[0]), "r"(vx[1]), "r"(vx[2]), "r"(vx[3]) : "memory");
+        }
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+          const int x = id + 128 * (i0 + i), r = x / UPR, u = x % UPR;
+          const __half2 kf = *reinterpret_cast<const __half2*>(&f[i].x), vf = *reinterpret_cast<const __half2*>(&f[i].y);
+          const __half2 kh2 = __low2half2(kf), kl2 = __high2half2(kf), vh2 = __low2half2(vf), vl2 = __high2half2(vf);
+          const uint32_t* kp = &kw[i].x;
+          const uint32_t* vp = &vw[i].x;
+          const uint32_t at = (u / 4) * (PAGE8 * 128) + r * 128;
+#pragma unroll
+          for (int h = 0; h < 2; ++h) {                                     // eight codes: 16 bytes of fp16
+            uint32_t kx[4], vx[4];
+#pragma unroll
+            for (int w = 0; w < 2; ++w) {                                   // a product is rounded once
+              uint32_t k0, k1, v0h, v1h;
+              halves8x4<HELD>(kp[2 * h + w], k0, k1);
+              halves8x4<HELD>(vp[2 * h + w], v0h, v1h);
+              kx[2 * w] = half2_bits(__hfma2(bits_half2(k0), kh2, __hmul2(bits_half2(k0), kl2)));
+              kx[2 * w + 1] = half2_bits(__hfma2(bits_half2(k1), kh2, __hmul2(bits_half2(k1), kl2)));
+              vx[2 * w] = half2_bits(__hfma2(bits_half2(v0h), vh2, __hmul2(bits_half2(v0h), vl2)));
+              vx[2 * w + 1] = half2_bits(__hfma2(bits_half2(v1h), vh2, __hmul2(bits_half2(v1h), vl2)));
+            }
+            const uint32_t o = at + (((2 * (u % 4) + h) ^ (r & 7)) << 4);
+            asm volatile("st.shared.v4.u32 [%0], {%1, %2, %3, %4};" ::"r"(k_dst + o), "r"(kx[0]), "r"(kx[1]), "r"(kx[2]), "r"(kx[3]));
+            asm volatile("st.shared.v4.u32 [%0], {%1, %2, %3, %4};" ::"r"(v_dst + o), "r"(vx[0]), "r"(vx[1]), "r"(vx[2]), "r"(vx[3]));
+          }
         }
       }
-      asm volatile("fence.proxy.async.shared::cta;" ::: "memory");        // the products read what was written, and the raw page may be overwritten
+      asm volatile("fence.proxy.async.shared::cta;" ::: "memory");        // the products read what was written
       __syncwarp();
-      if (lane == 0) {
-        mbar_arrive(kv_full(st));
-        mbar_arrive(raw_empty(s));
-      }
+      if (lane == 0) mbar_arrive(kv_full(st));
+      if (++st == STAGES) st = 0, phase ^= 1u;
     }
+    cp_async_wait_all();
   }
   asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
   __syncthreads();

@@ -76,19 +76,6 @@ __device__ __forceinline__ void mma_f16(float (&c)[4], const uint32_t (&a)[4], u
                : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3]) : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
 __device__ __forceinline__ uint32_t as_u32(__half2 h) { return *reinterpret_cast<uint32_t*>(&h); }
-// Four codes as fp16 numbers: bytes 0, 1 and bytes 2, 3.
-template <int HELD> __device__ __forceinline__ void halves4(uint32_t w, uint32_t& lo, uint32_t& hi) {
-  if (HELD == HELD_INT8) {
-    const uint32_t u = w ^ 0x80808080u;
-    asm("prmt.b32 %0, %1, %2, 0x4140;" : "=r"(lo) : "r"(u), "r"(0x64646464u));
-    asm("prmt.b32 %0, %1, %2, 0x4342;" : "=r"(hi) : "r"(u), "r"(0x64646464u));
-    const __half2 bias = __halves2half2(__ushort_as_half(0x6480), __ushort_as_half(0x6480));
-    lo = as_u32(__hsub2(*reinterpret_cast<__half2*>(&lo), bias));
-    hi = as_u32(__hsub2(*reinterpret_cast<__half2*>(&hi), bias));
-  } else {
-    asm("{\n\t.reg .b16 a, b;\n\tmov.b32 {a, b}, %2;\n\tcvt.rn.f16x2.e4m3x2 %0, a;\n\tcvt.rn.f16x2.e4m3x2 %1, b;\n\t}" : "=r"(lo), "=r"(hi) : "r"(w));
-  }
-}
 __device__ __forceinline__ uint32_t transpose8x8(uint32_t v) {
   uint32_t r;
   asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(r) : "r"(v));
@@ -397,8 +384,8 @@ __global__ void __launch_bounds__(RW8_WARPS * 32, (Rw8Cfg<D, NT, T>::BLOCKS)) at
 #pragma unroll
         for (int s = 0; s < KS; ++s) {
           uint32_t a[4];
-          halves4<HELD>(ka[s], a[0], a[2]);
-          halves4<HELD>(kb[s], a[1], a[3]);
+          halves8x4<HELD>(ka[s], a[0], a[2]);
+          halves8x4<HELD>(kb[s], a[1], a[3]);
 #pragma unroll
           for (int n = 0; n < NT; ++n)
 #pragma unroll
@@ -517,10 +504,10 @@ __global__ void __launch_bounds__(RW8_WARPS * 32, (Rw8Cfg<D, NT, T>::BLOCKS)) at
           asm("prmt.b32 %0, %1, %2, 0x7362;" : "=r"(z4[1]) : "r"(vw[0][w]), "r"(vw[1][w]));
           asm("prmt.b32 %0, %1, %2, 0x5140;" : "=r"(z4[2]) : "r"(vw[2][w]), "r"(vw[3][w]));
           asm("prmt.b32 %0, %1, %2, 0x7362;" : "=r"(z4[3]) : "r"(vw[2][w]), "r"(vw[3][w]));
-          halves4<HELD>(z4[0], a01[0], a01[1]);
-          halves4<HELD>(z4[2], a01[2], a01[3]);
-          halves4<HELD>(z4[1], a23[0], a23[1]);
-          halves4<HELD>(z4[3], a23[2], a23[3]);
+          halves8x4<HELD>(z4[0], a01[0], a01[1]);
+          halves8x4<HELD>(z4[2], a01[2], a01[3]);
+          halves8x4<HELD>(z4[1], a23[0], a23[1]);
+          halves8x4<HELD>(z4[3], a23[2], a23[3]);
 #pragma unroll
           for (int n = 0; n < NT; ++n)
 #pragma unroll

@@ -82,6 +82,20 @@ template <int HELD> __device__ __forceinline__ __half2 halves8(uint32_t w) {
   asm("cvt.rn.f16x2.e4m3x2 %0, %1;" : "=r"(r) : "h"((uint16_t)w));
   return *reinterpret_cast<__half2*>(&r);
 }
+// Four codes as fp16 numbers, exactly: bytes 0, 1 and bytes 2, 3.
+template <int HELD> __device__ __forceinline__ void halves8x4(uint32_t w, uint32_t& lo, uint32_t& hi) {
+  if (HELD == HELD_INT8) {
+    const uint32_t u = w ^ 0x80808080u;
+    asm("prmt.b32 %0, %1, %2, 0x4140;" : "=r"(lo) : "r"(u), "r"(0x64646464u));
+    asm("prmt.b32 %0, %1, %2, 0x4342;" : "=r"(hi) : "r"(u), "r"(0x64646464u));
+    const __half2 bias = __halves2half2(__ushort_as_half(0x6480), __ushort_as_half(0x6480));
+    const __half2 l = __hsub2(*reinterpret_cast<__half2*>(&lo), bias), h = __hsub2(*reinterpret_cast<__half2*>(&hi), bias);
+    lo = *reinterpret_cast<const uint32_t*>(&l), hi = *reinterpret_cast<const uint32_t*>(&h);
+  } else {
+    asm("{\n\t.reg .b16 a, b;\n\tmov.b32 {a, b}, %2;\n\tcvt.rn.f16x2.e4m3x2 %0, a;\n\tcvt.rn.f16x2.e4m3x2 %1, b;\n\t}" : "=r"(lo), "=r"(hi) : "r"(w));
+  }
+}
+
 // A sum of weights relative to a maximum that is `down` >= 0 below the new one (base 2).  In two steps: the maxima are those of score +
 // log2 of a value's scale, so the factor alone may be below what fp32 has where the sum times it is not.
 __device__ __forceinline__ float rescale8(float sum, float down) {

@@ -39,7 +39,7 @@ constexpr int P8_ROWS = 256, P8_TILE = 128;
 constexpr int P8_SOFTMAX = 4, P8_CONVERT = 20, P8_WARPS = 24;
 constexpr int P8_THREADS = P8_WARPS * 32;
 constexpr int P8_TMEM = 512;              // per tile of rows 256 columns: S of even and odd pages (64 each), O (D)
-constexpr float P8_LAZY = 1.0f, P8_MOST = 256.f;        // a weight beyond 2^8 moves the reference maximum where that is 1 behind
+constexpr float P8_LAZY = 8.0f;           // the reference maximum follows where it is 2^8 behind
 constexpr uint32_t PG_WIDE = 1u, PG_POISON = 2u;       // the page's scales are far apart; it has values that are no numbers
 constexpr float P8_LIGHT = 8.077935669463161e-28f;     // 2^-90
 constexpr float P8_APART = 2.44140625e-4f;             // 2^-12
@@ -459,69 +459,65 @@ __global__ void __launch_bounds__(P8_THREADS, 1) attention_prompt8_kernel(Prompt
         for (int c = 0; c < 32; ++c)
           if (c > b || c < a) sc[c] = -INFINITY;
       }
-      uint32_t packed[16];
-      float sum;
-      __half2 top2;
-      auto weigh = [&]() {
-        float2 sum2[4] = {{0.f, 0.f}, {0.f, 0.f}, {0.f, 0.f}, {0.f, 0.f}};
-        __half2 t2[2] = {__half2half2(__ushort_as_half(0)), __half2half2(__ushort_as_half(0))};
-        const float2 scale2 = make_float2(to_log2, to_log2), off2 = make_float2(off, off);
+      float mx4[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
-        for (int c = 0; c < 32; c += 2) {
-          const float2 x = __ffma2_rn(make_float2(sc[c], sc[c + 1]), scale2, off2);
-          const float2 e = make_float2(fast_exp2(x.x), fast_exp2(x.y));
-          sum2[(c >> 1) & 3] = __fadd2_rn(sum2[(c >> 1) & 3], e);
-          const __half2 h = __floats2half2_rn(e.x, e.y);
-          t2[(c >> 1) & 1] = __hmax2(t2[(c >> 1) & 1], h);
-          packed[c >> 1] = half2_bits(h);
-        }
-        const float2 s = __fadd2_rn(__fadd2_rn(sum2[0], sum2[1]), __fadd2_rn(sum2[2], sum2[3]));
-        sum = s.x + s.y;
-        top2 = __hmax2(t2[0], t2[1]);
-      };
-      weigh();
-      // The common page: no weight has outgrown the reference maximum, and the sum of w is that of P / vmax.  Otherwise both threads of
+      for (int c = 0; c < 32; c += 8)
+#pragma unroll
+        for (int u = 0; u < 4; ++u) mx4[u] = fmaxf(fmaxf(mx4[u], sc[c + 2 * u]), sc[c + 2 * u + 1]);
+      float top = fmaf(fmaxf(fmaxf(mx4[0], mx4[1]), fmaxf(mx4[2], mx4[3])), to_log2, page.y), corr = 1.f;
+      // The common page: nothing has outgrown the reference maximum, and the sum of w is that of P / vmax.  Otherwise both threads of
       // every row of the two warps go the long way.
-      float corr = 1.f;
-      const bool rare = m_ref == -INFINITY || fmaxf(__low2float(top2), __high2float(top2)) > P8_MOST || page.z * P8_LIGHT > l_run + l_other || look != 0u;
-      if (any_of_pair(rare)) {
-        float mx = -INFINITY;
-#pragma unroll
-        for (int c = 0; c < 32; ++c) mx = fmaxf(mx, sc[c]);
-        float top = fmaf(mx, to_log2, page.y);
+      const bool light = look != 0u || page.z * P8_LIGHT > l_run + l_other;
+      bool by_key = false;
+      if (any_of_pair(top > m_ref + P8_LAZY || light)) {
         s_top[tile][half][in_tile] = top;
         s_sum[tile][half][in_tile] = l_run;
         meet();
         top = fmaxf(top, s_top[tile][half ^ 1][in_tile]);
         l_other = s_sum[tile][half ^ 1][in_tile];
         meet();
-        if (top > m_ref + P8_LAZY || m_ref == -INFINITY) {         // (both -inf: nothing seen yet)
+        if (top > m_ref + P8_LAZY) {
           if (m_ref != -INFINITY) {
             corr = fast_exp2(m_ref - top);
             l_run = rescale8(l_run, m_ref - top);
             l_other = rescale8(l_other, m_ref - top);
           }
           m_ref = top;
-          neg_ref = top == -INFINITY ? 0.f : -top;
+          neg_ref = -top;
         }
         off = page.y + neg_ref;
-        weigh();
-        // The sum of w key by key where P may have lost some of it: in a page whose values are far smaller than another page's (zeros, for
-        // instance, say nothing about their weights).
-        if (__any_sync(0xffffffffu, look != 0u || page.z * P8_LIGHT > l_run + l_other)) {
+        by_key = __any_sync(0xffffffffu, look != 0u || page.z * P8_LIGHT > l_run + l_other);
+        if (by_key) {
+          // The sum of w key by key where P may have lost some of it: in a page whose values are far smaller than another page's (zeros,
+          // for instance, say nothing about their weights).
           const bool wide = (look & PG_WIDE) != 0u;
 #pragma unroll
           for (int c = 0; c < 32; ++c) l_run += fast_exp2(fmaf(sc[c], to_log2, off) - (wide ? s_key[st][1][32 * half + c] : page.y));
-        } else {
-          l_run = fmaf(sum, page.z, l_run);
+          const uint32_t bad = s_poison[st][half];
+          if (bad) {                                               // values that are no numbers: for the rows that see them
+            const int a = p.window > 0 ? max(qpos - p.window + 1 - key0, 0) : 0, b = min(qpos - key0, 31);
+            if (a <= b && ((bad >> a) << (31 - (b - a)))) l_run = __int_as_float(0x7fffffff);
+          }
         }
-        const uint32_t bad = s_poison[st][half];
-        if (bad) {                                                 // values that are no numbers: for the rows that see them
-          const int a = p.window > 0 ? max(qpos - p.window + 1 - key0, 0) : 0, b = min(qpos - key0, 31);
-          if (a <= b && ((bad >> a) << (31 - (b - a)))) l_run = __int_as_float(0x7fffffff);
-        }
-      } else {
-        l_run = fmaf(sum, page.z, l_run);
+      }
+      const float2 scale2 = make_float2(to_log2, to_log2), off2 = make_float2(off, off);
+#pragma unroll
+      for (int c = 0; c < 32; c += 2) {
+        const float2 x = __ffma2_rn(make_float2(sc[c], sc[c + 1]), scale2, off2);
+        sc[c] = x.x, sc[c + 1] = x.y;
+      }
+#pragma unroll
+      for (int c = 0; c < 32; ++c) sc[c] = fast_exp2(sc[c]);
+      uint32_t packed[16];
+      float2 sum2[4] = {{0.f, 0.f}, {0.f, 0.f}, {0.f, 0.f}, {0.f, 0.f}};
+#pragma unroll
+      for (int c = 0; c < 32; c += 2) {
+        sum2[(c >> 1) & 3] = __fadd2_rn(sum2[(c >> 1) & 3], make_float2(sc[c], sc[c + 1]));
+        packed[c >> 1] = half2_bits(__floats2half2_rn(sc[c], sc[c + 1]));
+      }
+      if (!by_key) {
+        const float2 s = __fadd2_rn(__fadd2_rn(sum2[0], sum2[1]), __fadd2_rn(sum2[2], sum2[3]));
+        l_run = fmaf(s.x + s.y, page.z, l_run);
       }
       if (j >= 1) {
         // (waited for on every page: a wait on a phase's parity is right only for a thread at most one phase behind)

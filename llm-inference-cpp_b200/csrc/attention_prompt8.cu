@@ -6,7 +6,7 @@
 // A block takes 256 query rows of one sequence and kv head — tokens times the heads of the group, token by token, so that a page
 // serves the whole group — as two tiles of 128 rows, and walks the pages (64 keys) that they see:
 //
-//   scales        one warp makes each row's factor of the page
+//   scales        a warp makes each row's factor of the page (three of them, for a page a stage each)
 //   codes -> fp16 four warps bring a page's codes into a ring with cp.async, each thread what it will read itself, so that nobody waits
 //                 for anybody (a thread that asks for bulk copies is busy half a microsecond with each: four a page were 2,000 clocks,
 //                 most of a page's time), and make K' = code * (k_scale / kmax) and V' = code * (v_scale / vmax) of a page, kmax and vmax its largest
@@ -34,7 +34,7 @@
 namespace llmi {
 
 constexpr int P8_ROWS = 256, P8_TILE = 128;
-// Warps: 0 scales, 1 products, (2, 3 none,) 4 .. 19 softmax (two tiles, two halves of a page's keys, four quarters of the rows),
+// Warps: 0, 2, 3 scales, 1 products, 4 .. 19 softmax (two tiles, two halves of a page's keys, four quarters of the rows),
 // 20 .. 23 codes to fp16.
 constexpr int P8_SOFTMAX = 4, P8_CONVERT = 20, P8_WARPS = 24;
 constexpr int P8_THREADS = P8_WARPS * 32;
@@ -186,7 +186,7 @@ __global__ void __launch_bounds__(P8_THREADS, 1) attention_prompt8_kernel(Prompt
   auto p_ready = [&](int tile, int b) { return bars + 8u * (5 + 3 * STAGES + 2 * tile + b); };
   auto o_done = [&](int tile) { return bars + 8u * (9 + 3 * STAGES + tile); };
   static_assert(8 * (11 + 3 * STAGES) <= 168, "barriers fit");
-  __shared__ float s_scales[RAWS][2 * PAGE8];            // pages under way: scales of keys, of values
+  __shared__ float s_scales[STAGES][2][2 * PAGE8];       // pages under way: scales of keys, of values
   __shared__ uint2 s_fac[STAGES][PAGE8];                 // a row's factors, each the sum of two fp16 numbers: of its keys, of its values
   __shared__ uint32_t s_none[STAGES][4];                 // rows whose key codes, and whose value codes, may be no numbers
   __shared__ float4 s_page[STAGES];                      // kmax, log2 vmax, 1 / vmax, whether the page needs a look (PG_*, as bits)
@@ -244,29 +244,26 @@ __global__ void __launch_bounds__(P8_THREADS, 1) attention_prompt8_kernel(Prompt
     const int at = pg0 + j, page = j < n_pg && at < p.kv.table_pages ? table[at] : -1;
     return (unsigned)page < (unsigned)p.kv.n_pages ? page : -1;
   };
-  if (warp == 0) {
-    // ---- scales: what the softmax needs of a page, and its rows' factors ----
-    int under_way[RAWS], next = page_at(0);
+  const int scale_stage = warp == 0 ? 0 : warp - 1;      // (of the warps 0, 2 and 3)
+  if (warp < P8_SOFTMAX && warp != 1) {
+    // ---- scales: what the softmax needs of a page, and its rows' factors; a warp for each of the three stages ----
+    static_assert(STAGES == 3, "warps 0, 2 and 3");
+    const int st = scale_stage;
     auto ask = [&](int j) {                                        // lanes 0 .. 15: the keys' scales, the others: the values'
-      const int page = next;
-      next = page_at(j + 1);
+      const int page = page_at(j);
       const size_t row = ((size_t)max(page, 0) * Hkv + kvh) * PAGE8 + (lane & 15) * 4;
-      cp_async16(&s_scales[j % RAWS][lane * 4], (lane < 16 ? p.k_scales : p.v_scales) + row, 16);
+      cp_async16(&s_scales[st][(j / STAGES) & 1][lane * 4], (lane < 16 ? p.k_scales : p.v_scales) + row, 16);
       cp_async_commit();
       return page;
     };
-#pragma unroll
-    for (int i = 0; i < RAWS - 1; ++i) under_way[i] = ask(i);
-    int st = 0;
+    int page = ask(st);
     uint32_t phase = 1u;
-    for (int j = 0; j < n_pg; ++j) {
-      under_way[RAWS - 1] = ask(j + RAWS - 1);
-      cp_async_wait<RAWS - 1>();
+    for (int j = st; j < n_pg; j += STAGES, phase ^= 1u) {
+      const bool known = page >= 0;
+      page = ask(j + STAGES);
+      cp_async_wait<1>();
       __syncwarp();
-      const float* ks = s_scales[j % RAWS];
-      const bool known = under_way[0] >= 0;
-#pragma unroll
-      for (int i = 0; i < RAWS - 1; ++i) under_way[i] = under_way[i + 1];
+      const float* ks = s_scales[st][(j / STAGES) & 1];
       const int a = max(d.lo - (pg0 + j) * PAGE8, 0), b = min(d.last - (pg0 + j) * PAGE8, 63);      // rows that some query sees
       // the page's largest scales (of rows that are numbers), the least but zeros, and its rows that are no numbers
       float x[2], y[2], km = 0.f, vm = 0.f, kn = INFINITY, vn = INFINITY;
@@ -314,7 +311,6 @@ __global__ void __launch_bounds__(P8_THREADS, 1) attention_prompt8_kernel(Prompt
       }
       __syncwarp();
       if (lane == 0) mbar_arrive(fac_full(st));
-      if (++st == STAGES) st = 0, phase ^= 1u;
     }
     cp_async_wait_all();
   } else if (warp == 1) {

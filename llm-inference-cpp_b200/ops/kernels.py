@@ -2124,8 +2124,12 @@ def softcap_rows(v: torch.Tensor, cap: float) -> None:
 
 
 # -- keys and values held in 8 bits ---------------------------------------------------------------------------------------------
+#
+# These launchers run between two kernels of a few microseconds each, so what they check and collect is asked of every tensor once.
 
 _HELD_CODE = {torch.int8: 0, torch.float8_e4m3fn: 1}
+_DTYPE8 = {torch.float32: 0, torch.bfloat16: 1}
+_current_device = torch._C._cuda_getDevice if hasattr(torch._C, "_cuda_getDevice") else torch.cuda.current_device
 
 
 def _refuse(name: str, wrong: bool, why: str) -> None:
@@ -2133,29 +2137,46 @@ def _refuse(name: str, wrong: bool, why: str) -> None:
         raise KernelError(f"{name}: {why}")
 
 
-def _check8(name: str, x: torch.Tensor, k: Rows8, v: Rows8, seq_pages, n_heads: int, n_kv_heads: int, head_dim: int, more=()) -> int:
+def _check8(name: str, x: torch.Tensor, k: Rows8, v: Rows8, seq_pages, n_heads: int, n_kv_heads: int, head_dim: int) -> int:
     """The checks that the 8-bit kernels share; the code of the type that the rows are held in."""
-    if not (x.is_cuda and all(t.is_cuda for t in (*k, *v, seq_pages, *more))):
-        raise KernelError(f"{name}: kernels take CUDA tensors only (there is no CPU path)")
+    kc, ks = k
+    vc, vs = v
     device = x.get_device()
-    _refuse(name, device != torch.cuda.current_device() or any(t.get_device() != device for t in (*k, *v, seq_pages, *more)),
-            "all tensors must lie on the current device")
-    _refuse(name, x.dtype not in (torch.bfloat16, torch.float32), f"unsupported element type {x.dtype}")
-    _refuse(name, k.codes.dtype not in _HELD_CODE or v.codes.dtype != k.codes.dtype, "keys and values are held in int8 or float8_e4m3fn, both in one of them")
-    _refuse(name, n_heads < 1 or n_kv_heads < 1 or n_heads % n_kv_heads != 0, "n_heads must be a multiple of n_kv_heads")
-    _refuse(name, not 1 <= head_dim <= 256, "head_dim must be 1 to 256")
-    shape = k.codes.shape
-    _refuse(name, tuple(shape[1:]) != (n_kv_heads, 64, head_dim) or shape[0] < 1 or v.codes.shape != shape, "codes must be [pages, n_kv_heads, 64, head_dim]")
-    for s in (k.scales, v.scales):
-        _refuse(name, s.dtype != torch.float32 or s.shape != shape[:-1], "scales must be fp32 [pages, n_kv_heads, 64]")
-    _refuse(name, not all(t.is_contiguous() for t in (*k, *v)), "codes and scales must be contiguous")
-    _refuse(name, seq_pages.dtype != torch.int32 or seq_pages.dim() != 2 or (seq_pages.shape[1] > 1 and seq_pages.stride(1) != 1),
-            "the page table must be int32 [sequences, pages]")
-    return _HELD_CODE[k.codes.dtype]
+    if not device == kc.get_device() == ks.get_device() == vc.get_device() == vs.get_device() == seq_pages.get_device():
+        raise KernelError(f"{name}: all tensors must lie on the current CUDA device (there is no CPU path)")
+    if device < 0 or device != _current_device():
+        raise KernelError(f"{name}: kernels take CUDA tensors of the current device only (there is no CPU path)")
+    if x.dtype not in _DTYPE8:
+        raise KernelError(f"{name}: unsupported element type {x.dtype}")
+    held = _HELD_CODE.get(kc.dtype)
+    if held is None or vc.dtype != kc.dtype:
+        raise KernelError(f"{name}: keys and values are held in int8 or float8_e4m3fn, both in one of them")
+    if n_heads < 1 or n_kv_heads < 1 or n_heads % n_kv_heads != 0:
+        raise KernelError(f"{name}: n_heads must be a multiple of n_kv_heads")
+    if not 1 <= head_dim <= 256:
+        raise KernelError(f"{name}: head_dim must be 1 to 256")
+    shape = kc.shape
+    if vc.shape != shape or len(shape) != 4 or shape[0] < 1 or shape[1] != n_kv_heads or shape[2] != 64 or shape[3] != head_dim:
+        raise KernelError(f"{name}: codes must be [pages, n_kv_heads, 64, head_dim]")
+    if ks.dtype != torch.float32 or vs.dtype != torch.float32 or ks.shape != shape[:3] or vs.shape != shape[:3]:
+        raise KernelError(f"{name}: scales must be fp32 [pages, n_kv_heads, 64]")
+    if not (kc.is_contiguous() and ks.is_contiguous() and vc.is_contiguous() and vs.is_contiguous()):
+        raise KernelError(f"{name}: codes and scales must be contiguous")
+    if seq_pages.dtype != torch.int32 or seq_pages.dim() != 2 or (seq_pages.shape[1] > 1 and seq_pages.stride(1) != 1):
+        raise KernelError(f"{name}: the page table must be int32 [sequences, pages]")
+    return held
 
 
-def _check_index(name: str, what: str, t: torch.Tensor, n: int) -> None:
-    _refuse(name, t.dtype != torch.int32 or t.dim() != 1 or t.shape[0] < n or (n > 1 and t.stride(0) != 1), f"{what} must be int32 [{n}]")
+def _index8(name: str, what: str, t: torch.Tensor, n: int, device: int) -> int:
+    """The address of an int32 array of at least ``n`` entries on the device, checked."""
+    if t.dtype != torch.int32 or t.dim() != 1 or t.shape[0] < n or (n > 1 and t.stride(0) != 1) or t.get_device() != device:
+        raise KernelError(f"{name}: {what} must be int32 [{n}] on the same CUDA device")
+    return t.data_ptr()
+
+
+def _stream8(device: int) -> int:
+    """The current stream of the tensors' device."""
+    return torch.cuda.current_stream(device).cuda_stream if _raw_stream is None else _raw_stream(device)
 
 
 def rope_store8(qkv: torch.Tensor, q_out: torch.Tensor, inv_freq: torch.Tensor | None, rotary_dim: int, tok_seq, tok_pos, seq_pages,
@@ -2165,43 +2186,31 @@ def rope_store8(qkv: torch.Tensor, q_out: torch.Tensor, inv_freq: torch.Tensor |
     The rotated q goes to ``q_out`` [T, n_heads * head_dim] (rows may be strided; ``qkv[:, :n_heads * head_dim]`` rotates in
     place).  ``tok_seq`` -1 marks a token of no sequence: nothing of it is written.  Two tokens of a call must not have the same
     place.  ``write_kv`` False: q only.  How a row is held: ``csrc/rows8.cuh``."""
+    held = _check8("rope_store8", qkv, k, v, seq_pages, n_heads, n_kv_heads, head_dim)
+    _rope_store8(held, qkv, q_out, inv_freq, rotary_dim, tok_seq, tok_pos, seq_pages, k, v, n_heads, n_kv_heads, head_dim, write_kv)
+
+
+def _rope_store8(held: int, qkv, q_out, inv_freq, rotary_dim, tok_seq, tok_pos, seq_pages, k, v, n_heads, n_kv_heads, head_dim, write_kv) -> None:
     name = "rope_store8"
-    held = _check8(name, qkv, k, v, seq_pages, n_heads, n_kv_heads, head_dim, (q_out, tok_seq, tok_pos))
-    T = qkv.shape[0]
-    _refuse(name, qkv.dim() != 2 or qkv.shape[1] != (n_heads + 2 * n_kv_heads) * head_dim or qkv.stride(1) != 1, "qkv must be [tokens, (n_heads + 2 n_kv_heads) * head_dim]")
-    _refuse(name, q_out.shape != (T, n_heads * head_dim) or q_out.dtype != qkv.dtype or q_out.stride(1) != 1, "q_out must be [tokens, n_heads * head_dim] of qkv's type")
-    _refuse(name, rotary_dim < 0 or rotary_dim % 2 != 0 or rotary_dim > head_dim, "rotary_dim must be even and at most head_dim")
-    if rotary_dim:
-        _refuse(name, inv_freq is None or not inv_freq.is_cuda or inv_freq.get_device() != qkv.get_device() or inv_freq.dtype != torch.float32
-                or inv_freq.numel() < rotary_dim // 2 or not inv_freq.is_contiguous(), "inv_freq must be fp32 with rotary_dim / 2 entries on the same device")
-    _check_index(name, "tok_seq", tok_seq, T)
-    _check_index(name, "tok_pos", tok_pos, T)
-    if T == 0 or seq_pages.numel() == 0:
+    device, T = qkv.get_device(), qkv.shape[0]
+    if qkv.dim() != 2 or qkv.shape[1] != (n_heads + 2 * n_kv_heads) * head_dim or (qkv.stride(1) != 1 and qkv.shape[1] > 1):
+        raise KernelError(f"{name}: qkv must be [tokens, (n_heads + 2 n_kv_heads) * head_dim]")
+    if q_out.dim() != 2 or q_out.shape[0] != T or q_out.shape[1] != n_heads * head_dim or q_out.dtype != qkv.dtype or q_out.get_device() != device \
+            or (q_out.stride(1) != 1 and q_out.shape[1] > 1):
+        raise KernelError(f"{name}: q_out must be [tokens, n_heads * head_dim] of qkv's type")
+    if rotary_dim < 0 or rotary_dim % 2 != 0 or rotary_dim > head_dim:
+        raise KernelError(f"{name}: rotary_dim must be even and at most head_dim")
+    if rotary_dim and (inv_freq is None or inv_freq.get_device() != device or inv_freq.dtype != torch.float32 or inv_freq.numel() < rotary_dim // 2
+                       or not inv_freq.is_contiguous()):
+        raise KernelError(f"{name}: inv_freq must be fp32 with rotary_dim / 2 entries on the same device")
+    seq, pos = _index8(name, "tok_seq", tok_seq, T, device), _index8(name, "tok_pos", tok_pos, T, device)
+    S, P = seq_pages.shape
+    if T == 0 or S == 0 or P == 0:
         return
     _check(name, lib().llmi_rope_store8(
-        _dtype_code(qkv), held, qkv.data_ptr(), qkv.stride(0), q_out.data_ptr(), q_out.stride(0), _addr(inv_freq) if rotary_dim else None, rotary_dim,
-        tok_seq.data_ptr(), tok_pos.data_ptr(), seq_pages.data_ptr(), seq_pages.stride(0), seq_pages.shape[1], seq_pages.shape[0],
-        k.codes.data_ptr(), k.scales.data_ptr(), v.codes.data_ptr(), v.scales.data_ptr(), k.codes.shape[0], T, n_heads, n_kv_heads, head_dim,
-        1 if write_kv else 0, _stream8(qkv)))
-
-
-def _stream8(t: torch.Tensor) -> int:
-    """The current stream of the tensor's device."""
-    return torch.cuda.current_stream(t.device).cuda_stream if _raw_stream is None else _raw_stream(t.get_device())
-
-
-def attention_any8(q: torch.Tensor, out: torch.Tensor, k: Rows8, v: Rows8, tok_seq, tok_pos, seq_pages, n_heads: int, n_kv_heads: int,
-                   head_dim: int, scale: float, window: int = 0) -> None:
-    """:func:`attention8` by the kernel that takes any sizes."""
-    name = "attention_any8"
-    held = _check8(name, q, k, v, seq_pages, n_heads, n_kv_heads, head_dim, (out, tok_seq, tok_pos))
-    T = out.shape[0]
-    _check_index(name, "tok_seq", tok_seq, T)
-    _check_index(name, "tok_pos", tok_pos, T)
-    _check(name, lib().llmi_attention_any8(
-        _dtype_code(q), held, q.data_ptr(), q.stride(0), out.data_ptr(), out.stride(0), k.codes.data_ptr(), k.scales.data_ptr(), v.codes.data_ptr(),
-        v.scales.data_ptr(), tok_seq.data_ptr(), tok_pos.data_ptr(), seq_pages.data_ptr(), seq_pages.stride(0), seq_pages.shape[1],
-        seq_pages.shape[0], k.codes.shape[0], T, n_heads, n_kv_heads, head_dim, scale, window, _stream8(q)))
+        _DTYPE8[qkv.dtype], held, qkv.data_ptr(), qkv.stride(0), q_out.data_ptr(), q_out.stride(0), inv_freq.data_ptr() if rotary_dim else None, rotary_dim,
+        seq, pos, seq_pages.data_ptr(), seq_pages.stride(0), P, S, k.codes.data_ptr(), k.scales.data_ptr(), v.codes.data_ptr(), v.scales.data_ptr(),
+        k.codes.shape[0], T, n_heads, n_kv_heads, head_dim, 1 if write_kv else 0, _stream8(device)))
 
 
 _sizes8: dict = {}
@@ -2211,57 +2220,34 @@ _kept8: dict = {}
 def _rows8_sizes(dtype: int, n_seqs: int, max_q: int, n_heads: int, n_kv_heads: int, head_dim: int, table_pages: int) -> tuple | None:
     """(floats of scratch, tickets) that attention_rows8 needs, None where it does not take the sizes."""
     key = (dtype, n_seqs, max_q, n_heads, n_kv_heads, head_dim, table_pages)
-    if key not in _sizes8:
+    sizes = _sizes8.get(key, False)
+    if sizes is False:
         floats, ints = c_long(0), c_long(0)
         rc = lib().llmi_attention_rows8_workspace(*map(c_int, key), ctypes.byref(floats), ctypes.byref(ints))
         if len(_sizes8) >= 4096:
             _sizes8.clear()
-        _sizes8[key] = (floats.value, ints.value) if rc == 0 else None
-    return _sizes8[key]
+        sizes = _sizes8[key] = (floats.value, ints.value) if rc == 0 else None
+    return sizes
 
 
-def _workspace8(q: torch.Tensor, rt, n_floats: int, n_ints: int) -> tuple:
+def _workspace8(device: int, stream: int, rt, n_floats: int, n_ints: int) -> tuple:
     """Scratch and zeroed tickets: the model's (``rt``), else kept per device and stream; a call that is captured has its own, since a
     graph may be replayed beside anything."""
     if rt is not None:
         return rt.scratch("attn8_slots", (max(n_floats, 1),), torch.float32), rt.zeroed("attn8_tickets", max(n_ints, 1))
     capturing = torch.cuda.is_current_stream_capturing()
-    key = (q.get_device(), _stream8(q))
+    key = (device, stream)
     kept = None if capturing else _kept8.get(key)
     if kept is None or kept[0].numel() < n_floats or kept[1].numel() < n_ints:
-        kept = (torch.empty(max(n_floats, 1), dtype=torch.float32, device=q.device), torch.zeros(max(n_ints, 1), dtype=torch.int32, device=q.device))
+        kept = (torch.empty(max(n_floats, 1), dtype=torch.float32, device=torch.device("cuda", device)),
+                torch.zeros(max(n_ints, 1), dtype=torch.int32, device=torch.device("cuda", device)))
         if not capturing:
             _kept8[key] = kept
     return kept
 
 
-def _aligned8(q, out, k: Rows8, v: Rows8) -> bool:
-    return ((q.data_ptr() | out.data_ptr() | k.codes.data_ptr() | v.codes.data_ptr() | k.scales.data_ptr() | v.scales.data_ptr()) % 16 == 0
-            and q.stride(0) * q.element_size() % 16 == 0 and out.stride(0) * out.element_size() % 16 == 0)
-
-
-def attention_rows8(q: torch.Tensor, out: torch.Tensor, k: Rows8, v: Rows8, seq_q_start, seq_kv_len, max_q: int, seq_pages, n_heads: int,
-                    n_kv_heads: int, head_dim: int, scale: float, window: int = 0, rt=None) -> None:
-    """:func:`attention8` by the kernel for few query rows a sequence (head size 64 or 128): ``seq_q_start`` [sequences + 1],
-    ``seq_kv_len`` [sequences], ``max_q`` the most tokens that a sequence brings."""
-    name = "attention_rows8"
-    held = _check8(name, q, k, v, seq_pages, n_heads, n_kv_heads, head_dim, (out, seq_q_start, seq_kv_len))
-    S, P = seq_pages.shape
-    _refuse(name, out.dtype != q.dtype, "out must have q's type")
-    _check_index(name, "seq_q_start", seq_q_start, S + 1)
-    _check_index(name, "seq_kv_len", seq_kv_len, S)
-    dtype = _dtype_code(q)
-    sizes = _rows8_sizes(dtype, S, max_q, n_heads, n_kv_heads, head_dim, P)
-    _refuse(name, sizes is None, "a size is out of the range this kernel takes")
-    slots, tickets = _workspace8(q, rt, *sizes)
-    _check(name, lib().llmi_attention_rows8(
-        dtype, held, q.data_ptr(), q.stride(0), out.data_ptr(), out.stride(0), k.codes.data_ptr(), k.scales.data_ptr(), v.codes.data_ptr(),
-        v.scales.data_ptr(), seq_q_start.data_ptr(), seq_kv_len.data_ptr(), seq_pages.data_ptr(), seq_pages.stride(0), P, S, k.codes.shape[0],
-        max_q, n_heads, n_kv_heads, head_dim, scale, window, slots.data_ptr(), slots.numel(), tickets.data_ptr(), tickets.numel(), _stream8(q)))
-
-
-_ROWS8_MOST = int(os.environ.get("ROWS8_MOST", "32"))
 _PROMPT8_PART_PAGES = 8       # the least pages of a part of a block of 256 query rows
+_ROWS8_MOST = 32              # query rows of a kv head that the kernel for few rows has in one tile
 
 
 def prompt8_parts(n_blocks: int, n_kv_heads: int, table_pages: int, max_q: int) -> int:
@@ -2274,70 +2260,76 @@ def prompt8_parts(n_blocks: int, n_kv_heads: int, table_pages: int, max_q: int) 
     return max(1, min(16, table_pages // _PROMPT8_PART_PAGES, -(-4 * sms // jobs)))
 
 
-def attention_prompt8(q: torch.Tensor, out: torch.Tensor, k: Rows8, v: Rows8, seq_q_start, seq_kv_len, n_blocks: int, max_q: int, seq_pages, n_heads: int,
-                      n_kv_heads: int, head_dim: int, scale: float, window: int = 0, rt=None) -> None:
-    """:func:`attention8` on the tcgen05 tensor cores (bf16, head size 64 or 128): arguments as :func:`attention_rows8`; ``n_blocks``:
-    at least the blocks of 256 rows (tokens times heads of a kv head) over all sequences."""
-    name = "attention_prompt8"
-    held = _check8(name, q, k, v, seq_pages, n_heads, n_kv_heads, head_dim, (out, seq_q_start, seq_kv_len))
-    S, P = seq_pages.shape
-    _refuse(name, q.dtype != torch.bfloat16 or out.dtype != torch.bfloat16, "takes bf16 only")
-    _check_index(name, "seq_q_start", seq_q_start, S + 1)
-    _check_index(name, "seq_kv_len", seq_kv_len, S)
-    parts = prompt8_parts(n_blocks, n_kv_heads, P, max_q)
-    partials = None
-    if parts > 1:
-        n = n_blocks * n_kv_heads * parts * 256 * (head_dim + 2)
-        partials = rt.scratch("attn8_parts", (n,), torch.float32) if rt is not None else torch.empty(n, dtype=torch.float32, device=q.device)
-    _check(name, lib().llmi_attention_prompt8(
-        held, q.data_ptr(), q.stride(0), out.data_ptr(), out.stride(0), k.codes.data_ptr(), k.scales.data_ptr(), v.codes.data_ptr(),
-        v.scales.data_ptr(), seq_q_start.data_ptr(), seq_kv_len.data_ptr(), seq_pages.data_ptr(), seq_pages.stride(0), P, S, k.codes.shape[0],
-        n_blocks, n_heads, n_kv_heads, head_dim, scale, window, parts, _PROMPT8_PART_PAGES, _addr(partials), partials.numel() if parts > 1 else 0,
-        tc_scratch(q.device).error.data_ptr(), _stream8(q)))
-
-
-def _most_new(ctx) -> int:
-    """A bound on the tokens that a sequence of the step brings, the same for every step that a recorded one is replayed for: a
-    prompt step may be padded to a shape, whose recording is told apart by ``short_message`` (the bound itself, or 0)."""
-    if ctx.decode:
-        return 1
-    return decide(ctx, _message_bound) or ctx.n_tokens
-
-
-def _message_bound(ctx) -> int:
-    return int(getattr(ctx, "short_message", 0))
-
-
 def attention8(q: torch.Tensor, out: torch.Tensor, k: Rows8, v: Rows8, ctx, seq_pages, n_heads: int, n_kv_heads: int, head_dim: int,
-               scale: float, window: int = 0, rt=None, rope=None) -> None:
+               scale: float, window: int = 0, rt=None, rope=None, kernel: str | None = None) -> None:
     """Causal attention of a step's tokens over a cache that holds keys and values in 8 bits: :func:`attention`'s counterpart.
 
     ``q`` [T, >= n_heads * head_dim], rotated; its first n_heads * head_dim columns count.  With ``rope=(inv_freq, rotary_dim,
     write_kv)`` it holds the rows [q | k | v] before their rotation instead: q and k are rotated and k, v appended first
     (:func:`rope_store8`); the rows themselves stay as they are.  ``out`` [T, n_heads * head_dim] of q's type; rows of no
     sequence are left as they are.  ``ctx`` says which tokens those are (the fields of a ``StepContext``: ``tok_seq``,
-    ``tok_pos``, ``seq_q_start``, ``seq_kv_len``, ``max_q_len``).  ``rt``: scratch is taken from it where it is given."""
+    ``tok_pos``, ``seq_q_start``, ``seq_kv_len``, ``n_tokens``, ``decode``, ``short_message``).  ``rt``: scratch is taken from it
+    where it is given.
+
+    Three kernels: "rows" for few query rows a sequence (head size 64 or 128), "prompt" on the tcgen05 tensor cores (bf16, head
+    size 64 or 128) and "any" for every size; ``kernel`` names one (it raises where that one does not take the call)."""
     name = "attention8"
-    _check8(name, q, k, v, seq_pages, n_heads, n_kv_heads, head_dim, (out, ctx.tok_seq, ctx.tok_pos, ctx.seq_q_start, ctx.seq_kv_len))
-    T, width = out.shape[0], n_heads * head_dim
-    _refuse(name, out.dim() != 2 or out.shape[1] != width or out.dtype != q.dtype or out.stride(1) != 1, "out must be [tokens, n_heads * head_dim] of q's type")
-    _refuse(name, q.dim() != 2 or q.shape[0] != T or q.shape[1] < width or q.stride(1) != 1, "q must be [tokens, >= n_heads * head_dim]")
-    _refuse(name, window < 0, "a window has at least one position (0: none)")
-    if T == 0 or seq_pages.numel() == 0:
+    held = _check8(name, q, k, v, seq_pages, n_heads, n_kv_heads, head_dim)
+    device, width = q.get_device(), n_heads * head_dim
+    if out.dim() != 2 or out.shape[1] != width or out.dtype != q.dtype or out.get_device() != device or (out.stride(1) != 1 and width > 1):
+        raise KernelError(f"{name}: out must be [tokens, n_heads * head_dim] of q's type")
+    T = out.shape[0]
+    if q.dim() != 2 or q.shape[0] != T or q.shape[1] < width or (q.stride(1) != 1 and width > 1):
+        raise KernelError(f"{name}: q must be [tokens, >= n_heads * head_dim]")
+    if window < 0:
+        raise KernelError(f"{name}: a window has at least one position (0: none)")
+    S, P = seq_pages.shape
+    start = _index8(name, "seq_q_start", ctx.seq_q_start, S + 1, device)
+    kv_len = _index8(name, "seq_kv_len", ctx.seq_kv_len, S, device)
+    if T == 0 or S == 0 or P == 0:
         return
     if rope is not None:
         inv_freq, rotary_dim, write_kv = rope
         rotated = rt.scratch("attn_q8", (T, width)) if rt is not None else torch.empty((T, width), dtype=q.dtype, device=q.device)
-        rope_store8(q, rotated, inv_freq, rotary_dim, ctx.tok_seq, ctx.tok_pos, seq_pages, k, v, n_heads, n_kv_heads, head_dim, write_kv)
+        _rope_store8(held, q, rotated, inv_freq, rotary_dim, ctx.tok_seq, ctx.tok_pos, seq_pages, k, v, n_heads, n_kv_heads, head_dim, write_kv)
         q = rotated
-    max_q, group = _most_new(ctx), n_heads // n_kv_heads
-    fast = head_dim in (64, 128) and _aligned8(q, out, k, v)
-    if fast and q.dtype == torch.bfloat16 and max_q * group > _ROWS8_MOST:
-        n_blocks = T * group // 256 + seq_pages.shape[0]
-        if n_blocks <= 4095:
-            attention_prompt8(q, out, k, v, ctx.seq_q_start, ctx.seq_kv_len, n_blocks, max_q, seq_pages, n_heads, n_kv_heads, head_dim, scale, window, rt)
-            return
-    if (fast and _rows8_sizes(_dtype_code(q), seq_pages.shape[0], max_q, n_heads, n_kv_heads, head_dim, seq_pages.shape[1]) is not None):
-        attention_rows8(q, out, k, v, ctx.seq_q_start, ctx.seq_kv_len, max_q, seq_pages, n_heads, n_kv_heads, head_dim, scale, window, rt)
+    dtype, ldq, ldo, group = _DTYPE8[q.dtype], q.stride(0), out.stride(0), n_heads // n_kv_heads
+    rows = (held, q.data_ptr(), ldq, out.data_ptr(), ldo, k.codes.data_ptr(), k.scales.data_ptr(), v.codes.data_ptr(), v.scales.data_ptr())
+    table = (seq_pages.data_ptr(), seq_pages.stride(0), P, S, k.codes.shape[0])
+    stream = _stream8(device)
+    # (rows in whole 16-byte pieces: 8 bf16 or 4 fp32 numbers)
+    fast = (head_dim in (64, 128) and (rows[1] | rows[3] | rows[5] | rows[6] | rows[7] | rows[8]) % 16 == 0
+            and (ldq | ldo) % (8 if dtype == 1 else 4) == 0)
+    max_q = 1 if ctx.decode else _most_new(ctx)
+    n_blocks = T * group // 256 + S
+    if kernel in (None, "prompt") and fast and dtype == 1 and n_blocks <= 4095 and (max_q * group > _ROWS8_MOST or kernel):
+        parts = prompt8_parts(n_blocks, n_kv_heads, P, max_q)
+        partials = None
+        if parts > 1:
+            n = n_blocks * n_kv_heads * parts * 256 * (head_dim + 2)
+            partials = rt.scratch("attn8_parts", (n,), torch.float32) if rt is not None else torch.empty(n, dtype=torch.float32, device=q.device)
+        _check("attention_prompt8", lib().llmi_attention_prompt8(
+            *rows, start, kv_len, *table, n_blocks, n_heads, n_kv_heads, head_dim, scale, window, parts, _PROMPT8_PART_PAGES,
+            partials.data_ptr() if parts > 1 else None, partials.numel() if parts > 1 else 0, tc_scratch(q.device).error.data_ptr(), stream))
         return
-    attention_any8(q, out, k, v, ctx.tok_seq, ctx.tok_pos, seq_pages, n_heads, n_kv_heads, head_dim, scale, window)
+    sizes = _rows8_sizes(dtype, S, max_q, n_heads, n_kv_heads, head_dim, P) if kernel in (None, "rows") and fast else None
+    if sizes is not None:
+        slots, tickets = _workspace8(device, stream, rt, *sizes)
+        _check("attention_rows8", lib().llmi_attention_rows8(
+            dtype, *rows, start, kv_len, *table, max_q, n_heads, n_kv_heads, head_dim, scale, window, slots.data_ptr(), slots.numel(),
+            tickets.data_ptr(), tickets.numel(), stream))
+        return
+    if kernel not in (None, "any"):
+        raise KernelError(f"{name}: the kernel {kernel!r} does not take this call")
+    seq, pos = _index8(name, "tok_seq", ctx.tok_seq, T, device), _index8(name, "tok_pos", ctx.tok_pos, T, device)
+    _check("attention_any8", lib().llmi_attention_any8(dtype, *rows, seq, pos, *table, T, n_heads, n_kv_heads, head_dim, scale, window, stream))
+
+
+def _most_new(ctx) -> int:
+    """A bound on the tokens that a sequence of a prompt step brings, the same for every step that a recorded one is replayed for: the
+    step may be padded to a shape, whose recording is told apart by ``short_message`` (the bound itself, or 0)."""
+    return decide(ctx, _message_bound) or ctx.n_tokens
+
+
+def _message_bound(ctx) -> int:
+    return int(getattr(ctx, "short_message", 0))

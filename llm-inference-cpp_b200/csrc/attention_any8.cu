@@ -28,6 +28,7 @@ struct Any8Params {
   int n_tokens, n_seqs, n_heads;
   float scale;
   int window;
+  int q_f32;                  // q is fp32 (where out is bf16)
 };
 
 template <typename T, int HELD, int NJ>
@@ -43,8 +44,8 @@ __global__ void __launch_bounds__(ANY8_WARPS * 32) attention_any8_kernel(Any8Par
   if (seq < 0 || seq >= p.n_seqs || pos < 0) return;          // a row of no sequence
   const int kvh = h / (p.n_heads / p.kv.n_kv_heads);
   const int lo = (p.window > 0 && pos - p.window + 1 > 0) ? pos - p.window + 1 : 0;
-  const T* qp = (const T*)p.q + (size_t)t * p.ldq + (size_t)h * hd;
-  for (int d = lane; d < hd; d += 32) q_s[warp][d] = to_f32(qp[d]);
+  const size_t q_at = (size_t)t * p.ldq + (size_t)h * hd;
+  for (int d = lane; d < hd; d += 32) q_s[warp][d] = p.q_f32 ? ((const float*)p.q)[q_at + d] : to_f32(((const T*)p.q)[q_at + d]);
   __syncwarp();
   float m = -INFINITY, l = 0.f, acc[NJ];
 #pragma unroll
@@ -108,13 +109,13 @@ using namespace llmi;
 LLMI_EXPORT int llmi_attention_any8(int dtype, int held, const void* q, long ldq, void* out, long ldo, const void* k_codes, const float* k_scales,
                                     const void* v_codes, const float* v_scales, const int32_t* tok_seq, const int32_t* tok_pos,
                                     const int32_t* seq_pages, int pages_stride, int table_pages, int n_seqs, int n_pages, int n_tokens,
-                                    int n_heads, int n_kv_heads, int head_dim, float scale, int window, cudaStream_t stream) {
+                                    int n_heads, int n_kv_heads, int head_dim, float scale, int window, int q_f32, cudaStream_t stream) {
   if (n_tokens <= 0 || n_seqs <= 0 || n_heads <= 0 || n_kv_heads <= 0 || n_heads % n_kv_heads || head_dim <= 0 || head_dim > ANY8_MAX_HD ||
       n_pages <= 0 || window < 0)
     return LLMI_ERR_BAD_SIZE;
   if (held != HELD_INT8 && held != HELD_E4M3) return LLMI_ERR_BAD_DTYPE;
   Any8Params p{q, ldq, out, ldo, (const uint8_t*)k_codes, k_scales, (const uint8_t*)v_codes, v_scales, tok_seq, tok_pos,
-               Paged8{seq_pages, pages_stride, table_pages, n_pages, n_kv_heads, head_dim}, n_tokens, n_seqs, n_heads, scale, window};
+               Paged8{seq_pages, pages_stride, table_pages, n_pages, n_kv_heads, head_dim}, n_tokens, n_seqs, n_heads, scale, window, q_f32};
   if (dtype == LLMI_DTYPE_F32)
     return held == HELD_INT8 ? launch_attention_any8<float, HELD_INT8>(p, stream) : launch_attention_any8<float, HELD_E4M3>(p, stream);
   if (dtype == LLMI_DTYPE_BF16)

@@ -46,7 +46,7 @@ constexpr float P8_APART = 2.44140625e-4f;             // 2^-12
 constexpr float P8_TINY = 7.888609052210118e-31f;      // 2^-100: smaller scales of a page count as this
 
 struct Prompt8Params {
-  const __nv_bfloat16* q;
+  const void* q;                // bf16, or fp32 with q_f32
   long ldq;
   __nv_bfloat16* out;
   long ldo;
@@ -60,6 +60,7 @@ struct Prompt8Params {
   int n_seqs, group;
   float scale_log2;
   int window;
+  int q_f32;
   int parts, part_pages;        // most parts of a block's pages; the least pages of a part
   float* partials;              // [block][kv head][part][256][D + 2] when parts > 1
   int* error_flag;
@@ -386,17 +387,29 @@ __global__ void __launch_bounds__(P8_THREADS, 1) attention_prompt8_kernel(Prompt
     // the row's queries, divided by a power of two above the largest
     float row_fac;
     {
-      const uint4* src = reinterpret_cast<const uint4*>(p.q + (size_t)(d.q_start + (row_ok ? tok : 0)) * p.ldq + (size_t)head * D);
+      const size_t src = (size_t)(d.q_start + (row_ok ? tok : 0)) * p.ldq + (size_t)head * D;
+      auto eight = [&](int c, float (&x)[8]) {                     // entries 8 c .. 8 c + 7; zeros for a row that there is none of
+        if (p.q_f32) {
+          const float4* f = reinterpret_cast<const float4*>((const float*)p.q + src + 8 * c);
+          const float4 u = row_ok ? f[0] : make_float4(0.f, 0.f, 0.f, 0.f), v = row_ok ? f[1] : make_float4(0.f, 0.f, 0.f, 0.f);
+          x[0] = u.x, x[1] = u.y, x[2] = u.z, x[3] = u.w, x[4] = v.x, x[5] = v.y, x[6] = v.z, x[7] = v.w;
+        } else {
+          const uint4 raw = row_ok ? *reinterpret_cast<const uint4*>((const __nv_bfloat16*)p.q + src + 8 * c) : make_uint4(0u, 0u, 0u, 0u);
+          const __nv_bfloat162* b = reinterpret_cast<const __nv_bfloat162*>(&raw);
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            const float2 f = __bfloat1622float2(b[i]);
+            x[2 * i] = f.x, x[2 * i + 1] = f.y;
+          }
+        }
+      };
       float a = 0.f;
 #pragma unroll
       for (int c = 0; c < D / 8; ++c) {
-        const uint4 raw = row_ok ? src[c] : make_uint4(0u, 0u, 0u, 0u);
-        const __nv_bfloat162* b = reinterpret_cast<const __nv_bfloat162*>(&raw);
+        float x[8];
+        eight(c, x);
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          const float2 f = __bfloat1622float2(b[i]);
-          a = fmaxf(a, fmaxf(fabsf(f.x), fabsf(f.y)));
-        }
+        for (int i = 0; i < 8; ++i) a = fmaxf(a, fabsf(x[i]));
       }
       int ex = 0;
       if (a > 0.f && a <= FLT_MAX) ex = max(-100, (int)((__float_as_uint(a) >> 23) & 255) - 126);
@@ -408,14 +421,11 @@ __global__ void __launch_bounds__(P8_THREADS, 1) attention_prompt8_kernel(Prompt
 #pragma unroll
       for (int i = 0; i < HD / 8; ++i) {
         const int c = half * (HD / 8) + i;
-        const uint4 raw = row_ok ? src[c] : make_uint4(0u, 0u, 0u, 0u);
-        const __nv_bfloat162* b = reinterpret_cast<const __nv_bfloat162*>(&raw);
+        float x[8];
+        eight(c, x);
         uint32_t h[4];
 #pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          const float2 f = __bfloat1622float2(b[e]);
-          h[e] = half2_bits(__floats2half2_rn(f.x * down * down2, f.y * down * down2));
-        }
+        for (int e = 0; e < 4; ++e) h[e] = half2_bits(__floats2half2_rn(x[2 * e] * down * down2, x[2 * e + 1] * down * down2));
         asm volatile("st.shared.v4.u32 [%0], {%1, %2, %3, %4};"
                      ::"r"(at + (c / 8) * (P8_TILE * 128) + (((c % 8) ^ (lane & 7)) << 4)), "r"(h[0]), "r"(h[1]), "r"(h[2]), "r"(h[3]) : "memory");
       }
@@ -719,7 +729,7 @@ using namespace llmi;
 LLMI_EXPORT int llmi_attention_prompt8(int held, const void* q, long ldq, void* out, long ldo, const void* k_codes, const float* k_scales,
                                        const void* v_codes, const float* v_scales, const int32_t* seq_q_start, const int32_t* seq_kv_len,
                                        const int32_t* seq_pages, int pages_stride, int table_pages, int n_seqs, int n_pages, int n_blocks,
-                                       int n_heads, int n_kv_heads, int head_dim, float scale, int window, int parts, int part_pages,
+                                       int n_heads, int n_kv_heads, int head_dim, float scale, int window, int q_f32, int parts, int part_pages,
                                        float* partials, long n_floats, int* error_flag, cudaStream_t stream) {
   if (n_seqs <= 0 || n_blocks <= 0 || n_kv_heads <= 0 || n_heads <= 0 || n_heads % n_kv_heads || (head_dim != 64 && head_dim != 128) ||
       table_pages <= 0 || n_pages <= 0 || window < 0 || parts <= 0 || part_pages <= 0)
@@ -728,11 +738,11 @@ LLMI_EXPORT int llmi_attention_prompt8(int held, const void* q, long ldq, void* 
   if (parts > 1 && (!partials || n_floats < (long)n_blocks * n_kv_heads * parts * P8_ROWS * (head_dim + 2))) return LLMI_ERR_BAD_SIZE;
   if (held != HELD_INT8 && held != HELD_E4M3) return LLMI_ERR_BAD_DTYPE;
   if ((((uintptr_t)q | (uintptr_t)out | (uintptr_t)k_codes | (uintptr_t)v_codes | (uintptr_t)k_scales | (uintptr_t)v_scales | (uintptr_t)partials) & 15) ||
-      (ldq & 7) || (ldo & 7))
+      (ldq & (q_f32 ? 3 : 7)) || (ldo & 7))
     return LLMI_ERR_ALIGN;
-  Prompt8Params p{(const __nv_bfloat16*)q, ldq, (__nv_bfloat16*)out, ldo, (const uint8_t*)k_codes, k_scales, (const uint8_t*)v_codes, v_scales,
+  Prompt8Params p{q, ldq, (__nv_bfloat16*)out, ldo, (const uint8_t*)k_codes, k_scales, (const uint8_t*)v_codes, v_scales,
                   seq_q_start, seq_kv_len, Paged8{seq_pages, pages_stride, table_pages, n_pages, n_kv_heads, head_dim}, n_seqs, n_heads / n_kv_heads,
-                  scale * 1.4426950408889634f, window, parts, part_pages, partials, error_flag};
+                  scale * 1.4426950408889634f, window, q_f32, parts, part_pages, partials, error_flag};
   if (head_dim == 64) return held == HELD_INT8 ? launch_prompt8<64, HELD_INT8>(p, n_blocks, stream) : launch_prompt8<64, HELD_E4M3>(p, n_blocks, stream);
   return held == HELD_INT8 ? launch_prompt8<128, HELD_INT8>(p, n_blocks, stream) : launch_prompt8<128, HELD_E4M3>(p, n_blocks, stream);
 }

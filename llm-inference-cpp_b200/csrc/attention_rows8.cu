@@ -48,6 +48,7 @@ struct Rows8Params {
   int n_seqs, group, row_tiles;
   float scale_log2;
   int window;
+  int q_f32;                    // q is fp32 (where out is bf16)
   float* slots;                 // [2 * blocks][REGS][32]
   int* tickets;                 // [n_seqs * row_tiles * n_kv_heads], zero before and after
 };
@@ -309,12 +310,12 @@ __global__ void __launch_bounds__(RW8_WARPS * 32, (Rw8Cfg<D, NT, T>::BLOCKS)) at
 #pragma unroll
       for (int c = 0; c < D / 64; ++c) {
         const int row = d.row0 + r;
-        const T* src = (const T*)p.q + (size_t)(d.q_start + row / G) * p.ldq + (size_t)(kvh * G + row % G) * D + 64 * c + 16 * t;
-        if (SP == 1) {
+        const size_t at = (size_t)(d.q_start + row / G) * p.ldq + (size_t)(kvh * G + row % G) * D + 64 * c + 16 * t;
+        if (SP == 1 && !p.q_f32) {
 #pragma unroll
           for (int h = 0; h < 2; ++h) {
             uint4 raw = make_uint4(0u, 0u, 0u, 0u);
-            if (r < d.rows) raw = *reinterpret_cast<const uint4*>(src + 8 * h);
+            if (r < d.rows) raw = *reinterpret_cast<const uint4*>((const __nv_bfloat16*)p.q + at + 8 * h);
             const __nv_bfloat162* b = reinterpret_cast<const __nv_bfloat162*>(&raw);
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
@@ -327,7 +328,7 @@ __global__ void __launch_bounds__(RW8_WARPS * 32, (Rw8Cfg<D, NT, T>::BLOCKS)) at
 #pragma unroll
           for (int h = 0; h < 4; ++h) {
             float4 f = make_float4(0.f, 0.f, 0.f, 0.f);
-            if (r < d.rows) f = *reinterpret_cast<const float4*>(src + 4 * h);
+            if (r < d.rows) f = *reinterpret_cast<const float4*>((const float*)p.q + at + 4 * h);
             x[c * 16 + 4 * h] = f.x, x[c * 16 + 4 * h + 1] = f.y, x[c * 16 + 4 * h + 2] = f.z, x[c * 16 + 4 * h + 3] = f.w;
           }
         }
@@ -737,8 +738,8 @@ LLMI_EXPORT int llmi_attention_rows8_workspace(int dtype, int n_seqs, int max_q,
 LLMI_EXPORT int llmi_attention_rows8(int dtype, int held, const void* q, long ldq, void* out, long ldo, const void* k_codes, const float* k_scales,
                                      const void* v_codes, const float* v_scales, const int32_t* seq_q_start, const int32_t* seq_kv_len,
                                      const int32_t* seq_pages, int pages_stride, int table_pages, int n_seqs, int n_pages, int max_q,
-                                     int n_heads, int n_kv_heads, int head_dim, float scale, int window, float* slots, long n_floats, int* tickets,
-                                     long n_ints, cudaStream_t stream) {
+                                     int n_heads, int n_kv_heads, int head_dim, float scale, int window, int q_f32, float* slots, long n_floats,
+                                     int* tickets, long n_ints, cudaStream_t stream) {
   long floats, ints;
   if (dtype != LLMI_DTYPE_F32 && dtype != LLMI_DTYPE_BF16) return LLMI_ERR_BAD_DTYPE;
   const int rc = llmi_attention_rows8_workspace(dtype, n_seqs, max_q, n_heads, n_kv_heads, head_dim, table_pages, &floats, &ints);
@@ -746,14 +747,14 @@ LLMI_EXPORT int llmi_attention_rows8(int dtype, int held, const void* q, long ld
   if (n_floats < floats || n_ints < ints || n_pages <= 0 || window < 0) return LLMI_ERR_BAD_SIZE;
   if (held != HELD_INT8 && held != HELD_E4M3) return LLMI_ERR_BAD_DTYPE;
   const long even = dtype == LLMI_DTYPE_F32 ? 3 : 7;         // rows are whole 16-byte pieces
-  if ((((uintptr_t)q | (uintptr_t)out | (uintptr_t)k_codes | (uintptr_t)v_codes | (uintptr_t)k_scales | (uintptr_t)v_scales) & 15) || (ldq & even) || (ldo & even))
+  if ((((uintptr_t)q | (uintptr_t)out | (uintptr_t)k_codes | (uintptr_t)v_codes | (uintptr_t)k_scales | (uintptr_t)v_scales) & 15) || (ldq & (q_f32 ? 3 : even)) || (ldo & even))
     return LLMI_ERR_ALIGN;
   const int group = n_heads / n_kv_heads;
   const long rows = (long)max_q * group;
   const int nt = rw8_tiles(dtype, head_dim, rows), tiles = (int)((rows + 8 * nt - 1) / (8 * nt));
   Rows8Params p{q, ldq, out, ldo, (const uint8_t*)k_codes, k_scales, (const uint8_t*)v_codes, v_scales,
                 seq_q_start, seq_kv_len, Paged8{seq_pages, pages_stride, table_pages, n_pages, n_kv_heads, head_dim}, n_seqs, group, tiles,
-                scale * 1.4426950408889634f, window, slots, tickets};
+                scale * 1.4426950408889634f, window, q_f32, slots, tickets};
   const int n_entries = n_seqs * tiles, grid = rw8_grid((long)n_entries * n_kv_heads * table_pages);
 #define LLMI_ROWS8(D_, NT_, T_) \
   (held == HELD_INT8 ? launch_rows8<D_, NT_, HELD_INT8, T_>(p, n_entries, grid, stream) : launch_rows8<D_, NT_, HELD_E4M3, T_>(p, n_entries, grid, stream))

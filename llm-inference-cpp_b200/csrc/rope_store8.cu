@@ -3,7 +3,8 @@
 // src/model/kernels.cpp:122-134, src/model/transformer.cpp:251-262); a rotated key is rounded once, to its codes.
 //
 // qkv is one row per token: [q heads | k heads | v heads], each head head_dim wide.  Rotated q goes to rows of its own (which may be
-// the q part of qkv itself); rows of no sequence (tok_seq -1) are left as they are, in q and in the cache.
+// the q part of qkv itself), of qkv's type or fp32 (attention8 asks for those, so that a query is not rounded to bf16 on its way: that
+// alone doubles the error of its output); rows of no sequence (tok_seq -1) are left as they are, in q and in the cache.
 #include "rows8.cuh"
 
 namespace llmi {
@@ -27,6 +28,7 @@ struct Rope8Params {
   uint8_t* v_codes;
   float* v_scales;
   int n_tokens, n_seqs, n_heads, write_kv;
+  int q_f32;                  // q_out is fp32 (where qkv is bf16)
 };
 
 // Any head size: one warp per (token, head of q, k or v).  The row lies in shared memory as fp32 between its rotation, its maximum
@@ -60,8 +62,11 @@ __global__ void __launch_bounds__(ROPE8_WARPS * 32) rope_store8_kernel(Rope8Para
     __syncwarp();
   }
   if (j < p.n_heads) {
-    T* dst = (T*)p.q_out + (size_t)t * p.ldq + (size_t)j * hd;
-    for (int i = lane; i < hd; i += 32) dst[i] = from_f32<T>(row[i]);
+    const size_t at = (size_t)t * p.ldq + (size_t)j * hd;
+    for (int i = lane; i < hd; i += 32) {
+      if (p.q_f32) ((float*)p.q_out)[at + i] = row[i];
+      else ((T*)p.q_out)[at + i] = from_f32<T>(row[i]);
+    }
     return;
   }
   const int kvh = turned ? j - p.n_heads : j - p.n_heads - p.kv.n_kv_heads;
@@ -154,9 +159,16 @@ __global__ void __launch_bounds__(128) rope_store8_rows_kernel(Rope8Params p, in
       hi[e] = turned ? rot_hi(a[e], b[e], cs[e], sn[e]) : b[e];
     }
     if (mine && j < p.n_heads) {
-      T* dst = (T*)p.q_out + (size_t)t * p.ldq + (size_t)j * hd + i0;
-      Piece8<T>::store(dst, lo);
-      Piece8<T>::store(dst + half, hi);
+      const size_t at = (size_t)t * p.ldq + (size_t)j * hd + i0;
+      if (sizeof(T) == 2 && p.q_f32) {
+        float* dst = (float*)p.q_out + at;
+#pragma unroll
+        for (int e = 0; e < N; e += 4) Piece8<float>::store(dst + e, lo + e), Piece8<float>::store(dst + half + e, hi + e);
+      } else {
+        T* dst = (T*)p.q_out + at;
+        Piece8<T>::store(dst, lo);
+        Piece8<T>::store(dst + half, hi);
+      }
     }
     if (j0 + lanes <= p.n_heads) continue;                                 // queries only, for every thread
     float m = 0.f;
@@ -193,7 +205,7 @@ template <typename T, int HELD>
 int launch_rope_store8(const Rope8Params& p, cudaStream_t stream) {
   const int pieces = p.kv.head_dim / 2 / Piece8<T>::N, heads = p.n_heads + (p.write_kv ? 2 * p.kv.n_kv_heads : 0);
   if ((p.rotary_dim == p.kv.head_dim || p.rotary_dim == 0) && p.kv.head_dim % (2 * Piece8<T>::N) == 0 && pieces <= 32 && (pieces & (pieces - 1)) == 0 &&
-      !(((uintptr_t)p.qkv | (uintptr_t)p.q_out | (uintptr_t)p.k_codes | (uintptr_t)p.v_codes) & 15) && !((p.ld * sizeof(T) | p.ldq * sizeof(T)) & 15)) {
+      !(((uintptr_t)p.qkv | (uintptr_t)p.q_out | (uintptr_t)p.k_codes | (uintptr_t)p.v_codes) & 15) && !((p.ld * sizeof(T) | p.ldq * (p.q_f32 ? 4 : sizeof(T))) & 15)) {
     int log_pieces = 0;
     while ((1 << log_pieces) < pieces) ++log_pieces;
     const int lanes = p.n_tokens >= ROPE8_MANY && heads > ROPE8_LANES ? ROPE8_LANES : heads;
@@ -214,14 +226,14 @@ using namespace llmi;
 LLMI_EXPORT int llmi_rope_store8(int dtype, int held, const void* qkv, long ld, void* q_out, long ldq, const float* inv_freq, int rotary_dim,
                                  const int32_t* tok_seq, const int32_t* tok_pos, const int32_t* seq_pages, int pages_stride, int table_pages,
                                  int n_seqs, void* k_codes, float* k_scales, void* v_codes, float* v_scales, int n_pages, int n_tokens,
-                                 int n_heads, int n_kv_heads, int head_dim, int write_kv, cudaStream_t stream) {
+                                 int n_heads, int n_kv_heads, int head_dim, int write_kv, int q_f32, cudaStream_t stream) {
   if (n_tokens <= 0 || n_seqs <= 0 || n_heads <= 0 || n_kv_heads <= 0 || head_dim <= 0 || head_dim > ROPE8_MAX_HD || n_pages <= 0)
     return LLMI_ERR_BAD_SIZE;
   if (rotary_dim < 0 || rotary_dim > head_dim || (rotary_dim & 1)) return LLMI_ERR_BAD_SIZE;
   if (held != HELD_INT8 && held != HELD_E4M3) return LLMI_ERR_BAD_DTYPE;
   Rope8Params p{qkv, ld, q_out, ldq, inv_freq, rotary_dim, tok_seq, tok_pos,
                 Paged8{seq_pages, pages_stride, table_pages, n_pages, n_kv_heads, head_dim},
-                (uint8_t*)k_codes, k_scales, (uint8_t*)v_codes, v_scales, n_tokens, n_seqs, n_heads, write_kv};
+                (uint8_t*)k_codes, k_scales, (uint8_t*)v_codes, v_scales, n_tokens, n_seqs, n_heads, write_kv, q_f32};
   if (dtype == LLMI_DTYPE_F32)
     return held == HELD_INT8 ? launch_rope_store8<float, HELD_INT8>(p, stream) : launch_rope_store8<float, HELD_E4M3>(p, stream);
   if (dtype == LLMI_DTYPE_BF16)

@@ -185,10 +185,10 @@ def lib():
         l.llmi_rmsnorm.argtypes = [I, P, P, P, P, I, I, F, P]
         l.llmi_rope_store.argtypes = [I, P, L, P, I, P, P, P, I, I, P, P, I, I, I, I, I, P]
         l.llmi_attention_prefill_tc.argtypes = [P, L, L, P, L, P, P, L, P, I, P, P, I, I, I, I, I, F, I, I, I, P, L, P, I, P, I, P, P, L, P, I, P, L, P, P, P, I, I, I, P, P]
-        l.llmi_rope_store8.argtypes = [I, I, P, L, P, L, P, I, P, P, P, I, I, I, P, P, P, P, I, I, I, I, I, I, P]
-        l.llmi_attention_any8.argtypes = [I, I, P, L, P, L, P, P, P, P, P, P, P, I, I, I, I, I, I, I, I, F, I, P]
-        l.llmi_attention_rows8.argtypes = [I, I, P, L, P, L, P, P, P, P, P, P, P, I, I, I, I, I, I, I, I, F, I, P, L, P, L, P]
-        l.llmi_attention_prompt8.argtypes = [I, P, L, P, L, P, P, P, P, P, P, P, I, I, I, I, I, I, I, I, F, I, I, I, P, L, P, P]
+        l.llmi_rope_store8.argtypes = [I, I, P, L, P, L, P, I, P, P, P, I, I, I, P, P, P, P, I, I, I, I, I, I, I, P]
+        l.llmi_attention_any8.argtypes = [I, I, P, L, P, L, P, P, P, P, P, P, P, I, I, I, I, I, I, I, I, F, I, I, P]
+        l.llmi_attention_rows8.argtypes = [I, I, P, L, P, L, P, P, P, P, P, P, P, I, I, I, I, I, I, I, I, F, I, I, P, L, P, L, P]
+        l.llmi_attention_prompt8.argtypes = [I, P, L, P, L, P, P, P, P, P, P, P, I, I, I, I, I, I, I, I, F, I, I, I, I, P, L, P, P]
         _configured = True
     return l
 
@@ -2183,8 +2183,8 @@ def rope_store8(qkv: torch.Tensor, q_out: torch.Tensor, inv_freq: torch.Tensor |
                 k: Rows8, v: Rows8, n_heads: int, n_kv_heads: int, head_dim: int, write_kv: bool = True) -> None:
     """Rotate q and k of each token's row [q | k | v] and append k, v to its sequence's pages, held in 8 bits.
 
-    The rotated q goes to ``q_out`` [T, n_heads * head_dim] (rows may be strided; ``qkv[:, :n_heads * head_dim]`` rotates in
-    place).  ``tok_seq`` -1 marks a token of no sequence: nothing of it is written.  Two tokens of a call must not have the same
+    The rotated q goes to ``q_out`` [T, n_heads * head_dim], of qkv's type or fp32 (rows may be strided; ``qkv[:, :n_heads *
+    head_dim]`` rotates in place).  ``tok_seq`` -1 marks a token of no sequence: nothing of it is written.  Two tokens of a call must not have the same
     place.  ``write_kv`` False: q only.  How a row is held: ``csrc/rows8.cuh``."""
     held = _check8("rope_store8", qkv, k, v, seq_pages, n_heads, n_kv_heads, head_dim)
     _rope_store8(held, qkv, q_out, inv_freq, rotary_dim, tok_seq, tok_pos, seq_pages, k, v, n_heads, n_kv_heads, head_dim, write_kv)
@@ -2195,9 +2195,9 @@ def _rope_store8(held: int, qkv, q_out, inv_freq, rotary_dim, tok_seq, tok_pos, 
     device, T = qkv.get_device(), qkv.shape[0]
     if qkv.dim() != 2 or qkv.shape[1] != (n_heads + 2 * n_kv_heads) * head_dim or (qkv.stride(1) != 1 and qkv.shape[1] > 1):
         raise KernelError(f"{name}: qkv must be [tokens, (n_heads + 2 n_kv_heads) * head_dim]")
-    if q_out.dim() != 2 or q_out.shape[0] != T or q_out.shape[1] != n_heads * head_dim or q_out.dtype != qkv.dtype or q_out.get_device() != device \
-            or (q_out.stride(1) != 1 and q_out.shape[1] > 1):
-        raise KernelError(f"{name}: q_out must be [tokens, n_heads * head_dim] of qkv's type")
+    if q_out.dim() != 2 or q_out.shape[0] != T or q_out.shape[1] != n_heads * head_dim or q_out.get_device() != device \
+            or (q_out.dtype != qkv.dtype and q_out.dtype != torch.float32) or (q_out.stride(1) != 1 and q_out.shape[1] > 1):
+        raise KernelError(f"{name}: q_out must be [tokens, n_heads * head_dim] of qkv's type or fp32")
     if rotary_dim < 0 or rotary_dim % 2 != 0 or rotary_dim > head_dim:
         raise KernelError(f"{name}: rotary_dim must be even and at most head_dim")
     if rotary_dim and (inv_freq is None or inv_freq.get_device() != device or inv_freq.dtype != torch.float32 or inv_freq.numel() < rotary_dim // 2
@@ -2210,7 +2210,7 @@ def _rope_store8(held: int, qkv, q_out, inv_freq, rotary_dim, tok_seq, tok_pos, 
     _check(name, lib().llmi_rope_store8(
         _DTYPE8[qkv.dtype], held, qkv.data_ptr(), qkv.stride(0), q_out.data_ptr(), q_out.stride(0), inv_freq.data_ptr() if rotary_dim else None, rotary_dim,
         seq, pos, seq_pages.data_ptr(), seq_pages.stride(0), P, S, k.codes.data_ptr(), k.scales.data_ptr(), v.codes.data_ptr(), v.scales.data_ptr(),
-        k.codes.shape[0], T, n_heads, n_kv_heads, head_dim, 1 if write_kv else 0, _stream8(device)))
+        k.codes.shape[0], T, n_heads, n_kv_heads, head_dim, 1 if write_kv else 0, 1 if q_out.dtype == torch.float32 else 0, _stream8(device)))
 
 
 _sizes8: dict = {}
@@ -2290,16 +2290,17 @@ def attention8(q: torch.Tensor, out: torch.Tensor, k: Rows8, v: Rows8, ctx, seq_
         return
     if rope is not None:
         inv_freq, rotary_dim, write_kv = rope
-        rotated = rt.scratch("attn_q8", (T, width)) if rt is not None else torch.empty((T, width), dtype=q.dtype, device=q.device)
+        rotated = rt.scratch("attn_q8", (T, width), torch.float32) if rt is not None else torch.empty((T, width), dtype=torch.float32, device=q.device)
         _rope_store8(held, q, rotated, inv_freq, rotary_dim, ctx.tok_seq, ctx.tok_pos, seq_pages, k, v, n_heads, n_kv_heads, head_dim, write_kv)
         q = rotated
-    dtype, ldq, ldo, group = _DTYPE8[q.dtype], q.stride(0), out.stride(0), n_heads // n_kv_heads
+    dtype, ldq, ldo, group = _DTYPE8[out.dtype], q.stride(0), out.stride(0), n_heads // n_kv_heads
+    q_f32 = 1 if q.dtype == torch.float32 else 0
     rows = (held, q.data_ptr(), ldq, out.data_ptr(), ldo, k.codes.data_ptr(), k.scales.data_ptr(), v.codes.data_ptr(), v.scales.data_ptr())
     table = (seq_pages.data_ptr(), seq_pages.stride(0), P, S, k.codes.shape[0])
     stream = _stream8(device)
     # (rows in whole 16-byte pieces: 8 bf16 or 4 fp32 numbers)
     fast = (head_dim in (64, 128) and (rows[1] | rows[3] | rows[5] | rows[6] | rows[7] | rows[8]) % 16 == 0
-            and (ldq | ldo) % (8 if dtype == 1 else 4) == 0)
+            and ldq % (4 if q_f32 else 8) == 0 and ldo % (8 if dtype == 1 else 4) == 0)
     max_q = 1 if ctx.decode else _most_new(ctx)
     n_blocks = T * group // 256 + S
     if kernel in (None, "prompt") and fast and dtype == 1 and n_blocks <= 4095 and (max_q * group > _ROWS8_MOST or kernel):
@@ -2309,20 +2310,20 @@ def attention8(q: torch.Tensor, out: torch.Tensor, k: Rows8, v: Rows8, ctx, seq_
             n = n_blocks * n_kv_heads * parts * 256 * (head_dim + 2)
             partials = rt.scratch("attn8_parts", (n,), torch.float32) if rt is not None else torch.empty(n, dtype=torch.float32, device=q.device)
         _check("attention_prompt8", lib().llmi_attention_prompt8(
-            *rows, start, kv_len, *table, n_blocks, n_heads, n_kv_heads, head_dim, scale, window, parts, _PROMPT8_PART_PAGES,
+            *rows, start, kv_len, *table, n_blocks, n_heads, n_kv_heads, head_dim, scale, window, q_f32, parts, _PROMPT8_PART_PAGES,
             partials.data_ptr() if parts > 1 else None, partials.numel() if parts > 1 else 0, tc_scratch(q.device).error.data_ptr(), stream))
         return
     sizes = _rows8_sizes(dtype, S, max_q, n_heads, n_kv_heads, head_dim, P) if kernel in (None, "rows") and fast else None
     if sizes is not None:
         slots, tickets = _workspace8(device, stream, rt, *sizes)
         _check("attention_rows8", lib().llmi_attention_rows8(
-            dtype, *rows, start, kv_len, *table, max_q, n_heads, n_kv_heads, head_dim, scale, window, slots.data_ptr(), slots.numel(),
+            dtype, *rows, start, kv_len, *table, max_q, n_heads, n_kv_heads, head_dim, scale, window, q_f32, slots.data_ptr(), slots.numel(),
             tickets.data_ptr(), tickets.numel(), stream))
         return
     if kernel not in (None, "any"):
         raise KernelError(f"{name}: the kernel {kernel!r} does not take this call")
     seq, pos = _index8(name, "tok_seq", ctx.tok_seq, T, device), _index8(name, "tok_pos", ctx.tok_pos, T, device)
-    _check("attention_any8", lib().llmi_attention_any8(dtype, *rows, seq, pos, *table, T, n_heads, n_kv_heads, head_dim, scale, window, stream))
+    _check("attention_any8", lib().llmi_attention_any8(dtype, *rows, seq, pos, *table, T, n_heads, n_kv_heads, head_dim, scale, window, q_f32, stream))
 
 
 def _most_new(ctx) -> int:

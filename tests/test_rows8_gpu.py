@@ -195,6 +195,9 @@ def test_append_in_place_and_of_queries_only():
     apart = torch.empty(b.T, H * D, device="cuda", dtype=torch.bfloat16)
     K().rope_store8(qkv, apart, inv, D, b.ctx.tok_seq, b.ctx.tok_pos, b.table, b.k, b.v, H, G, D, write_kv=False)
     assert (b.k.codes.view(torch.uint8) == POISON["int8"]).all() and torch.isnan(b.v.scales).all()
+    whole = torch.empty(b.T, H * D, device="cuda")           # fp32: the same queries before they are rounded
+    K().rope_store8(qkv, whole, inv, D, b.ctx.tok_seq, b.ctx.tok_pos, b.table, b.k, b.v, H, G, D, write_kv=False)
+    assert torch.equal(whole.bfloat16(), apart)
     K().rope_store8(qkv, qkv[:, :H * D], inv, D, b.ctx.tok_seq, b.ctx.tok_pos, b.table, b.k, b.v, H, G, D)
     assert torch.equal(qkv[:, :H * D], apart)
 
@@ -349,8 +352,8 @@ def test_append_and_attend_together(dtype, held, H, G, D, step, window):
     ref, sums, most = b.plain(exact_q, D ** -0.5, window)
     got = out.double().cpu().numpy().reshape(b.T, H, D)
     assert (got[b.n_real:] == 7.0).all()
-    # (the rotated q may be rounded to the compute type in between: half a step of bf16 is 2^-8 of the scores)
-    tol = tolerance(ref, sums, most, dtype) + (2 * (2.0 ** -8 if dtype == "bfloat16" else 2.0 ** -20) * sums * most)[..., None]
+    # (the rotation's fp32 arithmetic; the rotated q is not rounded in between)
+    tol = tolerance(ref, sums, most, dtype) + (2 * 2.0 ** -20 * sums * most)[..., None]
     assert (np.abs(got[:b.n_real] - ref) <= tol).all()
 
 
@@ -415,7 +418,7 @@ def test_refusals():
     i = b.ctx.tok_seq
     store = lambda qkv=q, qo=out, inv=None, rot=0, seq=i, H=4: k.rope_store8(qkv, qo, inv, rot, seq, b.ctx.tok_pos, b.table, b.k, b.v, H, 2, 64)  # noqa: E731
     store()
-    for wrong in (dict(rot=64), dict(rot=3), dict(rot=66, inv=torch.zeros(64, device="cuda")), dict(seq=i.long()), dict(qo=out.float()), dict(qkv=q[:, :-1]),
+    for wrong in (dict(rot=64), dict(rot=3), dict(rot=66, inv=torch.zeros(64, device="cuda")), dict(seq=i.long()), dict(qo=out.half()), dict(qkv=q[:, :-1]),
                   dict(rot=64, inv=torch.zeros(16, device="cuda"))):
         with pytest.raises(k.KernelError):
             store(**wrong)

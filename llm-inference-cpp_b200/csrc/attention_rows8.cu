@@ -7,8 +7,10 @@
 //  * All pages that the step's rows see, kv head by kv head and sequence by sequence, are one line of units (a unit: one page of one
 //    kv head), cut into as many equal ranges as there are blocks resident on the device.  A block works through its range whatever
 //    the sequences' lengths are, so no block waits for the longest one, and nothing about the cut depends on what the host knows.
-//    A (sequence, kv head) whose units several ranges share is joined by the block that comes last (a ticket per kv head and
-//    sequence), in the order of the ranges: the same call gives the same bits.
+//    A (sequence, kv head) that several ranges share leaves partial results, which a second kernel adds in the order of the ranges:
+//    the same call gives the same bits.  (Joined by the block that draws the last of a pair's tickets it took 12 to 17 us behind 22 to
+//    28 us of streaming: fences, atomics and cold code, one behind the other.)  Where there are no more of them than resident blocks
+//    and they are of about one length, or short, each has a block of its own instead.
 //  * Within a block each warp takes every eighth chunk (2 KB of key codes, 2 KB of value codes, their scales) into a ring of its own
 //    in shared memory with cp.async, across the borders of sequences; warps meet only where a (sequence, kv head) ends, through the
 //    stages that they have just read.
@@ -49,8 +51,8 @@ struct Rows8Params {
   float scale_log2;
   int window;
   int q_f32;                    // q is fp32 (where out is bf16)
-  float* slots;                 // [2 * blocks][REGS][32]
-  int* tickets;                 // [n_seqs * row_tiles * n_kv_heads], zero before and after
+  float* slots;                 // [2 * blocks][SLOT]: partial results, of a block's first segment and of its last
+  int* whose;                   // [2 * blocks]: 0, or (its (entry, kv head) + 1) * 2 + whether it is the first of the parts
 };
 
 // D: head size; NT: eighths of query rows; T: the type of q and out (float: two fp16 numbers each).
@@ -113,6 +115,68 @@ __device__ __forceinline__ Rw8Entry rw8_entry(const Rows8Params& p, int e, int t
   return d;
 }
 
+// One tile of an output — 16 dims by 8 rows — out of several states (a state without a maximum is zeros, or NaN, as it is), eight at a time.
+struct Rw8Tile {
+  float o[4], m[2], l[2];
+};
+template <typename C, int NT, typename State, typename Load>
+__device__ __forceinline__ Rw8Tile rw8_gather(int pair, int first, int n_states, int step, State state, Load load) {
+  const int lane = threadIdx.x & 31, n = pair % NT, t = lane & 3;
+  Rw8Tile r;
+  r.m[0] = r.m[1] = -INFINITY;
+  r.l[0] = r.l[1] = r.o[0] = r.o[1] = r.o[2] = r.o[3] = 0.f;
+  for (int w0 = first; w0 < n_states; w0 += 8 * step) {
+    Rw8Tile x[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      const float* at = state(min(w0 + i * step, n_states - 1));
+      const float* m = at + C::PAIRS * 128 + n * 8 + 2 * t;
+#pragma unroll
+      for (int j = 0; j < 2; ++j) x[i].m[j] = load(m + j), x[i].l[j] = load(m + 8 * NT + j);
+#pragma unroll
+      for (int j = 0; j < 4; ++j) x[i].o[j] = load(at + (pair * 4 + j) * 32 + lane);
+    }
+    float f[2], top[2] = {r.m[0], r.m[1]};
+#pragma unroll
+    for (int i = 0; i < 8; ++i)
+#pragma unroll
+      for (int j = 0; j < 2; ++j) top[j] = fmaxf(top[j], x[i].m[j]);
+#pragma unroll
+    for (int j = 0; j < 2; ++j) {
+      const float down = r.m[j] == -INFINITY ? 0.f : r.m[j] - top[j];
+      f[j] = fast_exp2(down), r.l[j] = rescale8(r.l[j], down), r.m[j] = top[j];
+    }
+#pragma unroll
+    for (int j = 0; j < 4; ++j) r.o[j] *= f[j & 1];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      if (w0 + i * step >= n_states) break;
+#pragma unroll
+      for (int j = 0; j < 2; ++j) {
+        const float down = x[i].m[j] == -INFINITY ? 0.f : x[i].m[j] - top[j];
+        f[j] = fast_exp2(down), r.l[j] += rescale8(x[i].l[j], down);
+      }
+#pragma unroll
+      for (int j = 0; j < 4; ++j) r.o[j] = fmaf(x[i].o[j], f[j & 1], r.o[j]);
+    }
+  }
+  return r;
+}
+template <int D, int NT, typename T>
+__device__ __forceinline__ void rw8_write(const Rows8Params& p, const Rw8Entry& d, int kvh, int pair, const Rw8Tile& r) {
+  const int lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3, G = p.group;
+#pragma unroll
+  for (int j = 0; j < 2; ++j) {
+    const int r8 = (pair % NT) * 8 + 2 * t + j;
+    if (r8 >= d.rows) continue;
+    const int row = d.row0 + r8;
+    const float inv = r.l[j] == 0.f ? 0.f : 1.f / r.l[j];
+    T* at = (T*)p.out + (size_t)(d.q_start + row / G) * p.ldo + (size_t)(kvh * G + row % G) * D + g * (D / 8) + 2 * (pair / NT);
+    if (sizeof(T) == 4) *reinterpret_cast<float2*>(at) = make_float2(r.o[j] * inv, r.o[j + 2] * inv);
+    else *reinterpret_cast<__nv_bfloat162*>(at) = __floats2bfloat162_rn(r.o[j] * inv, r.o[j + 2] * inv);
+  }
+}
+
 template <int D, int NT, int HELD, typename T>
 __global__ void __launch_bounds__(RW8_WARPS * 32, (Rw8Cfg<D, NT, T>::BLOCKS)) attention_rows8_kernel(Rows8Params p, int n_entries, Rw8Cut cut) {
   using C = Rw8Cfg<D, NT, T>;
@@ -120,14 +184,14 @@ __global__ void __launch_bounds__(RW8_WARPS * 32, (Rw8Cfg<D, NT, T>::BLOCKS)) at
   static_assert(RW8_WARPS % CPP == 0, "a warp keeps its place in a page");
   extern __shared__ __align__(128) uint8_t smem[];
   int* prefix = reinterpret_cast<int*>(smem + C::RING + C::MERGE);      // [n_entries + 1] units ahead of an entry
-  __shared__ int s_scan[RW8_WARPS], s_last;
+  __shared__ int s_scan[RW8_WARPS], s_top[RW8_WARPS];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
   const int G = p.group, Hkv = p.kv.n_kv_heads;
-  pdl_wait();
   pdl_launch_dependents();
+  // (ahead of the wait: the step's index block only, and the page table in it)
 
   // ---- the line of units: units ahead of each entry ----
-  int pairs = 0;                           // (entry, kv head)s that have pages
+  int pairs = 0, longest = 0;              // (entry, kv head)s that have pages; the most pages of one
   {
     int carry = 0;
     for (int e0 = 0; e0 < n_entries; e0 += RW8_WARPS * 32) {
@@ -140,13 +204,15 @@ __global__ void __launch_bounds__(RW8_WARPS * 32, (Rw8Cfg<D, NT, T>::BLOCKS)) at
         const int y = __shfl_up_sync(0xffffffffu, x, o);
         if (lane >= o) x += y;
       }
-      if (lane == 31) s_scan[warp] = x;
+      const int top = __reduce_max_sync(0xffffffffu, pages);
+      if (lane == 31) s_scan[warp] = x, s_top[warp] = top;
       pairs += __syncthreads_count(n > 0) * Hkv;
       int before = carry, all = carry;
 #pragma unroll
       for (int w = 0; w < RW8_WARPS; ++w) {
         if (w < warp) before += s_scan[w];
         all += s_scan[w];
+        longest = max(longest, s_top[w]);
       }
       if (e < n_entries) prefix[e] = before + x - n;
       carry = all;
@@ -156,8 +222,14 @@ __global__ void __launch_bounds__(RW8_WARPS * 32, (Rw8Cfg<D, NT, T>::BLOCKS)) at
     __syncthreads();
   }
   const int total = prefix[n_entries];
-  const int blocks = min((int)gridDim.x, max(total / cut.least, pairs));
-  if (blockIdx.x >= blocks || total == 0) return;
+  // each its own block, or the line in even ranges
+  const bool whole = pairs <= (int)gridDim.x && (longest <= cut.least || (5 * pairs >= 3 * (int)gridDim.x && (long)(longest + cut.front) * pairs <= total + total / 4));
+  const int blocks = whole ? pairs : min((int)gridDim.x, max(total / cut.least, pairs));
+  if (blockIdx.x >= blocks || total == 0) {
+    pdl_wait();
+    if (threadIdx.x < 2) p.whose[2 * blockIdx.x + threadIdx.x] = 0;
+    return;
+  }
   const int per = total / blocks, longer = total - per * blocks;      // even ranges: the first `longer` have per + 1 units
   auto find_entry = [&](int unit) {        // the entry that has the unit (the last one if they are all before it)
     int a = 0, b = n_entries;              // prefix[a] <= unit < prefix[b]
@@ -175,15 +247,28 @@ __global__ void __launch_bounds__(RW8_WARPS * 32, (Rw8Cfg<D, NT, T>::BLOCKS)) at
     const int e = find_entry(u), len = (prefix[e + 1] - prefix[e]) / Hkv, at = (u - prefix[e]) % len;
     return at <= near ? u - at : len - at <= near ? u - at + len : u;
   };
-  auto block_of = [&](int u) {             // whose range holds unit u
-    int c = u < longer * (per + 1) ? u / (per + 1) : (u - longer) / per;
-    while (c + 1 < blocks && range_start(c + 1) <= u) ++c;
-    while (range_start(c) > u) --c;
-    return c;
-  };
-  const int u0 = range_start(blockIdx.x), u1 = range_start(blockIdx.x + 1);
-  if (u0 >= u1) return;
-  const int e_first = find_entry(u0);
+  int u0, u1, e_first;
+  if (whole) {
+    // (its entry: the last one with no more than so many pairs ahead, found as the line's share of pairs: entries without pages take none)
+    int rank = blockIdx.x / Hkv;
+    e_first = -1;
+    for (int e0 = 0; e_first < 0; e0 += 32) {
+      const uint32_t some = __ballot_sync(0xffffffffu, e0 + lane < n_entries && prefix[e0 + lane + 1] > prefix[e0 + lane]);
+      if (rank < __popc(some)) e_first = e0 + __fns(some, 0, rank + 1);
+      else rank -= __popc(some);
+    }
+    const int len = (prefix[e_first + 1] - prefix[e_first]) / Hkv;
+    u0 = prefix[e_first] + (blockIdx.x % Hkv) * len;
+    u1 = u0 + len;
+  } else {
+    u0 = range_start(blockIdx.x), u1 = range_start(blockIdx.x + 1);
+    e_first = find_entry(u0 < total ? u0 : 0);
+  }
+  if (u0 >= u1) {
+    pdl_wait();
+    if (threadIdx.x < 2) p.whose[2 * blockIdx.x + threadIdx.x] = 0;
+    return;
+  }
   // the block's part of the (entry, kv head) that has unit `at`, from there on
   struct Segment {
     Rw8Entry d;
@@ -274,8 +359,10 @@ __global__ void __launch_bounds__(RW8_WARPS * 32, (Rw8Cfg<D, NT, T>::BLOCKS)) at
     issued = issued + 1 == STAGES ? 0 : issued + 1;
   };
   look_up();
+  pdl_wait();
 #pragma unroll
   for (int i = 0; i < STAGES - 1; ++i) issue();
+  int mine[2] = {0, 0};                    // whose partial results the block leaves
 
   // ---- segments: the block's part of one (entry, kv head) after the other ----
   int taken = 0;                           // the stage read next
@@ -569,69 +656,16 @@ __global__ void __launch_bounds__(RW8_WARPS * 32, (Rw8Cfg<D, NT, T>::BLOCKS)) at
       }
     }
     __syncthreads();
-    // other blocks have pages of it too: partial results, a block's of its first segment and of its last apart
+    // other blocks have pages of it too: a partial result, of the block's first segment or of its last
     const bool shared_out = s.n < d.n_pages;
-    int c_first = 0, c_last = 0, first_slot = 0;
-    float* my_slot = nullptr;
+    const int part = u0 < s.begin ? 1 : 0;
+    float* my_slot = p.slots + (size_t)(2 * blockIdx.x + part) * C::SLOT;
     if (shared_out) {
-      c_first = block_of(s.begin + cut.front), c_last = block_of(s.end - 1);
-      first_slot = 2 * c_first + (range_start(c_first) < s.begin ? 1 : 0);
-      my_slot = p.slots + (size_t)((int)blockIdx.x == c_first ? first_slot : 2 * (int)blockIdx.x) * C::SLOT;
+      const int id = ((e * Hkv + kvh + 1) << 1) | (s.first == 0 ? 1 : 0);
+      if (part) mine[1] = id;
+      else mine[0] = id;
     }
-    // one tile of the output out of several states (a state without a maximum is zeros, or NaN, as it is), eight at a time
-    struct Tile {
-      float o[4], m[2], l[2];
-    };
-    auto gather = [&](int pair, int first, int n_states, int step, auto state, auto load) {
-      const int n = pair % NT;
-      Tile r;
-      r.m[0] = r.m[1] = -INFINITY;
-      r.l[0] = r.l[1] = r.o[0] = r.o[1] = r.o[2] = r.o[3] = 0.f;
-      for (int w0 = first; w0 < n_states; w0 += 8 * step) {
-        Tile x[8];
-#pragma unroll
-        for (int i = 0; i < 8; ++i) {
-          const int w = w0 + i * step;
-          const float* at = state(min(w, n_states - 1));
-          const float* m = at + C::PAIRS * 128 + n * 8 + 2 * t;
-#pragma unroll
-          for (int j = 0; j < 2; ++j) x[i].m[j] = load(m + j), x[i].l[j] = load(m + 8 * NT + j);
-#pragma unroll
-          for (int j = 0; j < 4; ++j) x[i].o[j] = load(at + (pair * 4 + j) * 32 + lane);
-        }
-        float f[2], top[2] = {r.m[0], r.m[1]};
-#pragma unroll
-        for (int i = 0; i < 8; ++i)
-#pragma unroll
-          for (int j = 0; j < 2; ++j) top[j] = fmaxf(top[j], x[i].m[j]);
-#pragma unroll
-        for (int j = 0; j < 2; ++j) f[j] = r.m[j] == -INFINITY ? 1.f : fast_exp2(r.m[j] - top[j]), r.l[j] = r.m[j] == -INFINITY ? r.l[j] : rescale8(r.l[j], r.m[j] - top[j]), r.m[j] = top[j];
-#pragma unroll
-        for (int j = 0; j < 4; ++j) r.o[j] *= f[j & 1];
-#pragma unroll
-        for (int i = 0; i < 8; ++i) {
-          if (w0 + i * step >= n_states) break;
-#pragma unroll
-          for (int j = 0; j < 2; ++j) f[j] = x[i].m[j] == -INFINITY ? 1.f : fast_exp2(x[i].m[j] - top[j]), r.l[j] += rescale8(x[i].l[j], x[i].m[j] == -INFINITY ? 0.f : x[i].m[j] - top[j]);
-#pragma unroll
-          for (int j = 0; j < 4; ++j) r.o[j] = fmaf(x[i].o[j], f[j & 1], r.o[j]);
-        }
-      }
-      return r;
-    };
-    auto write_out = [&](int pair, const Tile& r) {
-#pragma unroll
-      for (int j = 0; j < 2; ++j) {
-        const int r8 = (pair % NT) * 8 + 2 * t + j;
-        if (r8 >= d.rows) continue;
-        const int row = d.row0 + r8;
-        const float inv = r.l[j] == 0.f ? 0.f : 1.f / r.l[j];
-        T* at = (T*)p.out + (size_t)(d.q_start + row / G) * p.ldo + (size_t)(kvh * G + row % G) * D + g * (D / 8) + 2 * (pair / NT);
-        if (SP == 2) *reinterpret_cast<float2*>(at) = make_float2(r.o[j] * inv, r.o[j + 2] * inv);
-        else *reinterpret_cast<__nv_bfloat162*>(at) = __floats2bfloat162_rn(r.o[j] * inv, r.o[j + 2] * inv);
-      }
-    };
-    auto store = [&](float* slot, int pair, const Tile& r) {
+    auto store = [&](float* slot, int pair, const Rw8Tile& r) {
 #pragma unroll
       for (int j = 0; j < 4; ++j) __stcg(slot + (pair * 4 + j) * 32 + lane, r.o[j]);
       if (pair < NT && g == 0) {
@@ -640,59 +674,65 @@ __global__ void __launch_bounds__(RW8_WARPS * 32, (Rw8Cfg<D, NT, T>::BLOCKS)) at
       }
     };
     for (int pair = warp; pair < C::PAIRS; pair += RW8_WARPS) {
-      const Tile r = gather(pair, 0, RW8_WARPS, 1, [&](int w) { return (const float*)state_of(w, s_stage[w]); }, [](const float* x) { return *x; });
+      const Rw8Tile r = rw8_gather<C, NT>(pair, 0, RW8_WARPS, 1, [&](int w) { return (const float*)state_of(w, s_stage[w]); }, [](const float* x) { return *x; });
       if (shared_out) store(my_slot, pair, r);
-      else write_out(pair, r);
+      else rw8_write<D, NT, T>(p, d, kvh, pair, r);
     }
-    if (shared_out) {
-      __threadfence();
-      __syncthreads();
-      int* ticket = p.tickets + (size_t)e * Hkv + kvh;
-      if (threadIdx.x == 0) {
-        s_last = atomicAdd(ticket, 1) == c_last - c_first;
-        __threadfence();
-      }
-      __syncthreads();
-      if (s_last) {
-        // the parts in order, a tile's shared by the warps that have no tile of their own (past L1: a line of it may hold the
-        // neighbour of a slot that was read before the neighbour was written)
-        constexpr int SHARE = C::PAIRS < RW8_WARPS ? RW8_WARPS / C::PAIRS : 1;
-        const int n_parts = c_last - c_first + 1;
-        for (int pair = warp / SHARE; pair < C::PAIRS; pair += RW8_WARPS / SHARE) {
-          Tile r = gather(pair, warp % SHARE, n_parts, SHARE,
-                          [&](int i) { return (const float*)(p.slots + (size_t)(i == 0 ? first_slot : 2 * (c_first + i)) * C::SLOT); },
-                          [](const float* x) { return __ldcg(x); });
-          if (SHARE > 1) {
-            float* mine = state_of(warp, s_stage[warp]);
-            mine[lane] = r.o[0], mine[32 + lane] = r.o[1], mine[64 + lane] = r.o[2], mine[96 + lane] = r.o[3];
-            mine[128 + lane] = r.m[0], mine[160 + lane] = r.m[1], mine[192 + lane] = r.l[0], mine[224 + lane] = r.l[1];
-            __syncthreads();
-            if (warp % SHARE) break;
-#pragma unroll
-            for (int w = 1; w < SHARE; ++w) {
-              const float* x = state_of(warp + w, s_stage[warp + w]) + lane;
-#pragma unroll
-              for (int j = 0; j < 2; ++j) {
-                const float m = x[128 + 32 * j], top = fmaxf(r.m[j], m);
-                const float f = r.m[j] == -INFINITY ? 1.f : fast_exp2(r.m[j] - top), h = m == -INFINITY ? 1.f : fast_exp2(m - top);
-                r.l[j] = rescale8(r.l[j], r.m[j] == -INFINITY ? 0.f : r.m[j] - top) + rescale8(x[192 + 32 * j], m == -INFINITY ? 0.f : m - top);
-                r.m[j] = top;
-                r.o[j] = r.o[j] * f + x[32 * j] * h;
-                r.o[j + 2] = r.o[j + 2] * f + x[64 + 32 * j] * h;
-              }
-            }
-          }
-          write_out(pair, r);
-        }
-        if (threadIdx.x == 0) *ticket = 0;
-      }
-    }
-    __syncthreads();                       // the stages may be filled again, s_last and s_stage written
+    __syncthreads();                       // the stages may be filled again, s_stage written
   }
   cp_async_wait_all();
+  if (threadIdx.x < 2) p.whose[2 * blockIdx.x + threadIdx.x] = mine[threadIdx.x];
 }
 
-template <int D, int NT, int HELD, typename T> int launch_rows8(const Rows8Params& p, int n_entries, int grid, cudaStream_t stream) {
+// The (entry, kv head)s that several blocks have pages of: block c joins the one whose first part block c of the kernel above left.
+template <int D, int NT, typename T> __global__ void __launch_bounds__(RW8_WARPS * 32) rows8_join_kernel(Rows8Params p) {
+  using C = Rw8Cfg<D, NT, T>;
+  constexpr int SHARE = C::PAIRS < RW8_WARPS ? RW8_WARPS / C::PAIRS : 1;      // warps that share a tile's parts
+  __shared__ float s_tile[RW8_WARPS][256];
+  const int c = blockIdx.x, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  pdl_wait();
+  pdl_launch_dependents();
+  const int last = (int)gridDim.x - 1, w0 = p.whose[2 * c], w1 = p.whose[2 * c + 1];
+  int next = p.whose[2 * min(c + 1 + lane, last)];         // (asked for with the others: the loads are the kernel's time)
+  const int which = (w1 & 1) ? 1 : 0, id = which ? w1 : w0;
+  if (!(id & 1)) return;
+  int n_parts = 1;
+  for (int z0 = c + 1;; z0 += 32) {
+    const uint32_t other = __ballot_sync(0xffffffffu, z0 + lane > last || next != id - 1);
+    n_parts += other ? __ffs(other) - 1 : 32;
+    if (other) break;
+    next = p.whose[2 * min(z0 + 32 + lane, last)];
+  }
+  const int pair_id = (id >> 1) - 1, e = pair_id / p.kv.n_kv_heads, kvh = pair_id - e * p.kv.n_kv_heads;
+  const Rw8Entry d = rw8_entry(p, e, 8 * NT);
+  for (int pair = warp / SHARE; pair < C::PAIRS; pair += RW8_WARPS / SHARE) {
+    Rw8Tile r = rw8_gather<C, NT>(pair, warp % SHARE, n_parts, SHARE,
+                                  [&](int z) { return (const float*)(p.slots + (size_t)(2 * (c + z) + (z == 0 ? which : 0)) * C::SLOT); },
+                                  [](const float* x) { return *x; });
+    if (SHARE > 1) {                       // (once through the loop)
+      float* mine = s_tile[warp] + lane;
+      mine[0] = r.o[0], mine[32] = r.o[1], mine[64] = r.o[2], mine[96] = r.o[3], mine[128] = r.m[0], mine[160] = r.m[1], mine[192] = r.l[0], mine[224] = r.l[1];
+      __syncthreads();
+      if (warp % SHARE) return;
+#pragma unroll
+      for (int w = 1; w < SHARE; ++w) {
+        const float* x = s_tile[warp + w] + lane;
+#pragma unroll
+        for (int j = 0; j < 2; ++j) {
+          const float m = x[128 + 32 * j], top = fmaxf(r.m[j], m);
+          const float f = r.m[j] == -INFINITY ? 0.f : r.m[j] - top, h = m == -INFINITY ? 0.f : m - top;
+          r.l[j] = rescale8(r.l[j], f) + rescale8(x[192 + 32 * j], h);
+          r.m[j] = top;
+          r.o[j] = r.o[j] * fast_exp2(f) + x[32 * j] * fast_exp2(h);
+          r.o[j + 2] = r.o[j + 2] * fast_exp2(f) + x[64 + 32 * j] * fast_exp2(h);
+        }
+      }
+    }
+    rw8_write<D, NT, T>(p, d, kvh, pair, r);
+  }
+}
+
+template <int D, int NT, int HELD, typename T> int launch_rows8(const Rows8Params& p, int n_entries, int grid, int most_pages, cudaStream_t stream) {
   using C = Rw8Cfg<D, NT, T>;
   constexpr auto kernel = attention_rows8_kernel<D, NT, HELD, T>;
   static PerDevice<bool> configured;
@@ -704,9 +744,12 @@ template <int D, int NT, int HELD, typename T> int launch_rows8(const Rows8Param
   const size_t smem = C::RING + C::MERGE + 4 * ((size_t)n_entries + 1);
   // no more blocks than are resident: many entries' table may leave room for one a SM only (228 KB; a block's own 1 KB and its statics)
   const int fit = (int)((228 << 10) / (smem + 1280));
-  const int resident = min(C::BLOCKS, max(1, fit)) * sm_count();
-  const Rw8Cut cut = {4, 1024 / D, 512 / D};
-  return launch_pdl(PDL_ATTENTION, kernel, (unsigned)min(grid, resident), RW8_WARPS * 32, smem, stream, p, n_entries, cut);
+  grid = min(grid, min(C::BLOCKS, max(1, fit)) * sm_count());
+  const Rw8Cut cut = {8, 1024 / D, 512 / D};
+  const int rc = launch_pdl(PDL_ATTENTION, kernel, (unsigned)grid, RW8_WARPS * 32, smem, stream, p, n_entries, cut);
+  // (short (entry, kv head)s that have a block each leave no parts)
+  if (rc != LLMI_OK || ((long)n_entries * p.kv.n_kv_heads <= grid && most_pages <= cut.least)) return rc;
+  return launch_pdl(PDL_ATTENTION, rows8_join_kernel<D, NT, T>, (unsigned)grid, RW8_WARPS * 32, 0, stream, p);
 }
 
 // Eighths of query rows in a tile: the fewest that hold a sequence's rows, of those there are.
@@ -720,31 +763,26 @@ inline int rw8_grid(long units) { return (int)(units < 2L * sm_count() ? units :
 
 using namespace llmi;
 
-// What a call needs: *floats of scratch for the blocks' partial results, *ints tickets (zero before the first call; every call
-// leaves them zero).  `max_q`: most tokens that a sequence brings.
-LLMI_EXPORT int llmi_attention_rows8_workspace(int dtype, int n_seqs, int max_q, int n_heads, int n_kv_heads, int head_dim, int table_pages, long* floats,
-                                               long* ints) {
+// The floats of scratch for the blocks' partial results (of any content); below 0: the sizes are not taken.  `max_q`: most tokens that a
+// sequence brings.
+LLMI_EXPORT long llmi_attention_rows8_workspace(int dtype, int n_seqs, int max_q, int n_heads, int n_kv_heads, int head_dim, int table_pages) {
   if (n_seqs <= 0 || max_q <= 0 || n_kv_heads <= 0 || n_heads <= 0 || n_heads % n_kv_heads || (head_dim != 64 && head_dim != 128) || table_pages <= 0)
     return LLMI_ERR_BAD_SIZE;
   const long rows = (long)max_q * (n_heads / n_kv_heads);
   const int nt = rw8_tiles(dtype, head_dim, rows);
   const long tiles = (rows + 8 * nt - 1) / (8 * nt);
   if (n_seqs * tiles > RW8_MAX_ENTRIES || n_seqs * tiles * n_kv_heads * ((long)table_pages + 64) > 0x7fffffffL) return LLMI_ERR_BAD_SIZE;
-  *ints = n_seqs * tiles * n_kv_heads;
-  *floats = 2L * rw8_grid(n_seqs * tiles * n_kv_heads * (long)table_pages) * (head_dim / 16 * nt * 128 + 16 * nt);
-  return LLMI_OK;
+  return 2L * rw8_grid(n_seqs * tiles * n_kv_heads * (long)table_pages) * (head_dim / 16 * nt * 128 + 16 * nt + 1);
 }
 
 LLMI_EXPORT int llmi_attention_rows8(int dtype, int held, const void* q, long ldq, void* out, long ldo, const void* k_codes, const float* k_scales,
                                      const void* v_codes, const float* v_scales, const int32_t* seq_q_start, const int32_t* seq_kv_len,
                                      const int32_t* seq_pages, int pages_stride, int table_pages, int n_seqs, int n_pages, int max_q,
                                      int n_heads, int n_kv_heads, int head_dim, float scale, int window, int q_f32, float* slots, long n_floats,
-                                     int* tickets, long n_ints, cudaStream_t stream) {
-  long floats, ints;
+                                     cudaStream_t stream) {
   if (dtype != LLMI_DTYPE_F32 && dtype != LLMI_DTYPE_BF16) return LLMI_ERR_BAD_DTYPE;
-  const int rc = llmi_attention_rows8_workspace(dtype, n_seqs, max_q, n_heads, n_kv_heads, head_dim, table_pages, &floats, &ints);
-  if (rc != LLMI_OK) return rc;
-  if (n_floats < floats || n_ints < ints || n_pages <= 0 || window < 0) return LLMI_ERR_BAD_SIZE;
+  const long floats = llmi_attention_rows8_workspace(dtype, n_seqs, max_q, n_heads, n_kv_heads, head_dim, table_pages);
+  if (floats < 0 || n_floats < floats || n_pages <= 0 || window < 0) return LLMI_ERR_BAD_SIZE;
   if (held != HELD_INT8 && held != HELD_E4M3) return LLMI_ERR_BAD_DTYPE;
   const long even = dtype == LLMI_DTYPE_F32 ? 3 : 7;         // rows are whole 16-byte pieces
   if ((((uintptr_t)q | (uintptr_t)out | (uintptr_t)k_codes | (uintptr_t)v_codes | (uintptr_t)k_scales | (uintptr_t)v_scales) & 15) || (ldq & (q_f32 ? 3 : even)) || (ldo & even))
@@ -754,10 +792,13 @@ LLMI_EXPORT int llmi_attention_rows8(int dtype, int held, const void* q, long ld
   const int nt = rw8_tiles(dtype, head_dim, rows), tiles = (int)((rows + 8 * nt - 1) / (8 * nt));
   Rows8Params p{q, ldq, out, ldo, (const uint8_t*)k_codes, k_scales, (const uint8_t*)v_codes, v_scales,
                 seq_q_start, seq_kv_len, Paged8{seq_pages, pages_stride, table_pages, n_pages, n_kv_heads, head_dim}, n_seqs, group, tiles,
-                scale * 1.4426950408889634f, window, q_f32, slots, tickets};
+                scale * 1.4426950408889634f, window, q_f32, slots, nullptr};
   const int n_entries = n_seqs * tiles, grid = rw8_grid((long)n_entries * n_kv_heads * table_pages);
+  p.whose = reinterpret_cast<int*>(slots + 2L * grid * (head_dim / 16 * nt * 128 + 16 * nt));
+  // most pages that a (sequence, kv head)'s rows of a tile see
+  const int most_pages = window > 0 && (window + max_q) / PAGE8 + 2 < table_pages ? (window + max_q) / PAGE8 + 2 : table_pages;
 #define LLMI_ROWS8(D_, NT_, T_) \
-  (held == HELD_INT8 ? launch_rows8<D_, NT_, HELD_INT8, T_>(p, n_entries, grid, stream) : launch_rows8<D_, NT_, HELD_E4M3, T_>(p, n_entries, grid, stream))
+  (held == HELD_INT8 ? launch_rows8<D_, NT_, HELD_INT8, T_>(p, n_entries, grid, most_pages, stream) : launch_rows8<D_, NT_, HELD_E4M3, T_>(p, n_entries, grid, most_pages, stream))
   if (dtype == LLMI_DTYPE_F32) return head_dim == 128 ? LLMI_ROWS8(128, 1, float) : nt == 1 ? LLMI_ROWS8(64, 1, float) : LLMI_ROWS8(64, 2, float);
   if (head_dim == 64) return nt == 1 ? LLMI_ROWS8(64, 1, __nv_bfloat16) : nt == 2 ? LLMI_ROWS8(64, 2, __nv_bfloat16) : LLMI_ROWS8(64, 4, __nv_bfloat16);
   return nt == 1 ? LLMI_ROWS8(128, 1, __nv_bfloat16) : LLMI_ROWS8(128, 2, __nv_bfloat16);

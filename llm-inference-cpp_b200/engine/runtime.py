@@ -36,15 +36,6 @@ class Runtime:
             self.generation += 1
         return buf[:n].view(*shape)
 
-    def zeroed(self, name: str, n: int) -> torch.Tensor:
-        """At least ``n`` int32 words that were zero when they were made, for kernels that leave them zero."""
-        buf = self._buffers.get(name)
-        if buf is None or buf.numel() < n:
-            buf = torch.zeros(max(n, 2 * buf.numel() if buf is not None else 256), dtype=torch.int32, device=self.device)
-            self._buffers[name] = buf
-            self.generation += 1
-        return buf
-
     def to_compute(self, t: torch.Tensor) -> torch.Tensor:
         """A matrix in the compute type (bf16 stays bf16; widening to fp32 is exact)."""
         return t.to(device=self.device, dtype=self.dtype).contiguous()

@@ -170,13 +170,14 @@ def lib():
                      "llmi_normed_pair", "llmi_stream_axpy_norm", "llmi_stream_postnorm", "llmi_softcap_rows", "llmi_moe_table",
                      "llmi_qkv_unit_prepare", "llmi_latent_prepare_direct", "llmi_channel_token_supported",
                      "llmi_channel_token_prepare", "llmi_channel_token_step", "llmi_cast_rows", "llmi_heads_token", "llmi_heads_token_supported",
-                     "llmi_rope_store8", "llmi_attention_any8", "llmi_attention_rows8", "llmi_attention_rows8_workspace", "llmi_attention_prompt8"):
+                     "llmi_rope_store8", "llmi_attention_any8", "llmi_attention_rows8", "llmi_attention_prompt8"):
             getattr(l, name).restype = c_int
         l.llmi_gemm_tc_workspace.restype = c_long
         l.llmi_delta_state_floats.restype = c_long
         l.llmi_attention_latent_mma_workspace.restype = c_long
         l.llmi_attention_maps_mma_workspace.restype = c_long
         l.llmi_moe_group_ints.restype = c_long
+        l.llmi_attention_rows8_workspace.restype = c_long
         l.llmi_attention_decode_workspace.restype = c_long
         # The launchers of a prompt's step are called a few hundred times per step from Python: with their argument
         # types declared, plain integers go in without a ctypes object being made for each (a third of a call's cost).
@@ -187,7 +188,7 @@ def lib():
         l.llmi_attention_prefill_tc.argtypes = [P, L, L, P, L, P, P, L, P, I, P, P, I, I, I, I, I, F, I, I, I, P, L, P, I, P, I, P, P, L, P, I, P, L, P, P, P, I, I, I, P, P]
         l.llmi_rope_store8.argtypes = [I, I, P, L, P, L, P, I, P, P, P, I, I, I, P, P, P, P, I, I, I, I, I, I, I, P]
         l.llmi_attention_any8.argtypes = [I, I, P, L, P, L, P, P, P, P, P, P, P, I, I, I, I, I, I, I, I, F, I, I, P]
-        l.llmi_attention_rows8.argtypes = [I, I, P, L, P, L, P, P, P, P, P, P, P, I, I, I, I, I, I, I, I, F, I, I, P, L, P, L, P]
+        l.llmi_attention_rows8.argtypes = [I, I, P, L, P, L, P, P, P, P, P, P, P, I, I, I, I, I, I, I, I, F, I, I, P, L, P]
         l.llmi_attention_prompt8.argtypes = [I, P, L, P, L, P, P, P, P, P, P, P, I, I, I, I, I, I, I, I, F, I, I, I, I, P, L, P, P]
         _configured = True
     return l
@@ -2214,36 +2215,17 @@ def _rope_store8(held: int, qkv, q_out, inv_freq, rotary_dim, tok_seq, tok_pos, 
 
 
 _sizes8: dict = {}
-_kept8: dict = {}
 
 
-def _rows8_sizes(dtype: int, n_seqs: int, max_q: int, n_heads: int, n_kv_heads: int, head_dim: int, table_pages: int) -> tuple | None:
-    """(floats of scratch, tickets) that attention_rows8 needs, None where it does not take the sizes."""
+def _rows8_floats(dtype: int, n_seqs: int, max_q: int, n_heads: int, n_kv_heads: int, head_dim: int, table_pages: int) -> int:
+    """The fp32 numbers of scratch that the kernel for few rows needs, below 0 where it does not take the sizes."""
     key = (dtype, n_seqs, max_q, n_heads, n_kv_heads, head_dim, table_pages)
-    sizes = _sizes8.get(key, False)
-    if sizes is False:
-        floats, ints = c_long(0), c_long(0)
-        rc = lib().llmi_attention_rows8_workspace(*map(c_int, key), ctypes.byref(floats), ctypes.byref(ints))
+    n = _sizes8.get(key)
+    if n is None:
         if len(_sizes8) >= 4096:
             _sizes8.clear()
-        sizes = _sizes8[key] = (floats.value, ints.value) if rc == 0 else None
-    return sizes
-
-
-def _workspace8(device: int, stream: int, rt, n_floats: int, n_ints: int) -> tuple:
-    """Scratch and zeroed tickets: the model's (``rt``), else kept per device and stream; a call that is captured has its own, since a
-    graph may be replayed beside anything."""
-    if rt is not None:
-        return rt.scratch("attn8_slots", (max(n_floats, 1),), torch.float32), rt.zeroed("attn8_tickets", max(n_ints, 1))
-    capturing = torch.cuda.is_current_stream_capturing()
-    key = (device, stream)
-    kept = None if capturing else _kept8.get(key)
-    if kept is None or kept[0].numel() < n_floats or kept[1].numel() < n_ints:
-        kept = (torch.empty(max(n_floats, 1), dtype=torch.float32, device=torch.device("cuda", device)),
-                torch.zeros(max(n_ints, 1), dtype=torch.int32, device=torch.device("cuda", device)))
-        if not capturing:
-            _kept8[key] = kept
-    return kept
+        n = _sizes8[key] = int(lib().llmi_attention_rows8_workspace(*map(c_int, key)))
+    return n
 
 
 _PROMPT8_PART_PAGES = 8       # the least pages of a part of a block of 256 query rows
@@ -2313,12 +2295,11 @@ def attention8(q: torch.Tensor, out: torch.Tensor, k: Rows8, v: Rows8, ctx, seq_
             *rows, start, kv_len, *table, n_blocks, n_heads, n_kv_heads, head_dim, scale, window, q_f32, parts, _PROMPT8_PART_PAGES,
             partials.data_ptr() if parts > 1 else None, partials.numel() if parts > 1 else 0, tc_scratch(q.device).error.data_ptr(), stream))
         return
-    sizes = _rows8_sizes(dtype, S, max_q, n_heads, n_kv_heads, head_dim, P) if kernel in (None, "rows") and fast else None
-    if sizes is not None:
-        slots, tickets = _workspace8(device, stream, rt, *sizes)
+    floats = _rows8_floats(dtype, S, max_q, n_heads, n_kv_heads, head_dim, P) if kernel in (None, "rows") and fast else -1
+    if floats >= 0:
+        slots = rt.scratch("attn8_slots", (floats,), torch.float32) if rt is not None else torch.empty(floats, dtype=torch.float32, device=q.device)
         _check("attention_rows8", lib().llmi_attention_rows8(
-            dtype, *rows, start, kv_len, *table, max_q, n_heads, n_kv_heads, head_dim, scale, window, q_f32, slots.data_ptr(), slots.numel(),
-            tickets.data_ptr(), tickets.numel(), stream))
+            dtype, *rows, start, kv_len, *table, max_q, n_heads, n_kv_heads, head_dim, scale, window, q_f32, slots.data_ptr(), floats, stream))
         return
     if kernel not in (None, "any"):
         raise KernelError(f"{name}: the kernel {kernel!r} does not take this call")

@@ -27,6 +27,8 @@
 // row in a workspace; a second kernel joins them in order.  Waits are bounded (sm100.cuh).
 #include <math.h>
 
+#include <type_traits>
+
 #include "mma_sync.cuh"
 #include "rows8.cuh"
 #include "tc_common.cuh"
@@ -38,6 +40,7 @@ constexpr int P8_ROWS = 256, P8_TILE = 128;
 // 20 .. 23 codes to fp16.
 constexpr int P8_SOFTMAX = 4, P8_CONVERT = 20, P8_WARPS = 24;
 constexpr int P8_THREADS = P8_WARPS * 32;
+constexpr int P8_JOINS = 16;              // blocks of 8 warps that join a block's rows
 constexpr int P8_TMEM = 512;              // per tile of rows 256 columns: S of even and odd pages (64 each), O (D)
 constexpr float P8_LAZY = 8.0f;           // the reference maximum follows where it is 2^8 behind
 constexpr uint32_t PG_WIDE = 1u, PG_POISON = 2u;       // the page's scales are far apart; it has values that are no numbers
@@ -199,13 +202,14 @@ __global__ void __launch_bounds__(P8_THREADS, 1) attention_prompt8_kernel(Prompt
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int kvh = blockIdx.x, G = p.group, Hkv = p.kv.n_kv_heads;
   const int blk = blockIdx.y / p.parts, part = blockIdx.y % p.parts;
-  pdl_wait();
-  const P8Block d = prompt8_block(p, blk);
-  if (d.rows <= 0) return;
+  const P8Block d = prompt8_block(p, blk);               // (of the step's index block)
   const int2 cut = prompt8_parts(p, d.n_pages);
-  if (part >= cut.x) return;
   const int v0 = part * cut.y, n_pg = min(cut.y, d.n_pages - v0);
-  if (n_pg <= 0) return;                                 // (positions below 0 only: nothing to see)
+  // (no such block or part; positions below 0 only: nothing to see)
+  if (d.rows <= 0 || part >= cut.x || n_pg <= 0) {
+    pdl_wait();
+    return;
+  }
   const int pg0 = d.pg_first + v0;                       // this part's first page
   // pages of this part that a tile's rows see the first key of
   int n_tile[2];
@@ -237,6 +241,7 @@ __global__ void __launch_bounds__(P8_THREADS, 1) attention_prompt8_kernel(Prompt
   asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
   uint32_t tmem;
   asm volatile("ld.shared.u32 %0, [%1];" : "=r"(tmem) : "r"(tmem_slot));
+  pdl_wait();
   pdl_launch_dependents();      // (not ahead of the tensor memory: a kernel behind this one could take it and wait for this block)
 
   // the page of the pool that page j of this part is, or -1
@@ -384,54 +389,70 @@ __global__ void __launch_bounds__(P8_THREADS, 1) attention_prompt8_kernel(Prompt
                    : "=r"(r) : "r"(1 + tile * 4 + quad), "r"(x ? 1u : 0u) : "memory");
       return r != 0u;
     };
-    // the row's queries, divided by a power of two above the largest
+    // The rows' queries, divided by a power of two above the row's largest.  The two warps of 32 rows take 16 each, the lanes of a row
+    // beside each other, with a row's 8 entries a lane and BATCH loads under way.
     float row_fac;
     {
-      const size_t src = (size_t)(d.q_start + (row_ok ? tok : 0)) * p.ldq + (size_t)head * D;
-      auto eight = [&](int c, float (&x)[8]) {                     // entries 8 c .. 8 c + 7; zeros for a row that there is none of
-        if (p.q_f32) {
-          const float4* f = reinterpret_cast<const float4*>((const float*)p.q + src + 8 * c);
-          const float4 u = row_ok ? f[0] : make_float4(0.f, 0.f, 0.f, 0.f), v = row_ok ? f[1] : make_float4(0.f, 0.f, 0.f, 0.f);
-          x[0] = u.x, x[1] = u.y, x[2] = u.z, x[3] = u.w, x[4] = v.x, x[5] = v.y, x[6] = v.z, x[7] = v.w;
-        } else {
-          const uint4 raw = row_ok ? *reinterpret_cast<const uint4*>((const __nv_bfloat16*)p.q + src + 8 * c) : make_uint4(0u, 0u, 0u, 0u);
-          const __nv_bfloat162* b = reinterpret_cast<const __nv_bfloat162*>(&raw);
+      constexpr int LANES = D / 8, AT_ONCE = 32 / LANES, BATCH = 4;
+      const int c = lane % LANES;
+      auto queries = [&](auto f32) {
+#pragma unroll 1
+        for (int r0 = quad * 32 + half * 16; r0 < quad * 32 + half * 16 + 16; r0 += BATCH * AT_ONCE) {
+          uint4 raw[BATCH][decltype(f32)::value ? 2 : 1];
 #pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            const float2 f = __bfloat1622float2(b[i]);
-            x[2 * i] = f.x, x[2 * i + 1] = f.y;
+          for (int i = 0; i < BATCH; ++i) {
+            const int r2 = tile * P8_TILE + r0 + i * AT_ONCE + lane / LANES, row2 = d.row0 + r2;
+            const size_t src = (size_t)(d.q_start + row2 / G) * p.ldq + (size_t)(kvh * G + row2 % G) * D + 8 * c;
+            const uint4* from = decltype(f32)::value ? reinterpret_cast<const uint4*>((const float*)p.q + src) : reinterpret_cast<const uint4*>((const __nv_bfloat16*)p.q + src);
+#pragma unroll
+            for (int u = 0; u < (decltype(f32)::value ? 2 : 1); ++u) raw[i][u] = r2 < d.rows ? from[u] : make_uint4(0u, 0u, 0u, 0u);
+          }
+#pragma unroll
+          for (int i = 0; i < BATCH; ++i) {
+            const int in = r0 + i * AT_ONCE + lane / LANES;
+            float x[8];
+            if (decltype(f32)::value) {
+#pragma unroll
+              for (int u = 0; u < 2; ++u) {
+                const uint4 w = raw[i][decltype(f32)::value ? u : 0];
+                x[4 * u] = __uint_as_float(w.x), x[4 * u + 1] = __uint_as_float(w.y), x[4 * u + 2] = __uint_as_float(w.z), x[4 * u + 3] = __uint_as_float(w.w);
+              }
+            } else {
+              const uint32_t w[4] = {raw[i][0].x, raw[i][0].y, raw[i][0].z, raw[i][0].w};
+#pragma unroll
+              for (int e = 0; e < 4; ++e) {
+                x[2 * e] = __uint_as_float(w[e] << 16);
+                x[2 * e + 1] = __uint_as_float(w[e] & 0xffff0000u);
+              }
+            }
+            float a = 0.f;
+#pragma unroll
+            for (int e = 0; e < 8; ++e) a = fmaxf(a, fabsf(x[e]));
+#pragma unroll
+            for (int o = LANES / 2; o; o >>= 1) a = fmaxf(a, __shfl_xor_sync(0xffffffffu, a, o));
+            int ex = 0;
+            if (a > 0.f && a <= FLT_MAX) ex = max(-100, (int)((__float_as_uint(a) >> 23) & 255) - 126);
+            float down = __uint_as_float((uint32_t)(127 - min(ex, 126)) << 23);
+            const float down2 = ex > 126 ? 1.f / (float)(1 << (ex - 126)) : 1.f;
+            if (p.scale_log2 < 0.f) down = -down;                  // the factor of the scores below is positive
+            // (never quite 0: 0 times a masked key's -inf is no number)
+            if (c == 0) s_top[tile][0][in] = fmaxf(ldexpf(fabsf(p.scale_log2), ex), 1e-30f);
+            uint32_t h[4];
+#pragma unroll
+            for (int e = 0; e < 4; ++e) h[e] = half2_bits(__floats2half2_rn(x[2 * e] * down * down2, x[2 * e + 1] * down * down2));
+            asm volatile("st.shared.v4.u32 [%0], {%1, %2, %3, %4};"
+                         ::"r"(q_smem + tile * C::Q_TILE + in * 128 + (c / 8) * (P8_TILE * 128) + (((c % 8) ^ (in & 7)) << 4)),
+                         "r"(h[0]), "r"(h[1]), "r"(h[2]), "r"(h[3]) : "memory");
           }
         }
       };
-      float a = 0.f;
-#pragma unroll
-      for (int c = 0; c < D / 8; ++c) {
-        float x[8];
-        eight(c, x);
-#pragma unroll
-        for (int i = 0; i < 8; ++i) a = fmaxf(a, fabsf(x[i]));
-      }
-      int ex = 0;
-      if (a > 0.f && a <= FLT_MAX) ex = max(-100, (int)((__float_as_uint(a) >> 23) & 255) - 126);
-      float down = __uint_as_float((uint32_t)(127 - min(ex, 126)) << 23);
-      const float down2 = ex > 126 ? 1.f / (float)(1 << (ex - 126)) : 1.f;
-      if (p.scale_log2 < 0.f) down = -down;                        // the factor of the scores below is positive
-      row_fac = fmaxf(ldexpf(fabsf(p.scale_log2), ex), 1e-30f);    // (never quite 0: 0 times a masked key's -inf is no number)
-      const uint32_t at = q_smem + tile * C::Q_TILE + in_tile * 128;
-#pragma unroll
-      for (int i = 0; i < HD / 8; ++i) {
-        const int c = half * (HD / 8) + i;
-        float x[8];
-        eight(c, x);
-        uint32_t h[4];
-#pragma unroll
-        for (int e = 0; e < 4; ++e) h[e] = half2_bits(__floats2half2_rn(x[2 * e] * down * down2, x[2 * e + 1] * down * down2));
-        asm volatile("st.shared.v4.u32 [%0], {%1, %2, %3, %4};"
-                     ::"r"(at + (c / 8) * (P8_TILE * 128) + (((c % 8) ^ (lane & 7)) << 4)), "r"(h[0]), "r"(h[1]), "r"(h[2]), "r"(h[3]) : "memory");
-      }
+      if (p.q_f32) queries(std::true_type{});
+      else queries(std::false_type{});
       asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
       __syncwarp();
       if (lane == 0) mbar_arrive(q_full);
+      meet();
+      row_fac = s_top[tile][0][in_tile];
     }
     const int n = n_tile[tile];
     const uint32_t t_lane = (uint32_t)(quad * 32) << 16, t_tile = tmem + 256u * tile + t_lane, t_o = t_tile + 128u + (uint32_t)(HD * half);
@@ -676,13 +697,13 @@ __global__ void __launch_bounds__(P8_THREADS, 1) attention_prompt8_kernel(Prompt
 // The parts of a block's rows, in order: a warp a row.
 template <int D>
 __global__ void __launch_bounds__(256) prompt8_join_kernel(Prompt8Params p) {
-  pdl_wait();
-  pdl_launch_dependents();
-  const int kvh = blockIdx.x, blk = blockIdx.y / 8, lane = threadIdx.x & 31, G = p.group;
+  const int kvh = blockIdx.x, blk = blockIdx.y / P8_JOINS, lane = threadIdx.x & 31, G = p.group;
   const P8Block d = prompt8_block(p, blk);
   const int2 cut = prompt8_parts(p, d.n_pages);
+  pdl_wait();
+  pdl_launch_dependents();
   if (d.rows <= 0 || d.n_pages <= 0 || cut.x <= 1) return;
-  for (int r = (blockIdx.y % 8) * 8 + (threadIdx.x >> 5); r < d.rows; r += 64) {
+  for (int r = (blockIdx.y % P8_JOINS) * 8 + (threadIdx.x >> 5); r < d.rows; r += 8 * P8_JOINS) {
     const float* slot = p.partials + ((size_t)blk * p.kv.n_kv_heads + kvh) * p.parts * (P8_ROWS * (D + 2));
     const size_t step = P8_ROWS * (D + 2);
     float m = -INFINITY, l = 0.f, o[D / 32];
@@ -716,7 +737,7 @@ template <int D, int HELD> int launch_prompt8(const Prompt8Params& p, int n_bloc
   const int rc = launch_pdl(PDL_ATTENTION, attention_prompt8_kernel<D, HELD>, dim3((unsigned)p.kv.n_kv_heads, (unsigned)(n_blocks * p.parts)), P8_THREADS,
                             P8Cfg<D>::SMEM, stream, p);
   if (rc != LLMI_OK || p.parts <= 1) return rc;
-  return launch_pdl(PDL_ATTENTION, prompt8_join_kernel<D>, dim3((unsigned)p.kv.n_kv_heads, (unsigned)(n_blocks * 8)), 256, 0, stream, p);
+  return launch_pdl(PDL_ATTENTION, prompt8_join_kernel<D>, dim3((unsigned)p.kv.n_kv_heads, (unsigned)(n_blocks * P8_JOINS)), 256, 0, stream, p);
 }
 
 }  // namespace llmi

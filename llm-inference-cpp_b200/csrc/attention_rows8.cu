@@ -87,10 +87,12 @@ __device__ __forceinline__ uint32_t transpose8x8(uint32_t v) {
 __device__ __forceinline__ uint32_t pack_half2(float lo, float hi) { return as_u32(__floats2half2_rn(lo, hi)); }
 
 // How the line of units is cut.  In pages: what a (sequence, kv head) costs beside its pages (its queries, the join of the warps, its
-// output), as units of no page at the front of its own; the least a range has; how near a border of two (sequence, kv head)s a cut is
-// moved to it (a part of one costs its partial result's way through memory and a ticket).
+// output), as units of no page at the front of its own; the most pages of the longest where each has a block of its own whatever their
+// number (the join of parts is a kernel of 4 us, 8 pages' time); the least a range has (one query head row, 9 heads of 64 by 3, 2,000
+// positions: 12.0 us in ranges of 16, 9.4 of 8, 9.0 of 4; 32 heads of 128 by 8, 4,000: 15.0 of 8, 16.3 of 4, 19.7 of 2: a part costs the
+// join as well); how near a border of two (sequence, kv head)s a cut is moved to it.
 struct Rw8Cut {
-  int front, least, near;
+  int front, most_whole, least, near;
 };
 
 // One (sequence, row tile): its rows and the pages that they see.
@@ -223,7 +225,7 @@ __global__ void __launch_bounds__(RW8_WARPS * 32, (Rw8Cfg<D, NT, T>::BLOCKS)) at
   }
   const int total = prefix[n_entries];
   // each its own block, or the line in even ranges
-  const bool whole = pairs <= (int)gridDim.x && (longest <= cut.least || (5 * pairs >= 3 * (int)gridDim.x && (long)(longest + cut.front) * pairs <= total + total / 4));
+  const bool whole = pairs <= (int)gridDim.x && (longest <= cut.most_whole || (5 * pairs >= 3 * (int)gridDim.x && (long)(longest + cut.front) * pairs <= total + total / 4));
   const int blocks = whole ? pairs : min((int)gridDim.x, max(total / cut.least, pairs));
   if (blockIdx.x >= blocks || total == 0) {
     pdl_wait();
@@ -745,10 +747,10 @@ template <int D, int NT, int HELD, typename T> int launch_rows8(const Rows8Param
   // no more blocks than are resident: many entries' table may leave room for one a SM only (228 KB; a block's own 1 KB and its statics)
   const int fit = (int)((228 << 10) / (smem + 1280));
   grid = min(grid, min(C::BLOCKS, max(1, fit)) * sm_count());
-  const Rw8Cut cut = {8, 1024 / D, 512 / D};
+  const Rw8Cut cut = {8, 1024 / D, 512 / D, 256 / D};
   const int rc = launch_pdl(PDL_ATTENTION, kernel, (unsigned)grid, RW8_WARPS * 32, smem, stream, p, n_entries, cut);
   // (short (entry, kv head)s that have a block each leave no parts)
-  if (rc != LLMI_OK || ((long)n_entries * p.kv.n_kv_heads <= grid && most_pages <= cut.least)) return rc;
+  if (rc != LLMI_OK || ((long)n_entries * p.kv.n_kv_heads <= grid && most_pages <= cut.most_whole)) return rc;
   return launch_pdl(PDL_ATTENTION, rows8_join_kernel<D, NT, T>, (unsigned)grid, RW8_WARPS * 32, 0, stream, p);
 }
 

@@ -249,6 +249,31 @@ def test_attention(dtype, held, H, G, D, step):
     check(b, H, q, attend(b, H, q, dtype), dtype)
 
 
+@pytest.mark.parametrize("kernel", ["rows", "prompt", "any"])
+@pytest.mark.parametrize("H,G,D,step", [(9, 3, 64, "one token"), (9, 3, 64, "a long prompt"), (8, 2, 128, "single tokens and padding"),
+                                        (32, 1, 128, "messages"), (4, 4, 64, "a portion"), (6, 2, 64, "a message on a long history"),
+                                        (16, 16, 128, "single tokens")])
+@pytest.mark.parametrize("window", [0, 90])
+def test_a_kernel_named(kernel, H, G, D, step, window):
+    """Each kernel takes what the others are chosen for."""
+    b = Batch(STEPS[step], G, D, "int8")
+    b.fill()
+    q = torch.tensor(b.rng.normal(size=(b.T, H * D)) * 1.5).to(torch.bfloat16).cuda()
+    out = torch.full((b.T, H * D), 7.0, dtype=torch.bfloat16, device="cuda")
+    K().attention8(q, out, b.k, b.v, b.ctx, b.table, H, G, D, D ** -0.5, window, kernel=kernel)
+    K().check_device_errors("cuda:0")
+    check(b, H, q, out, "bfloat16", window)
+
+
+@pytest.mark.parametrize("kernel,D,dtype", [("rows", 40, "bfloat16"), ("prompt", 32, "bfloat16"), ("prompt", 64, "float32"), ("columns", 64, "bfloat16")])
+def test_a_kernel_named_that_does_not_take_the_call(kernel, D, dtype):
+    b = Batch([(3, 10)], 2, D, "int8")
+    b.fill()
+    q = torch.zeros(3, 4 * D, dtype=DT[dtype], device="cuda")
+    with pytest.raises(K().KernelError, match=kernel):
+        K().attention8(q, torch.zeros_like(q), b.k, b.v, b.ctx, b.table, 4, 2, D, 0.1, kernel=kernel)
+
+
 @pytest.mark.parametrize("window", [1, 2, 63, 64, 65, 200])
 @pytest.mark.parametrize("H,G,D,step", [(9, 3, 64, "single tokens"), (9, 3, 64, "messages"), (8, 2, 128, "prompts"), (4, 4, 64, "a portion"),
                                         (4, 2, 32, "messages"), (32, 8, 128, "single tokens")])

@@ -11,7 +11,11 @@ namespace llmi {
 
 constexpr int ROPE8_MAX_HD = 256;
 constexpr int ROPE8_WARPS = 4;
-constexpr int ROPE8_MANY = 256, ROPE8_LANES = 16;      // from so many tokens on, threads of a token beside one another
+constexpr int ROPE8_THREADS = 512;                     // the most of a block
+// Heads of a token that are worked on at a time, each by threads of its own, where all heads would need more threads than the device
+// holds (all heads / 16 at a time: 256 tokens of 96 heads of 64 3.5 / 4.3 us, 1,000 of 48 of 128 10.0 / 5.9, 8,192 of 96 62.9 / 34.2).
+constexpr int ROPE8_LANES = 16;
+constexpr long ROPE8_HELD = 1024;                      // threads a SM
 
 struct Rope8Params {
   const void* qkv;
@@ -88,29 +92,25 @@ __global__ void __launch_bounds__(ROPE8_WARPS * 32) rope_store8_kernel(Rope8Para
 }
 
 // Whole-head rotation, or none, of heads that are 2^n 16-byte pieces twice (64, 128 and the like): a thread has one piece of the first
-// half of a head and its partner in the second, with the sines and cosines of the pairs between them, and walks over every
-// `lanes`-th head of the token; the threads of a head find its maximum by shuffles.  The angle of (position, pair) is the same for
-// all heads and sine and cosine are the costly part, so a prompt's threads take several heads (lanes = 16); a decode step's, which is all
-// latency, one each.  Bound by bytes: rows read once, q and the codes written once.
+// half of a head and its partner in the second and walks over every `lanes`-th head of the token; the threads of a head find its
+// maximum by shuffles.  The angle of (position, pair) is the same for all heads, and sine and cosine are the costly part: a block makes
+// each once, in shared memory.  Bound by bytes: rows read once, q and the codes written once.  8,192 tokens of 32 + 64 heads of 64 in
+// bf16 take 34 us, 5.0 TB/s (with the sines in every thread 43); 3,500 of 15 + 10 in fp32 14, 3.7 TB/s; a step's few tokens 2.6 to 3.0, a
+// kernel's latency.
 template <typename T> struct Piece8;
 template <> struct Piece8<float> {
   static constexpr int N = 4;
-  static __device__ __forceinline__ void load(const float* p, float* f) {
-    const float4 v = *reinterpret_cast<const float4*>(p);
-    f[0] = v.x, f[1] = v.y, f[2] = v.z, f[3] = v.w;
+  static __device__ __forceinline__ void numbers(const uint4& raw, float* f) {
+    f[0] = __uint_as_float(raw.x), f[1] = __uint_as_float(raw.y), f[2] = __uint_as_float(raw.z), f[3] = __uint_as_float(raw.w);
   }
   static __device__ __forceinline__ void store(float* p, const float* f) { *reinterpret_cast<float4*>(p) = make_float4(f[0], f[1], f[2], f[3]); }
 };
 template <> struct Piece8<__nv_bfloat16> {
   static constexpr int N = 8;
-  static __device__ __forceinline__ void load(const __nv_bfloat16* p, float* f) {
-    const uint4 raw = *reinterpret_cast<const uint4*>(p);
-    const __nv_bfloat162* h = reinterpret_cast<const __nv_bfloat162*>(&raw);
+  static __device__ __forceinline__ void numbers(const uint4& raw, float* f) {
+    const uint32_t w[4] = {raw.x, raw.y, raw.z, raw.w};
 #pragma unroll
-    for (int e = 0; e < 4; ++e) {
-      const float2 v = __bfloat1622float2(h[e]);
-      f[2 * e] = v.x, f[2 * e + 1] = v.y;
-    }
+    for (int e = 0; e < 4; ++e) f[2 * e] = __uint_as_float(w[e] << 16), f[2 * e + 1] = __uint_as_float(w[e] & 0xffff0000u);
   }
   static __device__ __forceinline__ void store(__nv_bfloat16* p, const float* f) {
     uint4 raw;
@@ -121,37 +121,64 @@ template <> struct Piece8<__nv_bfloat16> {
   }
 };
 
+// The larger in magnitude; NaN where one is.
+__device__ __forceinline__ float larger8(float m, float x) {
+  float r;
+  asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(m), "f"(fabsf(x)));
+  return r;
+}
+
 template <typename T, int HELD>
-__global__ void __launch_bounds__(128) rope_store8_rows_kernel(Rope8Params p, int lanes, int log_pieces) {
+__global__ void __launch_bounds__(ROPE8_THREADS) rope_store8_rows_kernel(Rope8Params p, int lanes, int log_pieces, int block_tokens) {
   constexpr int N = Piece8<T>::N;
+  extern __shared__ float2 turns[];        // [token][pair]: sine, cosine
   pdl_wait();
   pdl_launch_dependents();
   const int pieces = 1 << log_pieces, per_tok = lanes << log_pieces;       // (pieces divide a warp: a head's threads are neighbours)
-  const long item = (long)blockIdx.x * blockDim.x + threadIdx.x;
-  const long tok = item / per_tok;
-  const int rest = (int)(item - tok * per_tok), hl = rest >> log_pieces, i0 = (rest & (pieces - 1)) * N;
+  const int own = block_tokens == 1 ? 0 : (int)threadIdx.x / per_tok, rest = (int)threadIdx.x - own * per_tok, hl = rest >> log_pieces;
+  const int i0 = (rest & (pieces - 1)) * N;
+  const long tok0 = (long)blockIdx.x * block_tokens;
   // (threads without a token go along: the shuffles below are the whole warp's)
-  const bool there = tok < p.n_tokens;
-  const int t = there ? (int)tok : 0;
+  const bool there = own < block_tokens && hl < lanes && tok0 + own < p.n_tokens;
+  const int t = (int)(there ? tok0 + own : tok0);
+  const int hd = p.kv.head_dim, half = hd / 2, G = p.kv.n_kv_heads, heads = p.n_heads + (p.write_kv ? 2 * G : 0);
+  const T* row = (const T*)p.qkv + (size_t)t * p.ld;
+  // the rows of a head are under way while the one before is worked on
+  uint4 a4 = make_uint4(0u, 0u, 0u, 0u), b4 = a4;
+  auto ask = [&](int j) {
+    if (!there || j >= heads) return;
+    const T* src = row + (size_t)j * hd + i0;
+    a4 = *reinterpret_cast<const uint4*>(src), b4 = *reinterpret_cast<const uint4*>(src + half);
+  };
+  ask(hl);
   const int seq = p.tok_seq[t], pos = p.tok_pos[t];
   const bool live = there && seq >= 0 && seq < p.n_seqs && pos >= 0;
-  const int hd = p.kv.head_dim, half = hd / 2, G = p.kv.n_kv_heads, heads = p.n_heads + (p.write_kv ? 2 * G : 0);
   const int page = live && p.write_kv ? page8_of(p.kv, seq, pos) : -1;
   float sn[N], cs[N];
 #pragma unroll
-  for (int e = 0; e < N; ++e) {
-    if (p.rotary_dim > 0) sincosf(__fmul_rn((float)pos, p.inv_freq[i0 + e]), &sn[e], &cs[e]);
-    else sn[e] = 0.f, cs[e] = 1.f;
+  for (int e = 0; e < N; ++e) sn[e] = 0.f, cs[e] = 1.f;
+  if (p.rotary_dim > 0) {
+    const int n = (int)min((long)block_tokens, (long)p.n_tokens - tok0) * half;
+    for (int i = threadIdx.x; i < n; i += blockDim.x) {
+      const int tok = block_tokens == 1 ? 0 : i / half;
+      sincosf(__fmul_rn((float)p.tok_pos[tok0 + tok], p.inv_freq[i - tok * half]), &turns[i].x, &turns[i].y);
+    }
+    __syncthreads();
+    if (there) {
+#pragma unroll
+      for (int e = 0; e < N; ++e) {
+        const float2 x = turns[own * half + i0 + e];
+        sn[e] = x.x, cs[e] = x.y;
+      }
+    }
   }
-  const T* row = (const T*)p.qkv + (size_t)t * p.ld;
-#pragma unroll 2
   for (int j0 = 0; j0 < heads; j0 += lanes) {
     const int j = j0 + hl;
     const bool mine = live && j < heads;
     float a[N], b[N], lo[N], hi[N];
-    const T* src = row + (size_t)min(j, heads - 1) * hd + i0;
-    Piece8<T>::load(src, a);
-    Piece8<T>::load(src + half, b);
+    Piece8<T>::numbers(a4, a);
+    Piece8<T>::numbers(b4, b);
+    ask(j + lanes);
     const bool turned = j < p.n_heads + G && p.rotary_dim > 0;
 #pragma unroll
     for (int e = 0; e < N; ++e) {
@@ -172,15 +199,10 @@ __global__ void __launch_bounds__(128) rope_store8_rows_kernel(Rope8Params p, in
     }
     if (j0 + lanes <= p.n_heads) continue;                                 // queries only, for every thread
     float m = 0.f;
-    bool fine = true;
 #pragma unroll
-    for (int e = 0; e < N; ++e) {
-      m = fmaxf(m, fmaxf(fabsf(lo[e]), fabsf(hi[e])));
-      fine = fine && finite8(lo[e]) && finite8(hi[e]);
-    }
-    if (!fine) m = INFINITY;
-    for (int o = 1; o < pieces; o <<= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
-    fine = m <= FLT_MAX;
+    for (int e = 0; e < N; ++e) m = larger8(larger8(m, lo[e]), hi[e]);
+    for (int o = 1; o < pieces; o <<= 1) m = larger8(m, __shfl_xor_sync(0xffffffffu, m, o));
+    const bool fine = m <= FLT_MAX;
     if (!mine || j < p.n_heads || page < 0) continue;
     const bool key = j < p.n_heads + G;
     const Scale8 s = scale8<HELD>(m, fine);
@@ -208,10 +230,12 @@ int launch_rope_store8(const Rope8Params& p, cudaStream_t stream) {
       !(((uintptr_t)p.qkv | (uintptr_t)p.q_out | (uintptr_t)p.k_codes | (uintptr_t)p.v_codes) & 15) && !((p.ld * sizeof(T) | p.ldq * (p.q_f32 ? 4 : sizeof(T))) & 15)) {
     int log_pieces = 0;
     while ((1 << log_pieces) < pieces) ++log_pieces;
-    const int lanes = p.n_tokens >= ROPE8_MANY && heads > ROPE8_LANES ? ROPE8_LANES : heads;
-    const long n = ((long)p.n_tokens * lanes * pieces + 127) / 128;
-    if (n > 0x7fffffffL) return LLMI_ERR_BAD_SIZE;
-    return launch_pdl(PDL_ROPE, rope_store8_rows_kernel<T, HELD>, (unsigned)n, 128, 0, stream, p, lanes, log_pieces);
+    const bool many = (long)p.n_tokens * heads * pieces > ROPE8_HELD * sm_count();
+    const int most = many ? ROPE8_LANES : ROPE8_THREADS / pieces, lanes = heads < most ? heads : most;
+    const int per_tok = lanes * pieces, block_tokens = per_tok >= 128 ? 1 : 128 / per_tok;
+    const int threads = (block_tokens * per_tok + 31) / 32 * 32;
+    return launch_pdl(PDL_ROPE, rope_store8_rows_kernel<T, HELD>, (unsigned)((p.n_tokens + block_tokens - 1) / block_tokens), threads,
+                      block_tokens * (p.kv.head_dim / 2) * sizeof(float2), stream, p, lanes, log_pieces, block_tokens);
   }
   const long items = (long)p.n_tokens * (p.n_heads + (p.write_kv ? 2 * p.kv.n_kv_heads : 0));
   const long blocks = (items + ROPE8_WARPS - 1) / ROPE8_WARPS;

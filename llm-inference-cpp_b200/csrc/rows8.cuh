@@ -62,8 +62,9 @@ __device__ __forceinline__ bool finite8(float x) { return fabsf(x) <= FLT_MAX; }
 template <int HELD> __device__ __forceinline__ uint32_t codes8(float x0, float x1, float inv, bool finite) {
   if (!finite) return 0u;
   if (HELD == HELD_INT8) {
-    const int a = max(-127, min(127, __float2int_rn(__fmul_rn(x0, inv)))), b = max(-127, min(127, __float2int_rn(__fmul_rn(x1, inv))));
-    return (uint32_t)(a & 255) | ((uint32_t)(b & 255) << 8);
+    // (1.5 * 2^23 + x is rounded to an integer as rint does, which the low byte holds; |x| is 127 at most: a * rn(1 / rn(a / 127)))
+    const float a = __fadd_rn(__fmul_rn(x0, inv), 12582912.f), b = __fadd_rn(__fmul_rn(x1, inv), 12582912.f);
+    return __byte_perm(__float_as_uint(a), __float_as_uint(b), 0x0040) & 0xffffu;
   }
   uint16_t r;
   asm("cvt.rn.satfinite.e4m3x2.f32 %0, %1, %2;" : "=h"(r) : "f"(__fmul_rn(x1, inv)), "f"(__fmul_rn(x0, inv)));

@@ -9,19 +9,22 @@
 //   scales        a warp makes each row's factor of the page (three of them, for a page a stage each)
 //   codes -> fp16 four warps bring a page's codes into a ring with cp.async, each thread what it will read itself, so that nobody waits
 //                 for anybody (a thread that asks for bulk copies is busy half a microsecond with each: four a page were 2,000 clocks,
-//                 most of a page's time), and make K' = code * (k_scale / kmax) and V' = code * (v_scale / vmax) of a page, kmax and vmax its largest
-//                 scales, rounded to fp16 once (half a step is 2^-11 of a number; a bf16 cache's is 2^-8), in the swizzled layout
-//                 that the products read; so the scales cost the softmax nothing per key: kmax joins its scale, log2 vmax its offset.
-//                 (A page whose scales are more than 2^12 apart would lose bits of its small rows, which may be all that a query
-//                 sees: there K' and V' are the codes themselves and the softmax takes each key's scales.)
+//                 most of a page's time), and make K' = code * (k_scale / kmax) and V' = code * (v_scale / vmax) of a page, kmax and
+//                 vmax its largest scales, rounded to fp16 once (half a step is 2^-11 of a number; a bf16 cache's is 2^-8), in the
+//                 swizzled layout that the products read; so the scales cost the softmax nothing per key: kmax joins its scale,
+//                 log2 vmax its offset.  (A page whose scales are more than 2^12 apart would lose bits of its small rows, which may be
+//                 all that a query sees: there K' and V' are the codes themselves and the softmax takes each key's scales.)
 //   S = Q' K'^T   tcgen05.mma, Q' the queries divided by a power of two per row (fp16, exact but for entries 2^-14 of the largest)
-//   softmax       two threads own a row, 32 keys of a page each: tcgen05.ld, mask, maximum (exchanged), exp2, sum; P = 2^(s + log2 vmax - m) goes back to tensor memory
-//                 as fp16 over the S it has read; the sum of w is that of P / vmax
+//   softmax       two threads own a row, 32 keys of a page each: tcgen05.ld, mask, maximum, exp2, sum; P = 2^(s + log2 vmax - m) goes
+//                 back to tensor memory as fp16 over the S it has read; the sum of w is that of P / vmax
 //   O += P V'     tcgen05.mma with A in tensor memory, accumulating in fp32; m follows the running maximum (of s + log2 vmax) only
-//                 when that has grown by more than 8, so O is rescaled a few times per row
+//                 when that has grown by more than 8, so O is rescaled a few times per row, and only then the two threads exchange theirs
 //
-// What bounds it: the exponentials at head size 64 (16 a clock and SM; 64 x 128 of them a page and tile, 512 clocks), the products at
-// 128.  Two tiles share a converted page: the conversion, 2 x 64 x D codes, costs a sixth of their softmax.
+// What bounds it: a row's way through the softmax of a page, 1,800 clocks from S to P with four warps on each scheduler; the
+// exponentials alone (16 a clock and SM) are 1,024 for the two tiles, the products 256 at head size 64 and 512 at 128, the
+// conversion 700 and 1,300 beside them.  A page of two tiles takes 2,050 and 2,420 clocks.  Measured: 2,048 tokens, 32 heads of 64,
+// 55 us (310 TFLOP/s); 600 and 600 tokens over 20,011 to 31,001 positions, 32 heads by 8 of 128, 600 us (650 TFLOP/s, 0.40 of what a
+// library's bf16 product reaches).
 //
 // A step of few blocks leaves SMs idle: then a block's pages are cut into parts, each a block of its own that leaves (m, sum, O) per
 // row in a workspace; a second kernel joins them in order.  Waits are bounded (sm100.cuh).

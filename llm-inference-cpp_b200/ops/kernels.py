@@ -2231,7 +2231,10 @@ def _rows8_floats(dtype: int, n_seqs: int, max_q: int, n_heads: int, n_kv_heads:
 
 
 _PROMPT8_PART_PAGES = 4       # the least pages of a part of a block of 256 query rows
-_ROWS8_MOST = 32              # query rows of a kv head that the kernel for few rows has in one tile
+# Query rows of a kv head up to which the kernel for few rows takes a step, its largest tile (rows / prompt kernel, us, at 32 and 48
+# rows: 64 sequences of 200 to 4,000 positions, 32 heads by 8 of 128: 126 / 156 and 176 / 159; one of 30,000: 42 / 46 and 52 / 48;
+# eight of 500 to 3,000, 32 heads of 64: 52 / 66 and 71 / 67).
+_ROWS8_MOST = 32
 
 
 @functools.lru_cache(maxsize=4096)

@@ -18,12 +18,15 @@
 //   softmax       two threads own a row, 32 keys of a page each: tcgen05.ld, mask, maximum, exp2, sum; P = 2^(s + log2 vmax - m) goes
 //                 back to tensor memory as fp16 over the S it has read; the sum of w is that of P / vmax
 //   O += P V'     tcgen05.mma with A in tensor memory, accumulating in fp32; m follows the running maximum (of s + log2 vmax) only
-//                 when that has grown by more than 8, so O is rescaled a few times per row, and only then the two threads exchange theirs
+//                 when that has grown by more than 8, so O is rescaled a few times per row.  At head size 64 tensor memory has room for
+//                 an O of each thread's keys, with their own m and sum: nothing passes between the two before the end.  At 128 the two
+//                 share one O, ask each other on every page whether an m has to follow (a barrier of 64 threads, 7 % of the page at 64),
+//                 and exchange maxima only then.
 //
 // What bounds it: a row's way through the softmax of a page, 1,800 clocks from S to P with four warps on each scheduler; the
 // exponentials alone (16 a clock and SM) are 1,024 for the two tiles, the products 256 at head size 64 and 512 at 128, the
-// conversion 700 and 1,300 beside them.  A page of two tiles takes 2,050 and 2,420 clocks.  Measured: 2,048 tokens, 32 heads of 64,
-// 55 us (310 TFLOP/s); 600 and 600 tokens over 20,011 to 31,001 positions, 32 heads by 8 of 128, 600 us (650 TFLOP/s, 0.40 of what a
+// conversion 700 and 1,300 beside them.  A page of two tiles takes 1,900 and 2,400 clocks.  Measured: 2,048 tokens, 32 heads of 64,
+// 52 us (329 TFLOP/s); 600 and 600 tokens over 20,011 to 31,001 positions, 32 heads by 8 of 128, 595 us (657 TFLOP/s, 0.40 of what a
 // library's bf16 product reaches).
 //
 // A step of few blocks leaves SMs idle: then a block's pages are cut into parts, each a block of its own that leaves (m, sum, O) per
@@ -44,7 +47,7 @@ constexpr int P8_ROWS = 256, P8_TILE = 128;
 constexpr int P8_SOFTMAX = 4, P8_CONVERT = 20, P8_WARPS = 24;
 constexpr int P8_THREADS = P8_WARPS * 32;
 constexpr int P8_JOINS = 16;              // blocks of 8 warps that join a block's rows
-constexpr int P8_TMEM = 512;              // per tile of rows 256 columns: S of even and odd pages (64 each), O (D)
+constexpr int P8_TMEM = 512;              // per tile of rows 256 columns: S of even and odd pages (64 each), O (D, or 64 of each half of the keys)
 constexpr float P8_LAZY = 8.0f;           // the reference maximum follows where it is 2^8 behind
 constexpr uint32_t PG_WIDE = 1u, PG_POISON = 2u;       // the page's scales are far apart; it has values that are no numbers
 constexpr float P8_LIGHT = 8.077935669463161e-28f;     // 2^-90
@@ -75,6 +78,7 @@ struct Prompt8Params {
 template <int D>
 struct P8Cfg {
   static constexpr int SUBS = D / 64;                     // 64-column sub-tiles of a row
+  static constexpr bool OWN = D == 64;                    // each of a row's two threads has a maximum, a sum and an O of its own
   static constexpr int Q_TILE = SUBS * P8_TILE * 128;     // bytes of a tile's queries
   static constexpr int KV_TILE = SUBS * PAGE8 * 128;      // bytes of a page's K' or V'
   static constexpr int STAGE = 2 * KV_TILE, STAGES = 3;
@@ -181,6 +185,7 @@ template <int D, int HELD>
 __global__ void __launch_bounds__(P8_THREADS, 1) attention_prompt8_kernel(Prompt8Params p) {
   using C = P8Cfg<D>;
   constexpr int STAGES = C::STAGES, RAWS = C::RAWS;
+  constexpr bool OWN = C::OWN;
   extern __shared__ uint8_t smem_raw[];
   const uint32_t base = (smem_u32(smem_raw) + 1023u) & ~1023u;
   uint8_t* const base_p = smem_raw + (base - smem_u32(smem_raw));
@@ -347,7 +352,8 @@ __global__ void __launch_bounds__(P8_THREADS, 1) attention_prompt8_kernel(Prompt
       const uint32_t a = tm + 256u * tile + 64u * (j & 1), o = tm + 256u * tile + 128u;
 #pragma unroll
       for (int k = 0; k < 4; ++k)
-        p8_mma_ts(o, a + 32u * (k / 2) + 8u * (k % 2), desc_v + (uint32_t)(st * (C::STAGE >> 4)) + (k * (16 * 128) >> 4), idesc_o, (j > 0 || k > 0) ? 1u : 0u, one);
+        p8_mma_ts(OWN ? o + 64u * (k / 2) : o, a + 32u * (k / 2) + 8u * (k % 2), desc_v + (uint32_t)(st * (C::STAGE >> 4)) + (k * (16 * 128) >> 4), idesc_o,
+                  (j > 0 || (OWN ? k % 2 : k) > 0) ? 1u : 0u, one);
       p8_commit(o_done(tile), one);
     };
     bool ok = __all_sync(0xffffffffu, mbar_wait(q_full, 0, p.error_flag, 102));
@@ -377,7 +383,7 @@ __global__ void __launch_bounds__(P8_THREADS, 1) attention_prompt8_kernel(Prompt
     }
   } else if (warp >= P8_SOFTMAX && warp < P8_CONVERT) {
     // ---- softmax and output: two threads a row, each with 32 keys of every page and half of the row's output ----
-    constexpr int HD = D / 2;
+    constexpr int HD = D / 2, OC = OWN ? D : HD;                   // OC: columns of O that a thread rescales
     const int tile = (warp - P8_SOFTMAX) >> 3, half = ((warp - P8_SOFTMAX) >> 2) & 1, quad = warp & 3;
     const int in_tile = quad * 32 + lane, r = tile * P8_TILE + in_tile;       // the row's TMEM lane, the row of the block
     const int row = d.row0 + r, tok = row / G, head = kvh * G + row % G;
@@ -458,9 +464,9 @@ __global__ void __launch_bounds__(P8_THREADS, 1) attention_prompt8_kernel(Prompt
       row_fac = s_top[tile][0][in_tile];
     }
     const int n = n_tile[tile];
-    const uint32_t t_lane = (uint32_t)(quad * 32) << 16, t_tile = tmem + 256u * tile + t_lane, t_o = t_tile + 128u + (uint32_t)(HD * half);
+    const uint32_t t_lane = (uint32_t)(quad * 32) << 16, t_tile = tmem + 256u * tile + t_lane, t_o = t_tile + 128u + (uint32_t)(OC * half);
     // the reference maximum (of s + log2 vmax, base 2) and 0 less it (0 while there is none); the sum of 2^(s - m_ref) over this half, and
-    // over the other one when they last met
+    // (where the halves share a maximum) over the other one when they last met
     float m_ref = -INFINITY, neg_ref = 0.f, l_run = 0.f, l_other = 0.f;
     bool ok = true;
     int st = 0;                                                    // j % STAGES
@@ -495,17 +501,20 @@ __global__ void __launch_bounds__(P8_THREADS, 1) attention_prompt8_kernel(Prompt
 #pragma unroll
         for (int u = 0; u < 4; ++u) mx4[u] = fmaxf(fmaxf(mx4[u], sc[c + 2 * u]), sc[c + 2 * u + 1]);
       float top = fmaf(fmaxf(fmaxf(mx4[0], mx4[1]), fmaxf(mx4[2], mx4[3])), to_log2, page.y), corr = 1.f;
-      // The common page: nothing has outgrown the reference maximum, and the sum of w is that of P / vmax.  Otherwise both threads of
-      // every row of the two warps go the long way.
+      // The common page: nothing has outgrown the reference maximum, and the sum of w is that of P / vmax.  Otherwise all threads of
+      // the warp, or of the two that share rows and their Os, go the long way.
       const bool light = look != 0u || page.z * P8_LIGHT > l_run + l_other;
       bool by_key = false;
-      if (any_of_pair(top > m_ref + P8_LAZY || light)) {
-        s_top[tile][half][in_tile] = top;
-        s_sum[tile][half][in_tile] = l_run;
-        meet();
-        top = fmaxf(top, s_top[tile][half ^ 1][in_tile]);
-        l_other = s_sum[tile][half ^ 1][in_tile];
-        meet();
+      const bool grown = top > m_ref + P8_LAZY || light;
+      if (OWN ? __any_sync(0xffffffffu, grown) : any_of_pair(grown)) {
+        if (!OWN) {
+          s_top[tile][half][in_tile] = top;
+          s_sum[tile][half][in_tile] = l_run;
+          meet();
+          top = fmaxf(top, s_top[tile][half ^ 1][in_tile]);
+          l_other = s_sum[tile][half ^ 1][in_tile];
+          meet();
+        }
         if (top > m_ref + P8_LAZY) {
           if (m_ref != -INFINITY) {
             corr = fast_exp2(m_ref - top);
@@ -556,7 +565,7 @@ __global__ void __launch_bounds__(P8_THREADS, 1) attention_prompt8_kernel(Prompt
         if (__any_sync(0xffffffffu, corr != 1.f)) {
           asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
 #pragma unroll
-          for (int c = 0; c < HD; c += 16) {
+          for (int c = 0; c < OC; c += 16) {
             float t[16];
             uint32_t u[16];
             p8_ld16(t_o + (uint32_t)c, t);
@@ -576,34 +585,57 @@ __global__ void __launch_bounds__(P8_THREADS, 1) attention_prompt8_kernel(Prompt
     // (`fine` is the same in all lanes: the TMEM loads are the whole warp's)
     const bool fine = __all_sync(0xffffffffu, ok && (n == 0 || mbar_wait(o_done(tile), (n - 1) & 1, p.error_flag, 107)));
     asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+    // the row's maximum and sum, and what its two Os count for (only where each half has its own)
+    s_top[tile][half][in_tile] = m_ref;
     s_sum[tile][half][in_tile] = l_run;
     meet();
-    const float l_all = s_sum[tile][0][in_tile] + s_sum[tile][1][in_tile];
+    const float m2[2] = {s_top[tile][0][in_tile], s_top[tile][1][in_tile]}, l2[2] = {s_sum[tile][0][in_tile], s_sum[tile][1][in_tile]};
+    const float m_all = OWN ? fmaxf(m2[0], m2[1]) : m_ref;
+    const float down0 = !OWN || m2[0] == -INFINITY ? 0.f : m2[0] - m_all, down1 = !OWN || m2[1] == -INFINITY ? 0.f : m2[1] - m_all;
+    const float l_all = OWN ? rescale8(l2[0], down0) + rescale8(l2[1], down1) : l2[0] + l2[1];
+    const float part0 = fast_exp2(down0), part1 = fast_exp2(down1);
+    auto output = [&](int c, float (&o)[16]) {                     // dims HD * half + c .. + 15 (zeros without a page)
+      if (n == 0) {
+#pragma unroll
+        for (int e = 0; e < 16; ++e) o[e] = 0.f;
+        return;
+      }
+      p8_ld16(t_tile + 128u + (uint32_t)(HD * half + c), o);
+      if (OWN) {
+        float other[16];
+        p8_ld16(t_tile + 128u + (uint32_t)(D + HD * half + c), other);
+        p8_ld_wait();
+#pragma unroll
+        for (int e = 0; e < 16; ++e) o[e] = fmaf(other[e], part1, o[e] * part0);
+      } else {
+        p8_ld_wait();
+      }
+    };
     if (fine) {
       if (cut.x > 1) {
         float* slot = p.partials + (((size_t)blk * Hkv + kvh) * p.parts + part) * (P8_ROWS * (D + 2));
-        if (row_ok && half == 0) slot[r] = m_ref, slot[P8_ROWS + r] = l_all;
+        if (row_ok && half == 0) slot[r] = m_all, slot[P8_ROWS + r] = l_all;
         float* dst = slot + 2 * P8_ROWS + (size_t)r * D + HD * half;
 #pragma unroll 1
         for (int c = 0; c < HD; c += 16) {
           float o[16];
-          if (n > 0) p8_ld16(t_o + (uint32_t)c, o), p8_ld_wait();
+          output(c, o);
 #pragma unroll
           for (int e = 0; e < 16; e += 4)
-            if (row_ok) *reinterpret_cast<float4*>(dst + c + e) = n > 0 ? make_float4(o[e], o[e + 1], o[e + 2], o[e + 3]) : make_float4(0.f, 0.f, 0.f, 0.f);
+            if (row_ok) *reinterpret_cast<float4*>(dst + c + e) = make_float4(o[e], o[e + 1], o[e + 2], o[e + 3]);
         }
       } else {
+        // (without a page, or with weights that are all zero, the row sees nothing)
         const float inv = l_all == 0.f ? 0.f : 1.f / l_all;
         __nv_bfloat16* dst = p.out + (size_t)(d.q_start + tok) * p.ldo + (size_t)head * D + HD * half;
 #pragma unroll 1
         for (int c = 0; c < HD; c += 16) {
           float o[16];
-          if (n > 0) p8_ld16(t_o + (uint32_t)c, o), p8_ld_wait();
+          output(c, o);
           uint32_t w[8];
 #pragma unroll
           for (int e = 0; e < 8; ++e) {
-            // (without a page, or with weights that are all zero, the row sees nothing)
-            __nv_bfloat162 h = __floats2bfloat162_rn(n > 0 ? o[2 * e] * inv : 0.f, n > 0 ? o[2 * e + 1] * inv : 0.f);
+            __nv_bfloat162 h = __floats2bfloat162_rn(o[2 * e] * inv, o[2 * e + 1] * inv);
             w[e] = *reinterpret_cast<uint32_t*>(&h);
           }
           if (row_ok) {

@@ -71,7 +71,11 @@ __global__ void __launch_bounds__(ANY8_WARPS * 32) attention_any8_kernel(Any8Par
   for (long c0 = (long)(lo / ROUND) * ROUND + warp * 32; c0 <= pos; c0 += ROUND) {
     if (c0 + 31 < lo) continue;
     const int page = page8_of(p.kv, seq, (int)c0);
-    if (page < 0) continue;
+    if (page < 0) {
+      l = __int_as_float(0x7fffffff);
+      if (c0 / PAGE8 >= p.kv.table_pages) break;
+      continue;
+    }
     const size_t row0 = ((size_t)page * p.kv.n_kv_heads + kvh) * PAGE8 + c0 % PAGE8;
     const bool valid = c0 + lane >= lo && c0 + lane <= pos;
     float score = -INFINITY, vs = 0.f;
@@ -134,7 +138,7 @@ __global__ void __launch_bounds__(ANY8_WARPS * 32) attention_any8_kernel(Any8Par
     float x = 0.f;
 #pragma unroll
     for (int w = 0; w < ANY8_WARPS; ++w) x = fmaf(s_acc[w][d], expf(s_m[w] - top), x);
-    o[d] = from_f32<T>(sum == 0.f ? 0.f : x / sum);      // (0: no page of the sequence is one of the pool)
+    o[d] = from_f32<T>(sum == 0.f ? 0.f : x / sum);
   }
 }
 

@@ -118,8 +118,8 @@ __device__ __forceinline__ P8Block prompt8_block(const Prompt8Params& p, int b) 
       d.first = d.pos0 + d.row0 / p.group;
       d.last = d.pos0 + (d.row0 + d.rows - 1) / p.group;
       d.lo = (p.window > 0 && d.first - p.window + 1 > 0) ? d.first - p.window + 1 : 0;
-      d.pg_first = d.lo / PAGE8;
-      if (d.last >= 0) d.n_pages = d.last / PAGE8 - d.pg_first + 1;
+      d.pg_first = page_index8(p.kv, d.lo);
+      if (d.last >= 0) d.n_pages = page_index8(p.kv, d.last) - d.pg_first + 1;
       return d;
     }
     b -= all;

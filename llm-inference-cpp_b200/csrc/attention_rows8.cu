@@ -114,8 +114,8 @@ __device__ __forceinline__ Rw8Entry rw8_entry(const Rows8Params& p, int e, int t
   const int first = d.pos0 + d.row0 / p.group;
   d.last = d.pos0 + (d.row0 + d.rows - 1) / p.group;
   d.lo = (p.window > 0 && first - p.window + 1 > 0) ? first - p.window + 1 : 0;
-  d.pg_first = d.lo / PAGE8;
-  if (d.last >= 0) d.n_pages = d.last / PAGE8 - d.pg_first + 1;
+  d.pg_first = page_index8(p.kv, d.lo);
+  if (d.last >= 0) d.n_pages = page_index8(p.kv, d.last) - d.pg_first + 1;
   return d;
 }
 
@@ -749,7 +749,7 @@ template <int D, int NT, int HELD, typename T> int launch_rows8(const Rows8Param
   // no more blocks than are resident: many entries' table may leave room for one a SM only (228 KB; a block's own 1 KB and its statics)
   const int fit = (int)((228 << 10) / (smem + 1280));
   grid = min(grid, min(C::BLOCKS, max(1, fit)) * sm_count());
-  const Rw8Cut cut = {8, 1024 / D, 512 / D, 256 / D};
+  const Rw8Cut cut = {8, 1024 / D + 1, 512 / D, 256 / D};
   const int rc = launch_pdl(PDL_ATTENTION, kernel, (unsigned)grid, RW8_WARPS * 32, smem, stream, p, n_entries, cut);
   // (short (entry, kv head)s that have a block each leave no parts)
   if (rc != LLMI_OK || ((long)n_entries * p.kv.n_kv_heads <= grid && most_pages <= cut.most_whole)) return rc;
@@ -800,7 +800,8 @@ LLMI_EXPORT int llmi_attention_rows8(int dtype, int held, const void* q, long ld
   const int n_entries = n_seqs * tiles, grid = rw8_grid((long)n_entries * n_kv_heads * table_pages);
   p.whose = reinterpret_cast<int*>(slots + 2L * grid * (head_dim / 16 * nt * 128 + 16 * nt));
   // most pages that a (sequence, kv head)'s rows of a tile see
-  const int most_pages = window > 0 && (window + max_q) / PAGE8 + 2 < table_pages ? (window + max_q) / PAGE8 + 2 : table_pages;
+  const long seen = ((long)window + max_q) / PAGE8 + 2;
+  const int most_pages = window > 0 && seen <= table_pages ? (int)seen : table_pages + 1;      // (+ 1: page_index8)
 #define LLMI_ROWS8(D_, NT_, T_) \
   (held == HELD_INT8 ? launch_rows8<D_, NT_, HELD_INT8, T_>(p, n_entries, grid, most_pages, stream) : launch_rows8<D_, NT_, HELD_E4M3, T_>(p, n_entries, grid, most_pages, stream))
   if (dtype == LLMI_DTYPE_F32) return head_dim == 128 ? LLMI_ROWS8(128, 1, float) : nt == 1 ? LLMI_ROWS8(64, 1, float) : LLMI_ROWS8(64, 2, float);

@@ -32,13 +32,18 @@ struct Paged8 {
   int head_dim;
 };
 
-// The page of position `pos`, or -1 where the table or the pool has none such (a caller's mistake: nothing is read or written there).
+// The page of position `pos`, or -1 where the table or the pool has none such (a caller's mistake: nothing is read or written there, and
+// queries that see it are NaN).
 __device__ __forceinline__ int page8_of(const Paged8& c, int seq, int pos) {
   const int i = pos / PAGE8;
   if (i >= c.table_pages) return -1;
   const int page = c.seq_pages[(size_t)seq * c.pages_stride + i];
   return (unsigned)page < (unsigned)c.n_pages ? page : -1;
 }
+
+// The page index of the sequence's position `pos` >= 0, no further than one behind the table's last: a sequence longer than its table
+// (a caller's mistake, too) costs no time, and its first page without a place reads as NaN as an unknown one does.
+__device__ __forceinline__ int page_index8(const Paged8& c, int pos) { return min(pos / PAGE8, c.table_pages); }
 
 struct Scale8 {
   float scale, inv;

@@ -265,6 +265,88 @@ def test_a_kernel_named(kernel, H, G, D, step, window):
     check(b, H, q, out, "bfloat16", window)
 
 
+def attend_by(kernel, b, H, q, window=0, scale=None, table=None):
+    out = torch.full((b.T, H * b.D), 7.0, dtype=torch.bfloat16, device="cuda")
+    K().attention8(q, out, b.k, b.v, b.ctx, b.table if table is None else table, H, b.G, b.D, b.D ** -0.5 if scale is None else scale, window, kernel=kernel)
+    K().check_device_errors("cuda:0")
+    return out
+
+
+@pytest.mark.parametrize("kernel", ["rows", "prompt", "any"])
+@pytest.mark.parametrize("wrong", ["a table too short", "no page", "a page past the pool"])
+def test_pages_that_are_not_there_reach_only_who_sees_them(kernel, wrong):
+    """A sequence's rows that see such a page are NaN; nothing is read, and its neighbours and its own earlier rows stay as they are."""
+    b = Batch([(3, 40), (70, 150), (1, 64)], 2, 64, "int8")
+    b.fill()
+    q = torch.tensor(b.rng.normal(size=(b.T, 4 * 64))).to(torch.bfloat16).cuda()
+    want = attend_by(kernel, b, 4, q)
+    table = b.table.clone()
+    if wrong == "a table too short":
+        table = table[:, :2].contiguous()
+    else:
+        table[1, 2] = -1 if wrong == "no page" else b.n_pool
+    got = attend_by(kernel, b, 4, q, table=table)
+    sees = torch.tensor((b.seq == 1) & (b.pos >= 128)).cuda()
+    assert bool(got[sees].isnan().all()) and int(sees.sum()) == 22
+    rest = got[~sees].double() - want[~sees].double()
+    # (the other rows' sums may be cut otherwise: two roundings of the output)
+    assert bool((rest.abs() <= 2.0 ** -7 * want[~sees].double().abs() + 2.0 ** -9).all())
+
+
+@pytest.mark.parametrize("kernel", ["rows", "prompt", "any"])
+def test_sequences_far_longer_than_their_table_end(kernel):
+    """Lengths that no table holds: as many pages are walked as the table has."""
+    b = Batch([(3, 100), (2, 60)], 2, 64, "int8")
+    b.fill()
+    q = torch.tensor(b.rng.normal(size=(b.T, 4 * 64))).to(torch.bfloat16).cuda()
+    want = attend_by(kernel, b, 4, q)
+    b.ctx.seq_kv_len = torch.tensor([2 ** 31 - 64, 60], dtype=torch.int32, device="cuda")
+    b.ctx.tok_pos = torch.tensor([2 ** 31 - 67, 2 ** 31 - 66, 2 ** 31 - 65, 58, 59], dtype=torch.int32, device="cuda")
+    got = attend_by(kernel, b, 4, q)
+    assert bool(got[:3].isnan().all())
+    assert bool(((got[3:].double() - want[3:].double()).abs() <= 2.0 ** -7 * want[3:].double().abs() + 2.0 ** -9).all())
+
+
+@pytest.mark.parametrize("kernel", ["rows", "prompt", "any"])
+@pytest.mark.parametrize("scale,window", [(0.0, 0), (-0.2, 0), (1e-30, 0), (0.125, 2 ** 31 - 1), (3.0, 2 ** 31 - 1)])
+@pytest.mark.parametrize("step", ["one token", "single tokens", "messages"])
+def test_scales_and_windows_at_their_ends(kernel, scale, window, step):
+    b = Batch(STEPS[step], 2, 64, "int8")
+    b.fill()
+    q = torch.tensor(b.rng.normal(size=(b.T, 4 * 64))).to(torch.bfloat16).cuda()
+    check(b, 4, q, attend_by(kernel, b, 4, q, window, scale), "bfloat16", 0, scale)
+
+
+@pytest.mark.parametrize("held", ["int8", "float8_e4m3"])
+def test_offsets_past_32_bits(held):
+    """A pool of more than 2^32 codes: its last pages give the bits that its first ones give, append and attention."""
+    k = K()
+    G, D, H = 8, 128, 16
+    n_pool = 2 ** 32 // (G * 64 * D) + 40
+    near, far = Batch([(3, 130), (1, 200), (40, 90)], G, D, held), Batch([(3, 130), (1, 200), (40, 90)], G, D, held)
+    far.k, far.v = (k.Rows8(torch.empty((n_pool, G, 64, D), dtype=HELD[held], device="cuda"),
+                            torch.empty((n_pool, G, 64), dtype=torch.float32, device="cuda")) for _ in range(2))
+    near.fill()
+    there = torch.tensor(sorted(set(near.table_np[near.table_np >= 0].tolist()))).cuda()
+    for a, z in ((near.k, far.k), (near.v, far.v)):
+        z.codes.view(torch.uint8)[there + n_pool - near.n_pool] = a.codes.view(torch.uint8)[there]
+        z.scales[there + n_pool - near.n_pool] = a.scales[there]
+    far.table = torch.where(near.table >= 0, near.table + (n_pool - near.n_pool), near.table).to(torch.int32)
+    assert int(far.table.max()) * G * 64 * D > 2 ** 32
+    rows = torch.tensor(near.rng.normal(size=(near.T, (H + 2 * G) * D))).to(torch.bfloat16).cuda()
+    inv = (10000.0 ** (-torch.arange(0, D, 2, dtype=torch.float64) / D)).float().cuda()
+    for kernel in ("rows", "prompt", "any"):
+        outs = []
+        for b in (near, far):
+            out = torch.zeros(b.T, H * D, dtype=torch.bfloat16, device="cuda")
+            k.attention8(rows, out, b.k, b.v, b.ctx, b.table, H, G, D, D ** -0.5, rope=(inv, D, True), kernel=kernel)
+            outs.append(out)
+        k.check_device_errors("cuda:0")
+        assert torch.equal(outs[0], outs[1]) and not bool(outs[0].isnan().any())
+    assert torch.equal(far.k.codes.view(torch.uint8)[there + n_pool - near.n_pool], near.k.codes.view(torch.uint8)[there])
+    assert torch.equal(far.v.scales[there + n_pool - near.n_pool].nan_to_num(-1.0), near.v.scales[there].nan_to_num(-1.0))
+
+
 @pytest.mark.parametrize("kernel,D,dtype", [("rows", 40, "bfloat16"), ("prompt", 32, "bfloat16"), ("prompt", 64, "float32"), ("columns", 64, "bfloat16")])
 def test_a_kernel_named_that_does_not_take_the_call(kernel, D, dtype):
     b = Batch([(3, 10)], 2, D, "int8")

@@ -26,7 +26,7 @@
 // What bounds it: a row's way through the softmax of a page, 1,800 clocks from S to P with four warps on each scheduler; the
 // exponentials alone (16 a clock and SM) are 1,024 for the two tiles, the products 256 at head size 64 and 512 at 128, the
 // conversion 700 and 1,300 beside them.  A page of two tiles takes 1,900 and 2,400 clocks.  Measured: 2,048 tokens, 32 heads of 64,
-// 52 us (329 TFLOP/s); 600 and 600 tokens over 20,011 to 31,001 positions, 32 heads by 8 of 128, 595 us (657 TFLOP/s, 0.40 of what a
+// 52 us (329 TFLOP/s); 600 and 600 tokens over 20,011 to 31,001 positions, 32 heads by 8 of 128, 593 us (659 TFLOP/s, 0.40 of what a
 // library's bf16 product reaches).
 //
 // A step of few blocks leaves SMs idle: then a block's pages are cut into parts, each a block of its own that leaves (m, sum, O) per
@@ -46,7 +46,7 @@ constexpr int P8_ROWS = 256, P8_TILE = 128;
 // 20 .. 23 codes to fp16.
 constexpr int P8_SOFTMAX = 4, P8_CONVERT = 20, P8_WARPS = 24;
 constexpr int P8_THREADS = P8_WARPS * 32;
-constexpr int P8_JOINS = 16;              // blocks of 8 warps that join a block's rows
+constexpr int P8_JOINS = 32;              // blocks of 8 warps that join a block's rows
 constexpr int P8_TMEM = 512;              // per tile of rows 256 columns: S of even and odd pages (64 each), O (D, or 64 of each half of the keys)
 constexpr float P8_LAZY = 8.0f;           // the reference maximum follows where it is 2^8 behind
 constexpr uint32_t PG_WIDE = 1u, PG_POISON = 2u;       // the page's scales are far apart; it has values that are no numbers
@@ -738,27 +738,42 @@ __global__ void __launch_bounds__(256) prompt8_join_kernel(Prompt8Params p) {
   pdl_wait();
   pdl_launch_dependents();
   if (d.rows <= 0 || d.n_pages <= 0 || cut.x <= 1) return;
+  constexpr int AT_ONCE = 4;               // parts whose sums are under way
+  const size_t step = P8_ROWS * (D + 2);
   for (int r = (blockIdx.y % P8_JOINS) * 8 + (threadIdx.x >> 5); r < d.rows; r += 8 * P8_JOINS) {
-    const float* slot = p.partials + ((size_t)blk * p.kv.n_kv_heads + kvh) * p.parts * (P8_ROWS * (D + 2));
-    const size_t step = P8_ROWS * (D + 2);
-    float m = -INFINITY, l = 0.f, o[D / 32];
-    for (int z = lane; z < cut.x; z += 32) m = fmaxf(m, slot[z * step + r]);
-    m = warp_max(m);
+    const float* slot = p.partials + ((size_t)blk * p.kv.n_kv_heads + kvh) * p.parts * step;
+    float ms = -INFINITY, ls = 0.f;                                // of part `lane` (there are 32 at most)
+    if (lane < cut.x) ms = slot[lane * step + r], ls = slot[lane * step + P8_ROWS + r];
+    float2 x[AT_ONCE][D / 64], o[D / 64];
+    auto ask = [&](int z0) {
 #pragma unroll
-    for (int i = 0; i < D / 32; ++i) o[i] = 0.f;
-#pragma unroll 4
-    for (int z = 0; z < cut.x; ++z) {
-      const float mz = slot[z * step + r], f = mz == -INFINITY ? 1.f : fast_exp2(mz - m);
-      l += rescale8(slot[z * step + P8_ROWS + r], mz == -INFINITY ? 0.f : mz - m);
-      const float* src = slot + z * step + 2 * P8_ROWS + (size_t)r * D + lane * (D / 32);
+      for (int i = 0; i < AT_ONCE; ++i) {
+        const float2* src = reinterpret_cast<const float2*>(slot + min(z0 + i, cut.x - 1) * step + 2 * P8_ROWS + (size_t)r * D);
 #pragma unroll
-      for (int i = 0; i < D / 32; ++i) o[i] = fmaf(src[i], f, o[i]);
+        for (int c = 0; c < D / 64; ++c) x[i][c] = src[lane + 32 * c];
+      }
+    };
+    ask(0);
+    const float m = warp_max(ms), down = ms == -INFINITY ? 0.f : ms - m, f = ms == -INFINITY ? 1.f : fast_exp2(ms - m);
+    const float l = warp_sum(rescale8(ls, down));
+#pragma unroll
+    for (int c = 0; c < D / 64; ++c) o[c] = make_float2(0.f, 0.f);
+    for (int z0 = 0; z0 < cut.x; z0 += AT_ONCE) {
+      if (z0 > 0) ask(z0);
+#pragma unroll
+      for (int i = 0; i < AT_ONCE; ++i) {
+        const float fz = __shfl_sync(0xffffffffu, f, min(z0 + i, 31));
+        if (z0 + i < cut.x) {
+#pragma unroll
+          for (int c = 0; c < D / 64; ++c) o[c].x = fmaf(x[i][c].x, fz, o[c].x), o[c].y = fmaf(x[i][c].y, fz, o[c].y);
+        }
+      }
     }
     const int row = d.row0 + r;
     const float inv = l == 0.f ? 0.f : 1.f / l;
-    __nv_bfloat162* dst = reinterpret_cast<__nv_bfloat162*>(p.out + (size_t)(d.q_start + row / G) * p.ldo + (size_t)(kvh * G + row % G) * D + lane * (D / 32));
+    __nv_bfloat162* dst = reinterpret_cast<__nv_bfloat162*>(p.out + (size_t)(d.q_start + row / G) * p.ldo + (size_t)(kvh * G + row % G) * D);
 #pragma unroll
-    for (int i = 0; i < D / 32; i += 2) dst[i / 2] = __floats2bfloat162_rn(o[i] * inv, o[i + 1] * inv);
+    for (int c = 0; c < D / 64; ++c) dst[lane + 32 * c] = __floats2bfloat162_rn(o[c].x * inv, o[c].y * inv);
   }
 }
 
@@ -790,7 +805,7 @@ LLMI_EXPORT int llmi_attention_prompt8(int held, const void* q, long ldq, void* 
   if (n_seqs <= 0 || n_blocks <= 0 || n_kv_heads <= 0 || n_heads <= 0 || n_heads % n_kv_heads || (head_dim != 64 && head_dim != 128) ||
       table_pages <= 0 || n_pages <= 0 || window < 0 || parts <= 0 || part_pages <= 0)
     return LLMI_ERR_BAD_SIZE;
-  if ((long)n_blocks * parts > 65535 || n_blocks > 8191) return LLMI_ERR_BAD_SIZE;
+  if ((long)n_blocks * parts > 65535 || parts > 32 || (parts > 1 && n_blocks * P8_JOINS > 65535)) return LLMI_ERR_BAD_SIZE;
   if (parts > 1 && (!partials || n_floats < (long)n_blocks * n_kv_heads * parts * P8_ROWS * (head_dim + 2))) return LLMI_ERR_BAD_SIZE;
   if (held != HELD_INT8 && held != HELD_E4M3) return LLMI_ERR_BAD_DTYPE;
   if ((((uintptr_t)q | (uintptr_t)out | (uintptr_t)k_codes | (uintptr_t)v_codes | (uintptr_t)k_scales | (uintptr_t)v_scales | (uintptr_t)partials) & 15) ||

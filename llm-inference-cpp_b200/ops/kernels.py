@@ -2246,9 +2246,9 @@ def prompt8_parts(n_rows: int, n_kv_heads: int, head_dim: int, n_seqs: int, tabl
     Counted in pages' time (1.1 us): a block's start and end are 7, the join of parts 4 and 0.045 for each part of 256 x 128 sums.
     One sequence's parts are equal and go in whole waves; those of several fill the gaps that shorter ones leave (a sequence is
     taken to be 0.6 + 0.4 / n_seqs of the longest, its last block half full).  Measured, us in 1 / 2 / 4 / 8 parts, with the choice
-    marked: 100 tokens over 4,000 positions, 32 heads by 8 of 128: 96 / 62 / 43 / 39*; 256 over 8,192, 32 heads of 64: 164 / 94 /
-    57* / 68; four messages of 45 over 500 to 2,000: 47 / 36 / 30* / 32; eight of 60 over 1,000 to 3,000, 32 heads: 77* / 91 / 110 /
-    141."""
+    marked: 100 tokens over 4,000 positions, 32 heads by 8 of 128: 96 / 61 / 42 / 32*; 256 over 8,192, 32 heads of 64: 153 / 87 /
+    52* / 61; four messages of 45 over 500 to 2,000: 47 / 37 / 28* / 28; eight of 60 over 1,000 to 3,000, 32 heads: 70* / 94 / 113 /
+    145."""
     blocks = -(-n_rows // 256) if n_seqs == 1 else n_rows / 256 + (n_seqs - 1) / 2
     jobs = blocks * n_kv_heads
     if jobs >= 3 * sms or (jobs >= sms and 2 * max_q >= 64 * table_pages):
@@ -2305,7 +2305,8 @@ def attention8(q: torch.Tensor, out: torch.Tensor, k: Rows8, v: Rows8, ctx, seq_
             and ldq % (4 if q_f32 else 8) == 0 and ldo % (8 if dtype == 1 else 4) == 0)
     max_q = 1 if ctx.decode else _most_new(ctx)
     n_blocks = (T * group + 255 * S) // 256
-    if kernel in (None, "prompt") and fast and dtype == 1 and n_blocks <= 4095 and (max_q * group > _ROWS8_MOST or kernel):
+    floats = _rows8_floats(dtype, S, max_q, n_heads, n_kv_heads, head_dim, P) if kernel in (None, "rows") and fast else -1
+    if kernel in (None, "prompt") and fast and dtype == 1 and n_blocks <= 65535 and (floats < 0 or max_q * group > _ROWS8_MOST):
         parts = prompt8_parts(T * group, n_kv_heads, head_dim, S, P, max_q, sm_count())
         partials = None
         if parts > 1:
@@ -2315,7 +2316,6 @@ def attention8(q: torch.Tensor, out: torch.Tensor, k: Rows8, v: Rows8, ctx, seq_
             *rows, start, kv_len, *table, n_blocks, n_heads, n_kv_heads, head_dim, scale, window, q_f32, parts, _PROMPT8_PART_PAGES,
             partials.data_ptr() if parts > 1 else None, partials.numel() if parts > 1 else 0, tc_scratch(q.device).error.data_ptr(), stream))
         return
-    floats = _rows8_floats(dtype, S, max_q, n_heads, n_kv_heads, head_dim, P) if kernel in (None, "rows") and fast else -1
     if floats >= 0:
         slots = rt.scratch("attn8_slots", (floats,), torch.float32) if rt is not None else torch.empty(floats, dtype=torch.float32, device=q.device)
         _check("attention_rows8", lib().llmi_attention_rows8(

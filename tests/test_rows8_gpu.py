@@ -317,6 +317,15 @@ def test_scales_and_windows_at_their_ends(kernel, scale, window, step):
     check(b, 4, q, attend_by(kernel, b, 4, q, window, scale), "bfloat16", 0, scale)
 
 
+def test_more_sequences_than_the_kernel_for_few_rows_takes():
+    b = Batch([(1, 1 + i % 5) for i in range(4200)], 1, 64, "int8")
+    b.fill()
+    q = torch.tensor(b.rng.normal(size=(b.T, 2 * 64))).to(torch.bfloat16).cuda()
+    check(b, 2, q, attend(b, 2, q, "bfloat16"), "bfloat16")
+    with pytest.raises(K().KernelError, match="rows"):
+        attend_by("rows", b, 2, q)
+
+
 @pytest.mark.parametrize("held", ["int8", "float8_e4m3"])
 def test_offsets_past_32_bits(held):
     """A pool of more than 2^32 codes: its last pages give the bits that its first ones give, append and attention."""

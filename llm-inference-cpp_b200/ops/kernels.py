@@ -2189,18 +2189,22 @@ def rope_store8(qkv: torch.Tensor, q_out: torch.Tensor, inv_freq: torch.Tensor |
     The rotated q goes to ``q_out`` [T, n_heads * head_dim], of qkv's type or fp32 (rows may be strided; ``qkv[:, :n_heads *
     head_dim]`` rotates in place).  ``tok_seq`` -1 marks a token of no sequence: nothing of it is written.  Two tokens of a call must not have the same
     place.  ``write_kv`` False: q only.  How a row is held: ``csrc/rows8.cuh``."""
-    held = _check8("rope_store8", qkv, k, v, seq_pages, n_heads, n_kv_heads, head_dim)
-    _rope_store8(held, qkv, q_out, inv_freq, rotary_dim, tok_seq, tok_pos, seq_pages, k, v, n_heads, n_kv_heads, head_dim, write_kv)
+    name = "rope_store8"
+    held = _check8(name, qkv, k, v, seq_pages, n_heads, n_kv_heads, head_dim)
+    if q_out.dim() != 2 or q_out.shape[0] != qkv.shape[0] or q_out.shape[1] != n_heads * head_dim or q_out.get_device() != qkv.get_device() \
+            or (q_out.dtype != qkv.dtype and q_out.dtype != torch.float32) or (q_out.stride(1) != 1 and q_out.shape[1] > 1):
+        raise KernelError(f"{name}: q_out must be [tokens, n_heads * head_dim] of qkv's type or fp32")
+    _rope_store8(held, qkv, q_out.data_ptr(), q_out.stride(0), q_out.dtype == torch.float32, inv_freq, rotary_dim, tok_seq, tok_pos, seq_pages, k, v,
+                 n_heads, n_kv_heads, head_dim, write_kv)
 
 
-def _rope_store8(held: int, qkv, q_out, inv_freq, rotary_dim, tok_seq, tok_pos, seq_pages, k, v, n_heads, n_kv_heads, head_dim, write_kv) -> None:
+def _rope_store8(held: int, qkv, q_out: int, ldq: int, q_f32: bool, inv_freq, rotary_dim, tok_seq, tok_pos, seq_pages, k, v, n_heads, n_kv_heads,
+                 head_dim, write_kv) -> None:
+    """``rope_store8`` of checked caches, the rotated q to rows of ``ldq`` numbers from the address ``q_out`` on."""
     name = "rope_store8"
     device, T = qkv.get_device(), qkv.shape[0]
     if qkv.dim() != 2 or qkv.shape[1] != (n_heads + 2 * n_kv_heads) * head_dim or (qkv.stride(1) != 1 and qkv.shape[1] > 1):
         raise KernelError(f"{name}: qkv must be [tokens, (n_heads + 2 n_kv_heads) * head_dim]")
-    if q_out.dim() != 2 or q_out.shape[0] != T or q_out.shape[1] != n_heads * head_dim or q_out.get_device() != device \
-            or (q_out.dtype != qkv.dtype and q_out.dtype != torch.float32) or (q_out.stride(1) != 1 and q_out.shape[1] > 1):
-        raise KernelError(f"{name}: q_out must be [tokens, n_heads * head_dim] of qkv's type or fp32")
     if rotary_dim < 0 or rotary_dim % 2 != 0 or rotary_dim > head_dim:
         raise KernelError(f"{name}: rotary_dim must be even and at most head_dim")
     if rotary_dim and (inv_freq is None or inv_freq.get_device() != device or inv_freq.dtype != torch.float32 or inv_freq.numel() < rotary_dim // 2
@@ -2211,9 +2215,9 @@ def _rope_store8(held: int, qkv, q_out, inv_freq, rotary_dim, tok_seq, tok_pos, 
     if T == 0 or S == 0 or P == 0:
         return
     _check(name, lib().llmi_rope_store8(
-        _DTYPE8[qkv.dtype], held, qkv.data_ptr(), qkv.stride(0), q_out.data_ptr(), q_out.stride(0), inv_freq.data_ptr() if rotary_dim else None, rotary_dim,
+        _DTYPE8[qkv.dtype], held, qkv.data_ptr(), qkv.stride(0), q_out, ldq, inv_freq.data_ptr() if rotary_dim else None, rotary_dim,
         seq, pos, seq_pages.data_ptr(), seq_pages.stride(0), P, S, k.codes.data_ptr(), k.scales.data_ptr(), v.codes.data_ptr(), v.scales.data_ptr(),
-        k.codes.shape[0], T, n_heads, n_kv_heads, head_dim, 1 if write_kv else 0, 1 if q_out.dtype == torch.float32 else 0, _stream8(device)))
+        k.codes.shape[0], T, n_heads, n_kv_heads, head_dim, 1 if write_kv else 0, 1 if q_f32 else 0, _stream8(device)))
 
 
 _sizes8: dict = {}
@@ -2290,41 +2294,44 @@ def attention8(q: torch.Tensor, out: torch.Tensor, k: Rows8, v: Rows8, ctx, seq_
     kv_len = _index8(name, "seq_kv_len", ctx.seq_kv_len, S, device)
     if T == 0 or S == 0 or P == 0:
         return
-    if rope is not None:
-        inv_freq, rotary_dim, write_kv = rope
-        rotated = rt.scratch("attn_q8", (T, width), torch.float32) if rt is not None else torch.empty((T, width), dtype=torch.float32, device=q.device)
-        _rope_store8(held, q, rotated, inv_freq, rotary_dim, ctx.tok_seq, ctx.tok_pos, seq_pages, k, v, n_heads, n_kv_heads, head_dim, write_kv)
-        q = rotated
-    dtype, ldq, ldo, group = _DTYPE8[out.dtype], q.stride(0), out.stride(0), n_heads // n_kv_heads
-    q_f32 = 1 if q.dtype == torch.float32 else 0
-    rows = (held, q.data_ptr(), ldq, out.data_ptr(), ldo, k.codes.data_ptr(), k.scales.data_ptr(), v.codes.data_ptr(), v.scales.data_ptr())
-    table = (seq_pages.data_ptr(), seq_pages.stride(0), P, S, k.codes.shape[0])
-    stream = _stream8(device)
-    # (rows in whole 16-byte pieces: 8 bf16 or 4 fp32 numbers)
-    fast = (head_dim in (64, 128) and (rows[1] | rows[3] | rows[5] | rows[6] | rows[7] | rows[8]) % 16 == 0
+    dtype, ldo, group = _DTYPE8[out.dtype], out.stride(0), n_heads // n_kv_heads
+    # (rotated queries lie in scratch, as fp32)
+    q_f32 = 1 if rope is not None or dtype == 0 else 0
+    ldq, n_q = (width, (T * width + 3) // 4 * 4) if rope is not None else (q.stride(0), 0)
+    addresses = (k.codes.data_ptr(), k.scales.data_ptr(), v.codes.data_ptr(), v.scales.data_ptr())
+    at_q, at_out = 0 if rope is not None else q.data_ptr(), out.data_ptr()
+    # rows in whole 16-byte pieces: 8 bf16 or 4 fp32 numbers
+    fast = (head_dim in (64, 128) and (at_q | at_out | addresses[0] | addresses[1] | addresses[2] | addresses[3]) % 16 == 0
             and ldq % (4 if q_f32 else 8) == 0 and ldo % (8 if dtype == 1 else 4) == 0)
     max_q = 1 if ctx.decode else _most_new(ctx)
     n_blocks = (T * group + 255 * S) // 256
-    floats = _rows8_floats(dtype, S, max_q, n_heads, n_kv_heads, head_dim, P) if kernel in (None, "rows") and fast else -1
-    if kernel in (None, "prompt") and fast and dtype == 1 and n_blocks <= 65535 and (floats < 0 or max_q * group > _ROWS8_MOST):
-        parts = prompt8_parts(T * group, n_kv_heads, head_dim, S, P, max_q, sm_count())
-        partials = None
-        if parts > 1:
-            n = n_blocks * n_kv_heads * parts * 256 * (head_dim + 2)
-            partials = rt.scratch("attn8_parts", (n,), torch.float32) if rt is not None else torch.empty(n, dtype=torch.float32, device=q.device)
+    few = _rows8_floats(dtype, S, max_q, n_heads, n_kv_heads, head_dim, P) if kernel in (None, "rows") and fast else -1
+    prompt = kernel in (None, "prompt") and fast and dtype == 1 and n_blocks <= 65535 and (few < 0 or max_q * group > _ROWS8_MOST)
+    if not prompt and few < 0 and kernel not in (None, "any"):
+        raise KernelError(f"{name}: the kernel {kernel!r} does not take this call")
+    parts = prompt8_parts(T * group, n_kv_heads, head_dim, S, P, max_q, sm_count()) if prompt else 1
+    floats = (n_blocks * n_kv_heads * parts * 256 * (head_dim + 2) if parts > 1 else 0) if prompt else max(few, 0)
+    scratch = None
+    if n_q + floats:
+        scratch = rt.scratch("attn8", (n_q + floats,), torch.float32) if rt is not None else q.new_empty(n_q + floats, dtype=torch.float32)
+    at_scratch = scratch.data_ptr() if scratch is not None else 0
+    if rope is not None:
+        inv_freq, rotary_dim, write_kv = rope
+        at_q = at_scratch
+        _rope_store8(held, q, at_q, ldq, True, inv_freq, rotary_dim, ctx.tok_seq, ctx.tok_pos, seq_pages, k, v, n_heads, n_kv_heads, head_dim, write_kv)
+    rows = (held, at_q, ldq, at_out, ldo, *addresses)
+    table = (seq_pages.data_ptr(), seq_pages.stride(0), P, S, k.codes.shape[0])
+    stream = _stream8(device)
+    if prompt:
         _check("attention_prompt8", lib().llmi_attention_prompt8(
             *rows, start, kv_len, *table, n_blocks, n_heads, n_kv_heads, head_dim, scale, window, q_f32, parts, _PROMPT8_PART_PAGES,
-            partials.data_ptr() if parts > 1 else None, partials.numel() if parts > 1 else 0, tc_scratch(q.device).error.data_ptr(), stream))
-        return
-    if floats >= 0:
-        slots = rt.scratch("attn8_slots", (floats,), torch.float32) if rt is not None else torch.empty(floats, dtype=torch.float32, device=q.device)
+            at_scratch + 4 * n_q if parts > 1 else None, floats, tc_scratch(q.device).error.data_ptr(), stream))
+    elif few >= 0:
         _check("attention_rows8", lib().llmi_attention_rows8(
-            dtype, *rows, start, kv_len, *table, max_q, n_heads, n_kv_heads, head_dim, scale, window, q_f32, slots.data_ptr(), floats, stream))
-        return
-    if kernel not in (None, "any"):
-        raise KernelError(f"{name}: the kernel {kernel!r} does not take this call")
-    seq, pos = _index8(name, "tok_seq", ctx.tok_seq, T, device), _index8(name, "tok_pos", ctx.tok_pos, T, device)
-    _check("attention_any8", lib().llmi_attention_any8(dtype, *rows, seq, pos, *table, T, n_heads, n_kv_heads, head_dim, scale, window, q_f32, stream))
+            dtype, *rows, start, kv_len, *table, max_q, n_heads, n_kv_heads, head_dim, scale, window, q_f32, at_scratch + 4 * n_q, floats, stream))
+    else:
+        seq, pos = _index8(name, "tok_seq", ctx.tok_seq, T, device), _index8(name, "tok_pos", ctx.tok_pos, T, device)
+        _check("attention_any8", lib().llmi_attention_any8(dtype, *rows, seq, pos, *table, T, n_heads, n_kv_heads, head_dim, scale, window, q_f32, stream))
 
 
 def _most_new(ctx) -> int:

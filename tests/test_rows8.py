@@ -96,3 +96,23 @@ def test_plain_rows(kind):
     assert np.abs(codes).max() == R.MOST[kind] and (codes[1:4] == 0).all() and scale[1] == scale[2] == 0 and np.isnan(scale[3])
     fine = [0, 4, 5, 6]
     assert (np.abs(codes[fine] * scale[fine, None] - x[fine]) <= R.half_step(codes[fine], scale[fine], kind) * (1 + 1e-9)).all()
+
+
+def test_parts_of_a_prompt_block_stay_within_the_launch():
+    """However a step is made up: at least one part, none of fewer than four pages, and no more blocks than a grid has."""
+    from llmi_b200.ops.kernels import prompt8_parts
+    rng = np.random.default_rng(5)
+    cut = 0
+    for _ in range(4000):
+        S, G, D = int(2 ** rng.uniform(0, 13)), int(rng.integers(1, 65)), int(rng.choice([64, 128]))
+        rows = S + int(2 ** rng.uniform(0, 18))
+        P = int(2 ** rng.uniform(0, 14))
+        blocks = (rows + 255 * S) // 256
+        n = prompt8_parts(rows, G, D, S, P, int(rng.integers(1, rows + 1)), 148)
+        assert 1 <= n <= max(1, min(16, P // 4))
+        if n > 1:
+            cut += 1
+            assert blocks * n <= 65535 and blocks * 32 <= 65535
+    assert cut > 400
+    assert prompt8_parts(400, 8, 128, 1, 63, 100, 148) == 9                       # two blocks of rows a kv head: 144 blocks in a wave
+    assert prompt8_parts(2048, 32, 64, 1, 32, 2048, 148) == 1                     # a whole prompt that fills the device

@@ -97,8 +97,9 @@ __device__ __forceinline__ P8Block prompt8_block(const Prompt8Params& p, int b) 
   d.rows = d.n_pages = 0;
   for (int s0 = p.n_seqs - 1; s0 >= 0; s0 -= 32) {
     const int s = s0 - lane;
-    int n = 0;
-    if (s >= 0 && p.seq_kv_len[s] > 0) n = ((p.seq_q_start[s + 1] - p.seq_q_start[s]) * p.group + P8_ROWS - 1) / P8_ROWS;
+    int start = 0, q_len = 0, kv_len = 0;
+    if (s >= 0) start = p.seq_q_start[s], q_len = p.seq_q_start[s + 1] - start, kv_len = p.seq_kv_len[s];
+    const int n = kv_len > 0 ? (q_len * p.group + P8_ROWS - 1) / P8_ROWS : 0;
     int x = n;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
@@ -110,8 +111,9 @@ __device__ __forceinline__ P8Block prompt8_block(const Prompt8Params& p, int b) 
       const int src = __ffs(__ballot_sync(0xffffffffu, x > b)) - 1;
       d.seq = s0 - src;
       const int mb = __shfl_sync(0xffffffffu, x, src) - 1 - b;
-      d.q_start = p.seq_q_start[d.seq];
-      const int q_len = p.seq_q_start[d.seq + 1] - d.q_start, kv_len = p.seq_kv_len[d.seq];
+      d.q_start = __shfl_sync(0xffffffffu, start, src);
+      q_len = __shfl_sync(0xffffffffu, q_len, src);
+      kv_len = __shfl_sync(0xffffffffu, kv_len, src);
       d.row0 = mb * P8_ROWS;
       d.rows = min(P8_ROWS, q_len * p.group - d.row0);
       d.pos0 = kv_len - q_len;

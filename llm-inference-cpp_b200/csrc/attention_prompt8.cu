@@ -26,7 +26,7 @@
 // What bounds it: a row's way through the softmax of a page, 1,800 clocks from S to P with four warps on each scheduler; the
 // exponentials alone (16 a clock and SM) are 1,024 for the two tiles, the products 256 at head size 64 and 512 at 128, the
 // conversion 700 and 1,300 beside them.  A page of two tiles takes 1,900 and 2,400 clocks.  Measured: 2,048 tokens, 32 heads of 64,
-// 52 us (329 TFLOP/s); 600 and 600 tokens over 20,011 to 31,001 positions, 32 heads by 8 of 128, 593 us (659 TFLOP/s, 0.40 of what a
+// 52 us (331 TFLOP/s); 600 and 600 tokens over 20,011 to 31,001 positions, 32 heads by 8 of 128, 589 us (664 TFLOP/s, 0.41 of what a
 // library's bf16 product reaches).
 //
 // A step of few blocks leaves SMs idle: then a block's pages are cut into parts, each a block of its own that leaves (m, sum, O) per

@@ -446,7 +446,6 @@ __global__ void __launch_bounds__(P8_THREADS, 1) attention_prompt8_kernel(Prompt
             float down = __uint_as_float((uint32_t)(127 - min(ex, 126)) << 23);
             const float down2 = ex > 126 ? 1.f / (float)(1 << (ex - 126)) : 1.f;
             if (p.scale_log2 < 0.f) down = -down;                  // the factor of the scores below is positive
-            // (never quite 0: 0 times a masked key's -inf is no number)
             if (c == 0) s_top[tile][0][in] = fmaxf(ldexpf(fabsf(p.scale_log2), ex), 1e-30f);
             uint32_t h[4];
 #pragma unroll
@@ -484,7 +483,8 @@ __global__ void __launch_bounds__(P8_THREADS, 1) attention_prompt8_kernel(Prompt
       const float4 page = s_page[st];
       const uint32_t look = __float_as_uint(page.w);
       const int key0 = (pg0 + j) * PAGE8 + 32 * half;
-      float to_log2 = row_fac * page.x, off = page.y + neg_ref;
+      // (never 0, where small queries meet small keys: 0 times a masked key's -inf is no number)
+      float to_log2 = fmaxf(row_fac * page.x, FLT_MIN), off = page.y + neg_ref;
       p8_ld_wait();
       if (look & PG_WIDE) {                                        // (kmax 1 / row_fac, vmax 1: the scores are final)
         to_log2 = 1.f;

@@ -1,0 +1,35 @@
+"""Attention over a cache held in 8 bits where numbers are far apart or small: factors of a page's scores that underflow (GPU)."""
+import numpy as np
+import pytest
+import torch
+
+from test_rows8_gpu import STEPS, Batch, K, attend_by, check
+
+pytestmark = pytest.mark.gpu
+
+
+def times_keys(b, f, since=0):
+    """Every key from its sequence's position ``since`` on (below 0: from that many pages ahead of its last one) f times as large;
+    f = 0: with codes of zero, as the append leaves them."""
+    for i, (n, h) in enumerate(b.lens):
+        if h:
+            p = np.arange(max(0, (h - 1) // 64 + 1 + since) * 64 if since < 0 else since, h)
+            page, row = torch.tensor(b.table_np[i][p // 64]).long().cuda(), torch.tensor(p % 64).cuda()
+            b.k.scales[page, :, row] *= f
+            if f == 0.0:
+                b.k.codes.view(torch.uint8)[page, :, row] = 0
+            b.kx[i][p] *= f
+
+
+@pytest.mark.parametrize("kernel", ["rows", "prompt", "any"])
+@pytest.mark.parametrize("H,G,D,step", [(4, 2, 64, "prompts"), (8, 2, 128, "messages")])
+@pytest.mark.parametrize("queries,keys,scale", [(2.0 ** -60, 0.0, None), (2.0 ** -70, 2.0 ** -80, None), (1.0, 0.0, 0.0), (1.0, 0.0, 1e-30),
+                                                (1.0, 2.0 ** -60, 1e-30), (0.0, 0.0, -0.2)])
+def test_scores_whose_factor_is_tiny(kernel, H, G, D, step, queries, keys, scale):
+    """Queries, keys and softmax scales whose product is 0 in 32 bits: a mean of what is seen, not NaN, in the page that is partly masked."""
+    b = Batch(STEPS[step], G, D, "int8", seed=3)
+    b.fill()
+    times_keys(b, keys, since=-1)
+    q = torch.tensor(b.rng.normal(size=(b.T, H * D)) * queries).to(torch.bfloat16).cuda()
+    scale = D ** -0.5 if scale is None else scale
+    check(b, H, q, attend_by(kernel, b, H, q, 0, scale), "bfloat16", 0, scale)

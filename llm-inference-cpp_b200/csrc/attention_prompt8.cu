@@ -446,7 +446,7 @@ __global__ void __launch_bounds__(P8_THREADS, 1) attention_prompt8_kernel(Prompt
             float down = __uint_as_float((uint32_t)(127 - min(ex, 126)) << 23);
             const float down2 = ex > 126 ? 1.f / (float)(1 << (ex - 126)) : 1.f;
             if (p.scale_log2 < 0.f) down = -down;                  // the factor of the scores below is positive
-            if (c == 0) s_top[tile][0][in] = fmaxf(ldexpf(fabsf(p.scale_log2), ex), 1e-30f);
+            if (c == 0) s_top[tile][0][in] = ldexpf(fabsf(p.scale_log2), ex);
             uint32_t h[4];
 #pragma unroll
             for (int e = 0; e < 4; ++e) h[e] = half2_bits(__floats2half2_rn(x[2 * e] * down * down2, x[2 * e + 1] * down * down2));

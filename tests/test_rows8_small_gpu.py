@@ -1,9 +1,10 @@
-"""Attention over a cache held in 8 bits where numbers are far apart or small: factors of a page's scores that underflow (GPU)."""
+"""Attention over a cache held in 8 bits where numbers are far apart or small: factors of a page's scores that underflow,
+queries far below 1 (GPU)."""
 import numpy as np
 import pytest
 import torch
 
-from test_rows8_gpu import STEPS, Batch, K, attend_by, check
+from test_rows8_gpu import DT, STEPS, Batch, K, attend_by, check
 
 pytestmark = pytest.mark.gpu
 
@@ -33,3 +34,17 @@ def test_scores_whose_factor_is_tiny(kernel, H, G, D, step, queries, keys, scale
     q = torch.tensor(b.rng.normal(size=(b.T, H * D)) * queries).to(torch.bfloat16).cuda()
     scale = D ** -0.5 if scale is None else scale
     check(b, H, q, attend_by(kernel, b, H, q, 0, scale), "bfloat16", 0, scale)
+
+
+@pytest.mark.parametrize("kernel,dtype", [("rows", "bfloat16"), ("prompt", "bfloat16"), ("any", "bfloat16"), ("rows", "float32")])
+@pytest.mark.parametrize("H,G,D,step", [(4, 2, 64, "prompts"), (8, 2, 128, "messages")])
+def test_queries_far_below_one(kernel, dtype, H, G, D, step):
+    """Queries around 2^-100 and keys around 2^100: scores of ordinary size."""
+    b = Batch(STEPS[step], G, D, "int8", seed=3)
+    b.fill()
+    times_keys(b, 2.0 ** 100)
+    q = torch.tensor(b.rng.normal(size=(b.T, H * D)) * 2.0 ** -100).to(DT[dtype]).cuda()
+    out = torch.full((b.T, H * D), 7.0, dtype=DT[dtype], device="cuda")
+    K().attention8(q, out, b.k, b.v, b.ctx, b.table, H, G, D, D ** -0.5, kernel=kernel)
+    K().check_device_errors("cuda:0")
+    check(b, H, q, out, dtype)

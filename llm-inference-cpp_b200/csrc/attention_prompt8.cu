@@ -14,7 +14,9 @@
 //                 swizzled layout that the products read; so the scales cost the softmax nothing per key: kmax joins its scale,
 //                 log2 vmax its offset.  (A page whose scales are more than 2^12 apart would lose bits of its small rows, which may be
 //                 all that a query sees: there K' and V' are the codes themselves and the softmax takes each key's scales.)
-//   S = Q' K'^T   tcgen05.mma, Q' the queries divided by a power of two per row (fp16, exact but for entries 2^-14 of the largest)
+//   S = Q' K'^T   tcgen05.mma, Q' the queries times a power of two per row that brings its largest near 2^15, in fp16: bf16 queries
+//                 exactly, down to 2^-29 of the row's largest entry; 32-bit ones (those that `rope` makes) rounded to 11 bits, which
+//                 costs a score no more than what the keys' rounding costs it
 //   softmax       two threads own a row, 32 keys of a page each: tcgen05.ld, mask, maximum, exp2, sum; P = 2^(s + log2 vmax - m) goes
 //                 back to tensor memory as fp16 over the S it has read; the sum of w is that of P / vmax
 //   O += P V'     tcgen05.mma with A in tensor memory, accumulating in fp32; m follows the running maximum (of s + log2 vmax) only
@@ -400,7 +402,7 @@ __global__ void __launch_bounds__(P8_THREADS, 1) attention_prompt8_kernel(Prompt
                    : "=r"(r) : "r"(1 + tile * 4 + quad), "r"(x ? 1u : 0u) : "memory");
       return r != 0u;
     };
-    // The rows' queries, divided by a power of two above the row's largest.  The two warps of 32 rows take 16 each, the lanes of a row
+    // The rows' queries, times a power of two each.  The two warps of 32 rows take 16 each, the lanes of a row
     // beside each other, with a row's 8 entries a lane and BATCH loads under way.
     float row_fac;
     {
@@ -441,15 +443,15 @@ __global__ void __launch_bounds__(P8_THREADS, 1) attention_prompt8_kernel(Prompt
             for (int e = 0; e < 8; ++e) a = fmaxf(a, fabsf(x[e]));
 #pragma unroll
             for (int o = LANES / 2; o; o >>= 1) a = fmaxf(a, __shfl_xor_sync(0xffffffffu, a, o));
+            // the row's largest entry lies between 2^14 and 2^15 (rows that are zero or not finite: as they are, times 2^15)
             int ex = 0;
             if (a > 0.f && a <= FLT_MAX) ex = max(-100, (int)((__float_as_uint(a) >> 23) & 255) - 126);
-            float down = __uint_as_float((uint32_t)(127 - min(ex, 126)) << 23);
-            const float down2 = ex > 126 ? 1.f / (float)(1 << (ex - 126)) : 1.f;
+            float down = __uint_as_float((uint32_t)(127 + 15 - ex) << 23);
             if (p.scale_log2 < 0.f) down = -down;                  // the factor of the scores below is positive
-            if (c == 0) s_top[tile][0][in] = ldexpf(fabsf(p.scale_log2), ex);
+            if (c == 0) s_top[tile][0][in] = ldexpf(fabsf(p.scale_log2), ex - 15);
             uint32_t h[4];
 #pragma unroll
-            for (int e = 0; e < 4; ++e) h[e] = half2_bits(__floats2half2_rn(x[2 * e] * down * down2, x[2 * e + 1] * down * down2));
+            for (int e = 0; e < 4; ++e) h[e] = half2_bits(__floats2half2_rn(x[2 * e] * down, x[2 * e + 1] * down));
             asm volatile("st.shared.v4.u32 [%0], {%1, %2, %3, %4};"
                          ::"r"(q_smem + tile * C::Q_TILE + in * 128 + (c / 8) * (P8_TILE * 128) + (((c % 8) ^ (in & 7)) << 4)),
                          "r"(h[0]), "r"(h[1]), "r"(h[2]), "r"(h[3]) : "memory");

@@ -17,7 +17,9 @@
 //    in shared memory with cp.async, across the borders of sequences; warps meet only where a (sequence, kv head) ends, through the
 //    stages that they have just read.
 //  * The products run on mma.sync (m16n8k16, fp16): a chunk's keys are the 16 rows, the query rows the 8 columns, the G heads of the
-//    group together.  A code is an fp16 number exactly; a query row is divided by a power of two so that its entries are at most 1.
+//    group together.  A code is an fp16 number exactly; a query row is multiplied by a power of two that brings its largest entry near
+//    2^15, so that smaller ones keep their bits as far down as fp16 reaches: a bf16 query is exact down to 2^-29 of the largest, the
+//    32-bit ones that `rope` makes of bf16 rows are rounded to 11 bits.
 //    Both scales stay in fp32: k_scale on the scores, v_scale on the weights, before they are rounded to fp16.  In the 32-bit path
 //    queries and weights are the sums of two fp16 numbers (22 bits), and a chunk's sum is added to the output's in fp32.
 //  * The weights are kept relative to a maximum M of s_j + log2 v_scale[j] (not of s_j), so that the fp16 number w_j * v_scale[j] is at
@@ -428,20 +430,20 @@ __global__ void __launch_bounds__(RW8_WARPS * 32, (Rw8Cfg<D, NT, T>::BLOCKS)) at
       for (int i = 0; i < D / 4; ++i) a = fmaxf(a, fabsf(x[i]));
       a = fmaxf(a, __shfl_xor_sync(0xffffffffu, a, 1));
       a = fmaxf(a, __shfl_xor_sync(0xffffffffu, a, 2));
-      // the power of two above the row's largest entry (a row that is zero or not finite: 1)
+      // times a power of two that brings the row's largest entry between 2^14 and 2^15 (rows that are zero or not finite: 2^15)
       int ex = 0;
       if (a > 0.f && a <= FLT_MAX) ex = max(-100, (int)((__float_as_uint(a) >> 23) & 255) - 126);
-      const float down = __uint_as_float((uint32_t)(127 - min(ex, 126)) << 23), down2 = ex > 126 ? 1.f / (float)(1 << (ex - 126)) : 1.f;
+      const float down = __uint_as_float((uint32_t)(127 + 15 - ex) << 23);
 #pragma unroll
       for (int s = 0; s < KS; ++s)
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
-          const float y0 = x[4 * s + 2 * h] * down * down2, y1 = x[4 * s + 2 * h + 1] * down * down2;
+          const float y0 = x[4 * s + 2 * h] * down, y1 = x[4 * s + 2 * h + 1] * down;
           const __half2 hi = __floats2half2_rn(y0, y1);
           qf[0][n][s][h] = as_u32(hi);
           if (SP == 2) qf[SP - 1][n][s][h] = pack_half2(y0 - __low2float(hi), y1 - __high2float(hi));
         }
-      const float f = ldexpf(p.scale_log2, ex);
+      const float f = ldexpf(p.scale_log2, ex - 15);
 #pragma unroll
       for (int j = 0; j < 2; ++j) {
         fac[n][j] = __shfl_sync(0xffffffffu, f, (2 * t + j) * 4);

@@ -1,5 +1,5 @@
 """Attention over a cache held in 8 bits where numbers are far apart or small: factors of a page's scores that underflow,
-queries far below 1 (GPU)."""
+queries far below 1 and with one entry far above the others (GPU)."""
 import numpy as np
 import pytest
 import torch
@@ -44,6 +44,24 @@ def test_queries_far_below_one(kernel, dtype, H, G, D, step):
     b.fill()
     times_keys(b, 2.0 ** 100)
     q = torch.tensor(b.rng.normal(size=(b.T, H * D)) * 2.0 ** -100).to(DT[dtype]).cuda()
+    out = torch.full((b.T, H * D), 7.0, dtype=DT[dtype], device="cuda")
+    K().attention8(q, out, b.k, b.v, b.ctx, b.table, H, G, D, D ** -0.5, kernel=kernel)
+    K().check_device_errors("cuda:0")
+    check(b, H, q, out, dtype)
+
+
+@pytest.mark.parametrize("kernel,dtype,ratio", [("rows", "bfloat16", 22), ("prompt", "bfloat16", 22), ("any", "bfloat16", 22), ("rows", "float32", 14)])
+@pytest.mark.parametrize("H,G,D,step", [(4, 2, 64, "prompts"), (8, 2, 128, "messages")])
+def test_queries_with_one_entry_far_above_the_others(kernel, dtype, ratio, H, G, D, step):
+    """The entry that sticks out meets zeros in every key: the scores are those of the others, 2^-ratio as large."""
+    b = Batch(STEPS[step], G, D, "int8", seed=3)
+    b.fill()
+    b.k.codes[..., 5] = 0
+    for x in b.kx:
+        x[..., 5] = 0.0
+    q = b.rng.normal(size=(b.T, H, D)) * 1.5
+    q[..., 5] = 2.0 ** ratio
+    q = torch.tensor(q.reshape(b.T, H * D)).to(DT[dtype]).cuda()
     out = torch.full((b.T, H * D), 7.0, dtype=DT[dtype], device="cuda")
     K().attention8(q, out, b.k, b.v, b.ctx, b.table, H, G, D, D ** -0.5, kernel=kernel)
     K().check_device_errors("cuda:0")

@@ -21,9 +21,13 @@
 //    2^15, so that smaller ones keep their bits as far down as fp16 reaches: a bf16 query is exact down to 2^-29 of the largest, the
 //    32-bit ones that `rope` makes of bf16 rows are rounded to 11 bits.
 //    Both scales stay in fp32: k_scale on the scores, v_scale on the weights, before they are rounded to fp16.  In the 32-bit path
-//    queries and weights are the sums of two fp16 numbers (22 bits), and a chunk's sum is added to the output's in fp32.
-//  * The weights are kept relative to a maximum M of s_j + log2 v_scale[j] (not of s_j), so that the fp16 number w_j * v_scale[j] is at
-//    most 2^8 and small scales lose nothing.  M moves only when a weight passes 2^8: the common chunk has one vote and no shuffles.
+//    queries and weights are the sums of two fp16 numbers (22 bits), the second of a weight 2^11 as large as it counts, so that small
+//    weights have it too; sixteen keys' sum is added to the output's in fp32, and the weights' sum is compensated (Kahan).
+//  * The weights are kept relative to a maximum M of s_j + log2 v_scale[j] (not of s_j), so that small scales lose nothing: the fp16
+//    number w_j * v_scale[j] is 2^7 for the largest when M moves, and M moves only when one passes 2^15 — the common chunk has one vote
+//    and no shuffles.  A weight keeps 11 bits down to 2^-21 of the row's largest; below that it is off by at most 2^-32 of the largest
+//    (32-bit path: 22 bits, 2^-43).  Many small weights beside a large one need them that far down: of 32,000 keys 17.5 nats below
+//    another an eighth, its warp's, was lost with M 2^7 higher: 1e-4 of the output.
 #include <math.h>
 
 #include <type_traits>
@@ -35,9 +39,10 @@ namespace llmi {
 
 constexpr int RW8_WARPS = 8;
 constexpr int RW8_MAX_ENTRIES = 4096;      // (sequence, row tile)s of a call
-constexpr float RW8_LAZY = 256.f;          // weights up to this before the reference maximum moves
+constexpr float RW8_UP = 7.f;              // the largest weight is 2^7 where the reference maximum has moved
+constexpr float RW8_LAZY = 32768.f;        // weights up to 2^15 before it moves
 constexpr float RW8_SUM = 5.192296858534828e33f;   // 2^112: a sum of weights up to this (keys whose values are zeros may weigh that much)
-constexpr float RW8_TINY = 7.888609052210118e-31f; // 2^-100: smaller value scales count as this where M is made
+constexpr float RW8_TINY = 1.0097419586828951e-28f; // 2^-93: smaller value scales count as this where M is made
 
 struct Rows8Params {
   const void* q;
@@ -381,11 +386,12 @@ __global__ void __launch_bounds__(RW8_WARPS * 32, (Rw8Cfg<D, NT, T>::BLOCKS)) at
     at_unit = s.end;
     if (s.n <= 0) continue;                // (the range ends among the units of no page)
 
-    float O[KS][NT][4], M[NT][2], neg[NT][2], L[NT][2];      // neg: -M, 0 while there is no M
+    // neg: -M, 0 while there is no M; Lc: what L has too much (32-bit path)
+    float O[KS][NT][4], M[NT][2], neg[NT][2], L[NT][2], Lc[NT][2];
 #pragma unroll
     for (int n = 0; n < NT; ++n) {
 #pragma unroll
-      for (int j = 0; j < 2; ++j) M[n][j] = -INFINITY, neg[n][j] = 0.f, L[n][j] = 0.f;
+      for (int j = 0; j < 2; ++j) M[n][j] = -INFINITY, neg[n][j] = L[n][j] = Lc[n][j] = 0.f;
 #pragma unroll
       for (int i = 0; i < KS; ++i)
 #pragma unroll
@@ -507,7 +513,7 @@ __global__ void __launch_bounds__(RW8_WARPS * 32, (Rw8Cfg<D, NT, T>::BLOCKS)) at
         bool fine = true;
 #pragma unroll
         for (int n = 0; n < NT; ++n) {
-          sum[n][0] = L[n][0], sum[n][1] = L[n][1];
+          sum[n][0] = SP == 2 ? 0.f : L[n][0], sum[n][1] = SP == 2 ? 0.f : L[n][1];
 #pragma unroll
           for (int m = 0; m < MT; ++m) {
             float w[4];
@@ -523,10 +529,10 @@ __global__ void __launch_bounds__(RW8_WARPS * 32, (Rw8Cfg<D, NT, T>::BLOCKS)) at
               const __half2 hi = __floats2half2_rn(w[2 * h], w[2 * h + 1]);
               top = __hmax2(top, hi);
               pb[0][m][n][h] = as_u32(hi);
-              if (SP == 2) pb[SP - 1][m][n][h] = pack_half2(w[2 * h] - __low2float(hi), w[2 * h + 1] - __high2float(hi));
+              if (SP == 2) pb[SP - 1][m][n][h] = pack_half2((w[2 * h] - __low2float(hi)) * 2048.f, (w[2 * h + 1] - __high2float(hi)) * 2048.f);
             }
           }
-          fine = fine && !(sum[n][0] > RW8_SUM) && !(sum[n][1] > RW8_SUM);
+          fine = fine && !((SP == 2 ? L[n][0] : 0.f) + sum[n][0] > RW8_SUM) && !((SP == 2 ? L[n][1] : 0.f) + sum[n][1] > RW8_SUM);
         }
         return fine && !(fmaxf(__low2float(top), __high2float(top)) > RW8_LAZY);
       };
@@ -545,8 +551,11 @@ __global__ void __launch_bounds__(RW8_WARPS * 32, (Rw8Cfg<D, NT, T>::BLOCKS)) at
                 if (!is_hidden(m, n, j + 2 * h)) mx = fmaxf(mx, S[m][n][j + 2 * h] * (ks[m][h] * fac[n][j]) + fast_log2(fmaxf(vs[m][h], RW8_TINY)));
 #pragma unroll
             for (int o = 4; o < 32; o <<= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, o));
-            const float m_new = fmaxf(M[n][j], mx), f = M[n][j] == -INFINITY ? 1.f : fast_exp2(M[n][j] - m_new);
-            if (M[n][j] != -INFINITY) L[n][j] = rescale8(L[n][j], M[n][j] - m_new);
+            const float m_new = fmaxf(M[n][j], mx - RW8_UP), f = M[n][j] == -INFINITY ? 1.f : fast_exp2(M[n][j] - m_new);
+            if (M[n][j] != -INFINITY) {
+              L[n][j] = rescale8(L[n][j], M[n][j] - m_new);
+              if (SP == 2) Lc[n][j] = rescale8(Lc[n][j], M[n][j] - m_new);
+            }
 #pragma unroll
             for (int i = 0; i < KS; ++i) O[i][n][j] *= f, O[i][n][j + 2] *= f;
             M[n][j] = m_new;
@@ -556,17 +565,18 @@ __global__ void __launch_bounds__(RW8_WARPS * 32, (Rw8Cfg<D, NT, T>::BLOCKS)) at
         unset = __any_sync(0xffffffffu, unset);
         weigh();
       }
-      float Oc[SP == 2 ? KS : 1][SP == 2 ? NT : 1][4];
-      if (SP == 2) {
 #pragma unroll
-        for (int i = 0; i < KS; ++i)
+      for (int n = 0; n < NT; ++n)
 #pragma unroll
-          for (int n = 0; n < NT; ++n)
-#pragma unroll
-            for (int j = 0; j < 4; ++j) Oc[SP == 2 ? i : 0][SP == 2 ? n : 0][j] = 0.f;
-      }
-#pragma unroll
-      for (int n = 0; n < NT; ++n) L[n][0] = sum[n][0], L[n][1] = sum[n][1];
+        for (int j = 0; j < 2; ++j) {
+          if (SP == 2) {
+            const float x = sum[n][j] - Lc[n][j], l = L[n][j] + x;
+            Lc[n][j] = (l - L[n][j]) - x;
+            L[n][j] = l;
+          } else {
+            L[n][j] = sum[n][j];
+          }
+        }
       const int seen0 = max(d.lo - key0, 0), seen1 = d.last - key0;      // rows of the chunk that some query sees
 #pragma unroll
       for (int m = 0; m < MT; ++m) {
@@ -603,21 +613,23 @@ __global__ void __launch_bounds__(RW8_WARPS * 32, (Rw8Cfg<D, NT, T>::BLOCKS)) at
           halves8x4<HELD>(z4[1], a23[0], a23[1]);
           halves8x4<HELD>(z4[3], a23[2], a23[3]);
 #pragma unroll
-          for (int n = 0; n < NT; ++n)
+          for (int n = 0; n < NT; ++n) {
+            if (SP == 2) {
+              float c0[4] = {0.f, 0.f, 0.f, 0.f}, c1[4] = {0.f, 0.f, 0.f, 0.f};
+              mma_f16(c0, a01, pb[SP - 1][m][n][0], pb[SP - 1][m][n][1]);
+              mma_f16(c1, a23, pb[SP - 1][m][n][0], pb[SP - 1][m][n][1]);
 #pragma unroll
-            for (int z = 0; z < SP; ++z) {
-              mma_f16(SP == 2 ? Oc[SP == 2 ? 2 * w : 0][SP == 2 ? n : 0] : O[2 * w][n], a01, pb[z][m][n][0], pb[z][m][n][1]);
-              mma_f16(SP == 2 ? Oc[SP == 2 ? 2 * w + 1 : 0][SP == 2 ? n : 0] : O[2 * w + 1][n], a23, pb[z][m][n][0], pb[z][m][n][1]);
+              for (int j = 0; j < 4; ++j) c0[j] *= 1.f / 2048.f, c1[j] *= 1.f / 2048.f;
+              mma_f16(c0, a01, pb[0][m][n][0], pb[0][m][n][1]);
+              mma_f16(c1, a23, pb[0][m][n][0], pb[0][m][n][1]);
+#pragma unroll
+              for (int j = 0; j < 4; ++j) O[2 * w][n][j] += c0[j], O[2 * w + 1][n][j] += c1[j];
+            } else {
+              mma_f16(O[2 * w][n], a01, pb[0][m][n][0], pb[0][m][n][1]);
+              mma_f16(O[2 * w + 1][n], a23, pb[0][m][n][0], pb[0][m][n][1]);
             }
+          }
         }
-      }
-      if (SP == 2) {
-#pragma unroll
-        for (int i = 0; i < KS; ++i)
-#pragma unroll
-          for (int n = 0; n < NT; ++n)
-#pragma unroll
-            for (int j = 0; j < 4; ++j) O[i][n][j] += Oc[SP == 2 ? i : 0][SP == 2 ? n : 0][j];
       }
     };
 
@@ -635,9 +647,11 @@ __global__ void __launch_bounds__(RW8_WARPS * 32, (Rw8Cfg<D, NT, T>::BLOCKS)) at
 #pragma unroll
     for (int n = 0; n < NT; ++n)
 #pragma unroll
-      for (int j = 0; j < 2; ++j)
+      for (int j = 0; j < 2; ++j) {
+        if (SP == 2) L[n][j] -= Lc[n][j];
 #pragma unroll
         for (int o = 4; o < 32; o <<= 1) L[n][j] += __shfl_xor_sync(0xffffffffu, L[n][j], o);
+      }
 
     // ---- the warps' states meet: each leaves its own where nothing is being copied to (the stage read last; `issue` fills the one
     // before it first), then a warp has some tiles of the output from all eight ----

@@ -1,10 +1,10 @@
 """Attention over a cache held in 8 bits where numbers are far apart or small: factors of a page's scores that underflow,
-queries far below 1 and with one entry far above the others (GPU)."""
+queries far below 1 and with one entry far above the others, a weight far above many (GPU)."""
 import numpy as np
 import pytest
 import torch
 
-from test_rows8_gpu import DT, STEPS, Batch, K, attend_by, check
+from test_rows8_gpu import DT, HELD, STEPS, Batch, K, attend_by, check
 
 pytestmark = pytest.mark.gpu
 
@@ -66,3 +66,56 @@ def test_queries_with_one_entry_far_above_the_others(kernel, dtype, ratio, H, G,
     K().attention8(q, out, b.k, b.v, b.ctx, b.table, H, G, D, D ** -0.5, kernel=kernel)
     K().check_device_errors("cuda:0")
     check(b, H, q, out, dtype)
+
+
+def one_above(S, G, D, n, held, nats):
+    """S sequences of n positions: position 5 scores ``nats`` for a query whose first entry is 1, all others 0; its value is 1 in the
+    first dim, the others' are 1 in all dims but that."""
+    k = K()
+    P = -(-n // 64)
+    table = torch.randperm(S * P).to(torch.int32).view(S, P).cuda()
+    kk, vv = (k.Rows8(torch.zeros((S * P, G, 64, D), dtype=torch.uint8, device="cuda").view(HELD[held]), torch.ones((S * P, G, 64), device="cuda"))
+              for _ in range(2))
+    one = 1 if held == "int8" else 0x38           # the code of 1
+    first = table[:, 0].long()
+    kk.codes.view(torch.uint8)[first, :, 5, 0] = one
+    kk.scales[first, :, 5] = nats
+    values = vv.codes.view(torch.uint8)
+    values.fill_(one)
+    values[..., 0] = 0
+    values[first, :, 5] = 0
+    values[first, :, 5, 0] = one
+    return table, kk, vv
+
+
+@pytest.mark.parametrize("kernel,dtype,S,G,H,D,n,new", [
+    # (a block for each sequence and kv head, and many blocks for one)
+    ("rows", "float32", 3, 32, 32, 64, 32000, 1), ("rows", "float32", 6, 16, 16, 128, 16000, 1), ("rows", "float32", 1, 1, 1, 64, 100000, 1),
+    ("rows", "bfloat16", 6, 32, 32, 64, 32000, 1), ("rows", "bfloat16", 12, 16, 16, 128, 16000, 1), ("rows", "bfloat16", 1, 1, 1, 64, 100000, 1),
+    ("any", "float32", 1, 1, 1, 64, 100000, 3)])
+@pytest.mark.parametrize("held", ["int8", "float8_e4m3"])
+def test_one_key_far_above_many(kernel, dtype, S, G, H, D, n, new, held):
+    """One key 17.5 nats above tens of thousands, whose weights count together.
+
+    Tolerances: 2^-17 as elsewhere; a sum of n weights is n / 128 additions a thread or fewer, each rounded by 2^-24 of it; bf16: weights
+    and values are off by 2^-11 each, a weight far below the largest by 2^-32 of that, and the output by 2^-8."""
+    from llmi_b200.engine.batch import StepContext, short_message
+    nats = 17.5
+    table, k, v = one_above(S, G, D, n, held, nats)
+    cu = lambda a: torch.tensor(a, dtype=torch.int32, device="cuda")  # noqa: E731
+    c = StepContext()
+    c.tok_seq, c.tok_pos = cu([s for s in range(S) for _ in range(new)]), cu([p for s in range(S) for p in range(n - new, n)])
+    c.seq_q_start, c.seq_kv_len = cu([s * new for s in range(S + 1)]), cu([n] * S)
+    c.n_tokens, c.n_seqs, c.max_q_len, c.decode = S * new, S, new, new == 1
+    c.short_message = 0 if c.decode else short_message(new)
+    q = torch.zeros(S * new, H, D, dtype=DT[dtype], device="cuda")
+    q[..., 0] = 1.0
+    out = torch.full((S * new, H * D), 7.0, dtype=DT[dtype], device="cuda")
+    K().attention8(q.view(S * new, -1), out, k, v, c, table, H, G, D, 1.0, kernel=kernel)
+    K().check_device_errors("cuda:0")
+    others = torch.arange(n - new, n, dtype=torch.float64) * np.exp(-nats)
+    want = (others / (others + 1.0)).repeat(S)[:, None, None].repeat(1, H, D)
+    want[..., 0] = 1.0 - want[..., 0]
+    off = (out.double().cpu().view(-1, H, D) - want).abs()
+    tol = 2.0 ** -17 + n / 128 * 2.0 ** -24 * want + (2.0 ** -24 * want if dtype == "float32" else (2.0 ** -10 + 2.0 ** -8) * want + n * 2.0 ** -32)
+    assert bool((off <= tol).all()), (float((off / tol).max()), float(off[..., 0].max()), float(off[..., 1:].max()))

@@ -19,8 +19,11 @@
 //                 costs a score no more than what the keys' rounding costs it
 //   softmax       two threads own a row, 32 keys of a page each: tcgen05.ld, mask, maximum, exp2, sum; P = 2^(s + log2 vmax - m) goes
 //                 back to tensor memory as fp16 over the S it has read; the sum of w is that of P / vmax
-//   O += P V'     tcgen05.mma with A in tensor memory, accumulating in fp32; m follows the running maximum (of s + log2 vmax) only
-//                 when that has grown by more than 8, so O is rescaled a few times per row.  At head size 64 tensor memory has room for
+//   O += P V'     tcgen05.mma with A in tensor memory, accumulating in fp32; m lies 7 below the running maximum (of s + log2 vmax)
+//                 and follows it only when that has grown by more than 8, so O is rescaled a few times per row.  P is at most 2^15
+//                 and for the largest 2^7 or more: it keeps 11 bits down to 2^-21 of the row's largest, and what is below is off by
+//                 2^-32 of that at most (with m at the maximum itself 32,000 keys 17.5 nats below another were lost together: 8e-4 of
+//                 the output).  At head size 64 tensor memory has room for
 //                 an O of each thread's keys, with their own m and sum: nothing passes between the two before the end.  At 128 the two
 //                 share one O, ask each other on every page whether an m has to follow (a barrier of 64 threads, 7 % of the page at 64),
 //                 and exchange maxima only then.
@@ -50,11 +53,13 @@ constexpr int P8_SOFTMAX = 4, P8_CONVERT = 20, P8_WARPS = 24;
 constexpr int P8_THREADS = P8_WARPS * 32;
 constexpr int P8_JOINS = 32;              // blocks of 8 warps that join a block's rows
 constexpr int P8_TMEM = 512;              // per tile of rows 256 columns: S of even and odd pages (64 each), O (D, or 64 of each half of the keys)
-constexpr float P8_LAZY = 8.0f;           // the reference maximum follows where it is 2^8 behind
+constexpr float P8_UP = 7.0f;             // where the reference maximum moves it goes 7 below the largest score: weights of up to 2^7
+constexpr float P8_LAZY = 15.0f;          // it moves where a weight would pass 2^15
 constexpr uint32_t PG_WIDE = 1u, PG_POISON = 2u;       // the page's scales are far apart; it has values that are no numbers
 constexpr float P8_LIGHT = 8.077935669463161e-28f;     // 2^-90
 constexpr float P8_APART = 2.44140625e-4f;             // 2^-12
 constexpr float P8_TINY = 7.888609052210118e-31f;      // 2^-100: smaller scales of a page count as this
+constexpr float P8_MUCH = 5.192296858534828e33f;       // 2^112: sums of weights beyond this move the reference, too (values near 2^-100)
 
 struct Prompt8Params {
   const void* q;                // bf16, or fp32 with q_f32
@@ -444,11 +449,11 @@ __global__ void __launch_bounds__(P8_THREADS, 1) attention_prompt8_kernel(Prompt
 #pragma unroll
             for (int o = LANES / 2; o; o >>= 1) a = fmaxf(a, __shfl_xor_sync(0xffffffffu, a, o));
             // the row's largest entry lies between 2^14 and 2^15 (rows that are zero or not finite: as they are, times 2^15)
-            int ex = 0;
-            if (a > 0.f && a <= FLT_MAX) ex = max(-100, (int)((__float_as_uint(a) >> 23) & 255) - 126);
-            float down = __uint_as_float((uint32_t)(127 + 15 - ex) << 23);
+            int up = 15;
+            if (a > 0.f && a <= FLT_MAX) up = min(115, 141 - (int)(__float_as_uint(a) >> 23));
+            float down = __uint_as_float((uint32_t)(127 + up) << 23);
             if (p.scale_log2 < 0.f) down = -down;                  // the factor of the scores below is positive
-            if (c == 0) s_top[tile][0][in] = ldexpf(fabsf(p.scale_log2), ex - 15);
+            if (c == 0) s_top[tile][0][in] = ldexpf(fabsf(p.scale_log2), -up);
             uint32_t h[4];
 #pragma unroll
             for (int e = 0; e < 4; ++e) h[e] = half2_bits(__floats2half2_rn(x[2 * e] * down, x[2 * e + 1] * down));
@@ -468,7 +473,7 @@ __global__ void __launch_bounds__(P8_THREADS, 1) attention_prompt8_kernel(Prompt
     }
     const int n = n_tile[tile];
     const uint32_t t_lane = (uint32_t)(quad * 32) << 16, t_tile = tmem + 256u * tile + t_lane, t_o = t_tile + 128u + (uint32_t)(OC * half);
-    // the reference maximum (of s + log2 vmax, base 2) and 0 less it (0 while there is none); the sum of 2^(s - m_ref) over this half, and
+    // the reference (7 below a maximum of s + log2 vmax, base 2) and 0 less it (0 while there is none); the sum of 2^(s - m_ref) over this half, and
     // (where the halves share a maximum) over the other one when they last met
     float m_ref = -INFINITY, neg_ref = 0.f, l_run = 0.f, l_other = 0.f;
     bool ok = true;
@@ -509,7 +514,7 @@ __global__ void __launch_bounds__(P8_THREADS, 1) attention_prompt8_kernel(Prompt
       // the warp, or of the two that share rows and their Os, go the long way.
       const bool light = look != 0u || page.z * P8_LIGHT > l_run + l_other;
       bool by_key = false;
-      const bool grown = top > m_ref + P8_LAZY || light;
+      const bool grown = top > m_ref + P8_LAZY || light || l_run > P8_MUCH;
       if (OWN ? __any_sync(0xffffffffu, grown) : any_of_pair(grown)) {
         if (!OWN) {
           s_top[tile][half][in_tile] = top;
@@ -519,7 +524,9 @@ __global__ void __launch_bounds__(P8_THREADS, 1) attention_prompt8_kernel(Prompt
           l_other = s_sum[tile][half ^ 1][in_tile];
           meet();
         }
-        if (top > m_ref + P8_LAZY) {
+        const bool much = l_run + l_other > P8_MUCH;
+        if (top > m_ref + P8_LAZY || much) {
+          top = fmaxf(top - P8_UP, much ? m_ref + P8_LAZY : -INFINITY);
           if (m_ref != -INFINITY) {
             corr = fast_exp2(m_ref - top);
             l_run = rescale8(l_run, m_ref - top);

@@ -88,20 +88,10 @@ def one_above(S, G, D, n, held, nats):
     return table, kk, vv
 
 
-@pytest.mark.parametrize("kernel,dtype,S,G,H,D,n,new", [
-    # (a block for each sequence and kv head, and many blocks for one)
-    ("rows", "float32", 3, 32, 32, 64, 32000, 1), ("rows", "float32", 6, 16, 16, 128, 16000, 1), ("rows", "float32", 1, 1, 1, 64, 100000, 1),
-    ("rows", "bfloat16", 6, 32, 32, 64, 32000, 1), ("rows", "bfloat16", 12, 16, 16, 128, 16000, 1), ("rows", "bfloat16", 1, 1, 1, 64, 100000, 1),
-    ("any", "float32", 1, 1, 1, 64, 100000, 3)])
-@pytest.mark.parametrize("held", ["int8", "float8_e4m3"])
-def test_one_key_far_above_many(kernel, dtype, S, G, H, D, n, new, held):
-    """One key 17.5 nats above tens of thousands, whose weights count together.
-
-    Tolerances: 2^-17 as elsewhere; a sum of n weights is n / 128 additions a thread or fewer, each rounded by 2^-24 of it; bf16: weights
-    and values are off by 2^-11 each, a weight far below the largest by 2^-32 of that, and the output by 2^-8."""
+def of_the_last(kernel, dtype, table, k, v, H, n, new):
+    """Attention of the last ``new`` of n tokens of every sequence, with queries whose first entry is 1 and softmax scale 1."""
     from llmi_b200.engine.batch import StepContext, short_message
-    nats = 17.5
-    table, k, v = one_above(S, G, D, n, held, nats)
+    S, G, D = table.shape[0], k.codes.shape[1], k.codes.shape[3]
     cu = lambda a: torch.tensor(a, dtype=torch.int32, device="cuda")  # noqa: E731
     c = StepContext()
     c.tok_seq, c.tok_pos = cu([s for s in range(S) for _ in range(new)]), cu([p for s in range(S) for p in range(n - new, n)])
@@ -113,9 +103,45 @@ def test_one_key_far_above_many(kernel, dtype, S, G, H, D, n, new, held):
     out = torch.full((S * new, H * D), 7.0, dtype=DT[dtype], device="cuda")
     K().attention8(q.view(S * new, -1), out, k, v, c, table, H, G, D, 1.0, kernel=kernel)
     K().check_device_errors("cuda:0")
+    return out
+
+
+@pytest.mark.parametrize("kernel,dtype,S,G,H,D,n,new", [
+    # (a block for each sequence and kv head, and many blocks for one)
+    ("rows", "float32", 3, 32, 32, 64, 32000, 1), ("rows", "float32", 6, 16, 16, 128, 16000, 1), ("rows", "float32", 1, 1, 1, 64, 100000, 1),
+    ("rows", "bfloat16", 6, 32, 32, 64, 32000, 1), ("rows", "bfloat16", 12, 16, 16, 128, 16000, 1), ("rows", "bfloat16", 1, 1, 1, 64, 100000, 1),
+    ("prompt", "bfloat16", 3, 32, 32, 64, 32000, 3), ("prompt", "bfloat16", 6, 16, 32, 128, 16000, 20), ("prompt", "bfloat16", 1, 1, 1, 64, 100000, 200),
+    ("any", "float32", 1, 1, 1, 64, 100000, 3)])
+@pytest.mark.parametrize("held", ["int8", "float8_e4m3"])
+def test_one_key_far_above_many(kernel, dtype, S, G, H, D, n, new, held):
+    """One key 17.5 nats above tens of thousands, whose weights count together.
+
+    Tolerances: 2^-17 as elsewhere; a sum of n weights is n / 64 additions a thread or fewer, each rounded by 2^-24 of it; bf16: weights
+    and values are off by 2^-11 each, a weight far below the largest by 2^-32 of that, and the output by 2^-8."""
+    nats = 17.5
+    table, k, v = one_above(S, G, D, n, held, nats)
+    out = of_the_last(kernel, dtype, table, k, v, H, n, new)
     others = torch.arange(n - new, n, dtype=torch.float64) * np.exp(-nats)
     want = (others / (others + 1.0)).repeat(S)[:, None, None].repeat(1, H, D)
     want[..., 0] = 1.0 - want[..., 0]
     off = (out.double().cpu().view(-1, H, D) - want).abs()
-    tol = 2.0 ** -17 + n / 128 * 2.0 ** -24 * want + (2.0 ** -24 * want if dtype == "float32" else (2.0 ** -10 + 2.0 ** -8) * want + n * 2.0 ** -32)
+    tol = 2.0 ** -17 + n / 64 * 2.0 ** -24 * want + (2.0 ** -24 * want if dtype == "float32" else (2.0 ** -10 + 2.0 ** -8) * want + n * 2.0 ** -32)
     assert bool((off <= tol).all()), (float((off / tol).max()), float(off[..., 0].max()), float(off[..., 1:].max()))
+
+
+@pytest.mark.parametrize("kernel,dtype", [("rows", "float32"), ("rows", "bfloat16"), ("prompt", "bfloat16"), ("any", "float32")])
+@pytest.mark.parametrize("D", [64, 128])
+def test_many_values_near_the_least_that_there_are(kernel, dtype, D):
+    """100,000 values of 127 * 2^-107, next to what counts as zero, and weights that grow late by less than moves a running maximum: the sum
+    of weights relative to it stays a number of 32 bits.  All values are equal, so the output is that value; it is off by 2^-11 for each
+    of weights and values, 2^-8 or 2^-24 for the output, and n / 64 additions."""
+    k, n, G = K(), 100000, 2
+    P = -(-n // 64)
+    table = torch.randperm(P).to(torch.int32).view(1, P).cuda()
+    kk, vv = (k.Rows8(torch.full((P, G, 64, D), c, dtype=torch.int8, device="cuda"), torch.full((P, G, 64), s, device="cuda"))
+              for c, s in ((1, 0.0), (127, 2.0 ** -107)))
+    kk.scales[table[0, 1:].long()] = 7.9 * float(np.log(2.0))          # scores of 0 on the first page, 7.9 (to base 2) on the others
+    out = of_the_last(kernel, dtype, table, kk, vv, 2 * G, n, 40 if kernel == "prompt" else 1).double().cpu()
+    want = 127 * 2.0 ** -107
+    tol = (2.0 ** -10 + 2.0 ** -8 if dtype == "bfloat16" else 2.0 ** -17) + n / 64 * 2.0 ** -24
+    assert bool(((out - want).abs() <= tol * want).all()), (float(out.min() / want), float(out.max() / want))

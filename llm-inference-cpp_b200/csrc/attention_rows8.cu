@@ -38,7 +38,7 @@
 namespace llmi {
 
 constexpr int RW8_WARPS = 8;
-constexpr int RW8_MAX_ENTRIES = 4096;      // (sequence, row tile)s of a call
+constexpr int RW8_MAX_ENTRIES = 4096;      // (sequence, row tile)s of a call, and sequences
 constexpr float RW8_UP = 7.f;              // the largest weight is 2^7 where the reference maximum has moved
 constexpr float RW8_LAZY = 32768.f;        // weights up to 2^15 before it moves
 constexpr float RW8_SUM = 5.192296858534828e33f;   // 2^112: a sum of weights up to this (keys whose values are zeros may weigh that much)
@@ -56,18 +56,20 @@ struct Rows8Params {
   const int32_t* seq_q_start;   // [n_seqs + 1]
   const int32_t* seq_kv_len;    // [n_seqs]
   Paged8 kv;
-  int n_seqs, group, row_tiles;
+  int n_seqs, group;
+  int row_tiles;                // most row tiles of a sequence
   float scale_log2;
   int window;
   int q_f32;                    // q is fp32 (where out is bf16)
   float* slots;                 // [2 * blocks][SLOT]: partial results, of a block's first segment and of its last
-  int* whose;                   // [2 * blocks]: 0, or (its (entry, kv head) + 1) * 2 + whether it is the first of the parts
+  int* whose;                   // [2 * blocks]: 0, or (its (sequence, row tile, kv head) + 1) * 2 + whether it is the first of the parts
 };
 
 // D: head size; NT: eighths of query rows; T: the type of q and out (float: two fp16 numbers each).
 template <int D, int NT, typename T>
 struct Rw8Cfg {
   static constexpr int SP = std::is_same<T, float>::value ? 2 : 1;
+  static constexpr bool SEVERAL = NT == (SP == 2 ? 2 : 4) * 64 / D;      // a sequence may have several row tiles: rw8_tiles' widest
   static constexpr int KC = D == 64 && NT == 1 ? 32 : 16;          // keys of a chunk
   static constexpr int CPP = PAGE8 / KC;           // chunks of a page
   static constexpr int MT = KC / 16, KS = D / 16;  // key tiles of a chunk; 16-dim steps of a row
@@ -104,14 +106,14 @@ struct Rw8Cut {
   int front, most_whole, least, near;
 };
 
-// One (sequence, row tile): its rows and the pages that they see.
+// One (sequence, row tile), number sequence * row_tiles + tile: its rows and the pages that they see.
 struct Rw8Entry {
   int seq, q_start, row0, rows, pos0, last, lo, pg_first, n_pages;
 };
-__device__ __forceinline__ Rw8Entry rw8_entry(const Rows8Params& p, int e, int tile_rows) {
+__device__ __forceinline__ Rw8Entry rw8_entry(const Rows8Params& p, int number, int tile_rows) {
   Rw8Entry d;
-  d.seq = e / p.row_tiles;
-  d.row0 = (e - d.seq * p.row_tiles) * tile_rows;
+  d.seq = number / p.row_tiles;
+  d.row0 = (number - d.seq * p.row_tiles) * tile_rows;
   d.q_start = p.seq_q_start[d.seq];
   const int q_len = p.seq_q_start[d.seq + 1] - d.q_start, kv_len = p.seq_kv_len[d.seq];
   d.rows = min(tile_rows, q_len * p.group - d.row0);
@@ -201,23 +203,40 @@ __global__ void __launch_bounds__(RW8_WARPS * 32, (Rw8Cfg<D, NT, T>::BLOCKS)) at
   pdl_launch_dependents();
   // (ahead of the wait: the step's index block only, and the page table in it)
 
-  // ---- the line of units: units ahead of each entry ----
+  // ---- entries: where a sequence may have several row tiles, those that there are, one sequence behind the other (how many each has is
+  // known here only); else a sequence each.  The line of units: units ahead of each entry ----
+  uint16_t* starts = reinterpret_cast<uint16_t*>(prefix + n_entries + 1);      // [n_seqs + 1] tiles ahead of a sequence (where row_tiles > 1)
+  auto last_before = [](const auto* ahead, int n, int x) {      // the i with ahead[i] <= x < ahead[i + 1] (the last one if x is behind all)
+    int a = 0, b = n;
+    while (b - a > 1) {
+      const int m = (a + b) >> 1;
+      if (ahead[m] <= x) a = m;
+      else b = m;
+    }
+    return a;
+  };
+  auto number_of = [&](int e) {            // of an entry, as rw8_entry takes it (-1: there are fewer)
+    if (!C::SEVERAL || p.row_tiles == 1) return e;
+    if (e >= starts[p.n_seqs]) return -1;
+    const int seq = last_before(starts, p.n_seqs, e);
+    return seq * p.row_tiles + e - starts[seq];
+  };
   int pairs = 0, longest = 0;              // (entry, kv head)s that have pages; the most pages of one
-  {
+  auto line_up = [&](auto* into, int count, auto of) {          // into[i] = the sum of `of` (number, pages) over all ahead of i
+    constexpr int MOST = sizeof(*into) == 2 ? 0xffff : 0x7fffffff;
     int carry = 0;
-    for (int e0 = 0; e0 < n_entries; e0 += RW8_WARPS * 32) {
-      const int e = e0 + threadIdx.x;
-      const int pages = e < n_entries ? rw8_entry(p, e, 8 * NT).n_pages : 0;
-      const int n = pages > 0 ? (pages + cut.front) * Hkv : 0;
-      int x = n;
+    for (int i0 = 0; i0 < count; i0 += RW8_WARPS * 32) {
+      const int i = i0 + threadIdx.x;
+      const int2 mine = i < count ? of(i) : make_int2(0, 0);
+      int x = mine.x;
 #pragma unroll
       for (int o = 1; o < 32; o <<= 1) {
         const int y = __shfl_up_sync(0xffffffffu, x, o);
         if (lane >= o) x += y;
       }
-      const int top = __reduce_max_sync(0xffffffffu, pages);
+      const int top = __reduce_max_sync(0xffffffffu, mine.y);
       if (lane == 31) s_scan[warp] = x, s_top[warp] = top;
-      pairs += __syncthreads_count(n > 0) * Hkv;
+      pairs += __syncthreads_count(mine.y > 0) * Hkv;
       int before = carry, all = carry;
 #pragma unroll
       for (int w = 0; w < RW8_WARPS; ++w) {
@@ -225,13 +244,22 @@ __global__ void __launch_bounds__(RW8_WARPS * 32, (Rw8Cfg<D, NT, T>::BLOCKS)) at
         all += s_scan[w];
         longest = max(longest, s_top[w]);
       }
-      if (e < n_entries) prefix[e] = before + x - n;
+      if (i < count) into[i] = min(before + x - mine.x, MOST);
       carry = all;
       __syncthreads();
     }
-    if (threadIdx.x == 0) prefix[n_entries] = carry;
+    if (threadIdx.x == 0) into[count] = min(carry, MOST);
     __syncthreads();
-  }
+  };
+  if (C::SEVERAL && p.row_tiles > 1)
+    line_up(starts, p.n_seqs, [&](int seq) {
+      const int rows = (p.seq_q_start[seq + 1] - p.seq_q_start[seq]) * G;
+      return make_int2(p.seq_kv_len[seq] > 0 && rows > 0 ? min((rows + 8 * NT - 1) / (8 * NT), p.row_tiles) : 0, 0);
+    });
+  line_up(prefix, n_entries, [&](int e) {
+    const int number = number_of(e), pages = number < 0 ? 0 : rw8_entry(p, number, 8 * NT).n_pages;
+    return make_int2(pages > 0 ? (pages + cut.front) * Hkv : 0, pages);
+  });
   const int total = prefix[n_entries];
   // each its own block, or the line in even ranges
   const bool whole = pairs <= (int)gridDim.x && (longest <= cut.most_whole || (5 * pairs >= 3 * (int)gridDim.x && (long)(longest + cut.front) * pairs <= total + total / 4));
@@ -242,15 +270,7 @@ __global__ void __launch_bounds__(RW8_WARPS * 32, (Rw8Cfg<D, NT, T>::BLOCKS)) at
     return;
   }
   const int per = total / blocks, longer = total - per * blocks;      // even ranges: the first `longer` have per + 1 units
-  auto find_entry = [&](int unit) {        // the entry that has the unit (the last one if they are all before it)
-    int a = 0, b = n_entries;              // prefix[a] <= unit < prefix[b]
-    while (b - a > 1) {
-      const int m = (a + b) >> 1;
-      if (prefix[m] <= unit) a = m;
-      else b = m;
-    }
-    return a;
-  };
+  auto find_entry = [&](int unit) { return last_before(prefix, n_entries, unit); };
   const int near = min(cut.near, per / 2);
   auto range_start = [&](int c) {          // an even cut, moved to the border of two (entry, kv head)s that is near
     const int u = c * per + min(c, longer);
@@ -283,13 +303,14 @@ __global__ void __launch_bounds__(RW8_WARPS * 32, (Rw8Cfg<D, NT, T>::BLOCKS)) at
   // the block's part of the (entry, kv head) that has unit `at`, from there on
   struct Segment {
     Rw8Entry d;
-    int kvh, begin, end;                   // all units of the (entry, kv head)
+    int number, kvh, begin, end;           // all units of the (entry, kv head)
     int first, n;                          // of its pages: the block's first, and how many
   };
   auto segment_at = [&](int at, int& e) {
     while (prefix[e + 1] <= at) ++e;
     Segment s;
-    s.d = rw8_entry(p, e, 8 * NT);
+    s.number = number_of(e);
+    s.d = rw8_entry(p, s.number, 8 * NT);
     const int len = s.d.n_pages + cut.front;
     s.kvh = (at - prefix[e]) / len;
     s.begin = prefix[e] + s.kvh * len;
@@ -681,7 +702,7 @@ __global__ void __launch_bounds__(RW8_WARPS * 32, (Rw8Cfg<D, NT, T>::BLOCKS)) at
     const int part = u0 < s.begin ? 1 : 0;
     float* my_slot = p.slots + (size_t)(2 * blockIdx.x + part) * C::SLOT;
     if (shared_out) {
-      const int id = ((e * Hkv + kvh + 1) << 1) | (s.first == 0 ? 1 : 0);
+      const int id = ((s.number * Hkv + kvh + 1) << 1) | (s.first == 0 ? 1 : 0);
       if (part) mine[1] = id;
       else mine[0] = id;
     }
@@ -723,8 +744,8 @@ template <int D, int NT, typename T> __global__ void __launch_bounds__(RW8_WARPS
     if (other) break;
     next = p.whose[2 * min(z0 + 32 + lane, last)];
   }
-  const int pair_id = (id >> 1) - 1, e = pair_id / p.kv.n_kv_heads, kvh = pair_id - e * p.kv.n_kv_heads;
-  const Rw8Entry d = rw8_entry(p, e, 8 * NT);
+  const int pair_id = (id >> 1) - 1, number = pair_id / p.kv.n_kv_heads, kvh = pair_id - number * p.kv.n_kv_heads;
+  const Rw8Entry d = rw8_entry(p, number, 8 * NT);
   for (int pair = warp / SHARE; pair < C::PAIRS; pair += RW8_WARPS / SHARE) {
     Rw8Tile r = rw8_gather<C, NT>(pair, warp % SHARE, n_parts, SHARE,
                                   [&](int z) { return (const float*)(p.slots + (size_t)(2 * (c + z) + (z == 0 ? which : 0)) * C::SLOT); },
@@ -757,11 +778,11 @@ template <int D, int NT, int HELD, typename T> int launch_rows8(const Rows8Param
   constexpr auto kernel = attention_rows8_kernel<D, NT, HELD, T>;
   static PerDevice<bool> configured;
   if (!configured.here()) {
-    if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, C::RING + C::MERGE + 4 * (RW8_MAX_ENTRIES + 1)) != cudaSuccess)
+    if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, C::RING + C::MERGE + 6 * (RW8_MAX_ENTRIES + 1)) != cudaSuccess)
       return LLMI_ERR_LAUNCH;
     configured.here() = true;
   }
-  const size_t smem = C::RING + C::MERGE + 4 * ((size_t)n_entries + 1);
+  const size_t smem = C::RING + C::MERGE + 4 * ((size_t)n_entries + 1) + (p.row_tiles > 1 ? 2 * ((size_t)p.n_seqs + 1) : 0);
   // no more blocks than are resident: many entries' table may leave room for one a SM only (228 KB; a block's own 1 KB and its statics)
   const int fit = (int)((228 << 10) / (smem + 1280));
   grid = min(grid, min(C::BLOCKS, max(1, fit)) * sm_count());
@@ -777,43 +798,50 @@ inline int rw8_tiles(int dtype, int D, long rows) {
   if (dtype == LLMI_DTYPE_F32) return rows <= 8 || D == 128 ? 1 : 2;
   return rows <= 8 ? 1 : (rows <= 16 || D == 128) ? 2 : 4;
 }
+// Row tiles that a sequence of `max_q` tokens has; entries that a call has at most: the tiles of all sequences, each of which may leave
+// its last one all but empty, or (one tile a sequence) a sequence each.
+inline long rw8_row_tiles(int nt, int max_q, int group) { return ((long)max_q * group + 8 * nt - 1) / (8 * nt); }
+inline long rw8_entries(int nt, int n_tokens, int n_seqs, long tiles, int group) {
+  const long all = n_seqs * tiles, there = ((long)n_tokens * group + (8L * nt - 1) * n_seqs) / (8 * nt);
+  return tiles == 1 || all < there ? all : there;
+}
 inline int rw8_grid(long units) { return (int)(units < 2L * sm_count() ? units : 2L * sm_count()); }
 
 }  // namespace llmi
 
 using namespace llmi;
 
-// The floats of scratch for the blocks' partial results (of any content); below 0: the sizes are not taken.  `max_q`: most tokens that a
-// sequence brings.
-LLMI_EXPORT long llmi_attention_rows8_workspace(int dtype, int n_seqs, int max_q, int n_heads, int n_kv_heads, int head_dim, int table_pages) {
-  if (n_seqs <= 0 || max_q <= 0 || n_kv_heads <= 0 || n_heads <= 0 || n_heads % n_kv_heads || (head_dim != 64 && head_dim != 128) || table_pages <= 0)
+// The floats of scratch for the blocks' partial results (of any content); below 0: the sizes are not taken.  `n_tokens`: at least those of
+// all sequences; `max_q`: most tokens that a sequence brings.
+LLMI_EXPORT long llmi_attention_rows8_workspace(int dtype, int n_tokens, int n_seqs, int max_q, int n_heads, int n_kv_heads, int head_dim, int table_pages) {
+  if (n_tokens <= 0 || n_seqs <= 0 || max_q <= 0 || n_kv_heads <= 0 || n_heads <= 0 || n_heads % n_kv_heads || (head_dim != 64 && head_dim != 128) || table_pages <= 0)
     return LLMI_ERR_BAD_SIZE;
-  const long rows = (long)max_q * (n_heads / n_kv_heads);
-  const int nt = rw8_tiles(dtype, head_dim, rows);
-  const long tiles = (rows + 8 * nt - 1) / (8 * nt);
-  if (n_seqs * tiles > RW8_MAX_ENTRIES || n_seqs * tiles * n_kv_heads * ((long)table_pages + 64) > 0x7fffffffL) return LLMI_ERR_BAD_SIZE;
-  return 2L * rw8_grid(n_seqs * tiles * n_kv_heads * (long)table_pages) * (head_dim / 16 * nt * 128 + 16 * nt + 1);
+  const int group = n_heads / n_kv_heads, nt = rw8_tiles(dtype, head_dim, (long)max_q * group);
+  const long tiles = rw8_row_tiles(nt, max_q, group), entries = rw8_entries(nt, n_tokens, n_seqs, tiles, group);
+  if (entries > RW8_MAX_ENTRIES || n_seqs > RW8_MAX_ENTRIES || n_seqs * tiles * n_kv_heads > 0x3ffffff0L ||
+      entries * n_kv_heads * ((long)table_pages + 64) > 0x7fffffffL)
+    return LLMI_ERR_BAD_SIZE;
+  return 2L * rw8_grid(entries * n_kv_heads * (long)table_pages) * (head_dim / 16 * nt * 128 + 16 * nt + 1);
 }
 
 LLMI_EXPORT int llmi_attention_rows8(int dtype, int held, const void* q, long ldq, void* out, long ldo, const void* k_codes, const float* k_scales,
                                      const void* v_codes, const float* v_scales, const int32_t* seq_q_start, const int32_t* seq_kv_len,
-                                     const int32_t* seq_pages, int pages_stride, int table_pages, int n_seqs, int n_pages, int max_q,
-                                     int n_heads, int n_kv_heads, int head_dim, float scale, int window, int q_f32, float* slots, long n_floats,
+                                     const int32_t* seq_pages, int pages_stride, int table_pages, int n_seqs, int n_pages, int n_tokens,
+                                     int max_q, int n_heads, int n_kv_heads, int head_dim, float scale, int window, int q_f32, float* slots, long n_floats,
                                      cudaStream_t stream) {
   if (dtype != LLMI_DTYPE_F32 && dtype != LLMI_DTYPE_BF16) return LLMI_ERR_BAD_DTYPE;
-  const long floats = llmi_attention_rows8_workspace(dtype, n_seqs, max_q, n_heads, n_kv_heads, head_dim, table_pages);
+  const long floats = llmi_attention_rows8_workspace(dtype, n_tokens, n_seqs, max_q, n_heads, n_kv_heads, head_dim, table_pages);
   if (floats < 0 || n_floats < floats || n_pages <= 0 || window < 0) return LLMI_ERR_BAD_SIZE;
   if (held != HELD_INT8 && held != HELD_E4M3) return LLMI_ERR_BAD_DTYPE;
   const long even = dtype == LLMI_DTYPE_F32 ? 3 : 7;         // rows are whole 16-byte pieces
   if ((((uintptr_t)q | (uintptr_t)out | (uintptr_t)k_codes | (uintptr_t)v_codes | (uintptr_t)k_scales | (uintptr_t)v_scales) & 15) || (ldq & (q_f32 ? 3 : even)) || (ldo & even))
     return LLMI_ERR_ALIGN;
   const int group = n_heads / n_kv_heads;
-  const long rows = (long)max_q * group;
-  const int nt = rw8_tiles(dtype, head_dim, rows), tiles = (int)((rows + 8 * nt - 1) / (8 * nt));
+  const int nt = rw8_tiles(dtype, head_dim, (long)max_q * group), tiles = (int)rw8_row_tiles(nt, max_q, group);
   Rows8Params p{q, ldq, out, ldo, (const uint8_t*)k_codes, k_scales, (const uint8_t*)v_codes, v_scales,
                 seq_q_start, seq_kv_len, Paged8{seq_pages, pages_stride, table_pages, n_pages, n_kv_heads, head_dim}, n_seqs, group, tiles,
                 scale * 1.4426950408889634f, window, q_f32, slots, nullptr};
-  const int n_entries = n_seqs * tiles, grid = rw8_grid((long)n_entries * n_kv_heads * table_pages);
+  const int n_entries = (int)rw8_entries(nt, n_tokens, n_seqs, tiles, group), grid = rw8_grid((long)n_entries * n_kv_heads * table_pages);
   p.whose = reinterpret_cast<int*>(slots + 2L * grid * (head_dim / 16 * nt * 128 + 16 * nt));
   // most pages that a (sequence, kv head)'s rows of a tile see
   const long seen = ((long)window + max_q) / PAGE8 + 2;

@@ -190,7 +190,7 @@ def lib():
         l.llmi_attention_prefill_tc.argtypes = [P, L, L, P, L, P, P, L, P, I, P, P, I, I, I, I, I, F, I, I, I, P, L, P, I, P, I, P, P, L, P, I, P, L, P, P, P, I, I, I, P, P]
         l.llmi_rope_store8.argtypes = [I, I, P, L, P, L, P, I, P, P, P, I, I, I, P, P, P, P, I, I, I, I, I, I, I, P]
         l.llmi_attention_any8.argtypes = [I, I, P, L, P, L, P, P, P, P, P, P, P, I, I, I, I, I, I, I, I, F, I, I, P]
-        l.llmi_attention_rows8.argtypes = [I, I, P, L, P, L, P, P, P, P, P, P, P, I, I, I, I, I, I, I, I, F, I, I, P, L, P]
+        l.llmi_attention_rows8.argtypes = [I, I, P, L, P, L, P, P, P, P, P, P, P, I, I, I, I, I, I, I, I, I, F, I, I, P, L, P]
         l.llmi_attention_prompt8.argtypes = [I, P, L, P, L, P, P, P, P, P, P, P, I, I, I, I, I, I, I, I, F, I, I, I, I, P, L, P, P]
         _configured = True
     return l
@@ -2223,9 +2223,9 @@ def _rope_store8(held: int, qkv, q_out: int, ldq: int, q_f32: bool, inv_freq, ro
 _sizes8: dict = {}
 
 
-def _rows8_floats(dtype: int, n_seqs: int, max_q: int, n_heads: int, n_kv_heads: int, head_dim: int, table_pages: int) -> int:
+def _rows8_floats(dtype: int, n_tokens: int, n_seqs: int, max_q: int, n_heads: int, n_kv_heads: int, head_dim: int, table_pages: int) -> int:
     """The fp32 numbers of scratch that the kernel for few rows needs, below 0 where it does not take the sizes."""
-    key = (dtype, n_seqs, max_q, n_heads, n_kv_heads, head_dim, table_pages)
+    key = (dtype, n_tokens, n_seqs, max_q, n_heads, n_kv_heads, head_dim, table_pages)
     n = _sizes8.get(key)
     if n is None:
         if len(_sizes8) >= 4096:
@@ -2305,7 +2305,7 @@ def attention8(q: torch.Tensor, out: torch.Tensor, k: Rows8, v: Rows8, ctx, seq_
             and ldq % (4 if q_f32 else 8) == 0 and ldo % (8 if dtype == 1 else 4) == 0)
     max_q = 1 if ctx.decode else _most_new(ctx)
     n_blocks = (T * group + 255 * S) // 256
-    few = _rows8_floats(dtype, S, max_q, n_heads, n_kv_heads, head_dim, P) if kernel in (None, "rows") and fast else -1
+    few = _rows8_floats(dtype, T, S, max_q, n_heads, n_kv_heads, head_dim, P) if kernel in (None, "rows") and fast else -1
     prompt = kernel in (None, "prompt") and fast and dtype == 1 and n_blocks <= 65535 and (few < 0 or max_q * group > _ROWS8_MOST)
     if not prompt and few < 0 and kernel not in (None, "any"):
         raise KernelError(f"{name}: the kernel {kernel!r} does not take this call")
@@ -2328,7 +2328,7 @@ def attention8(q: torch.Tensor, out: torch.Tensor, k: Rows8, v: Rows8, ctx, seq_
             at_scratch + 4 * n_q if parts > 1 else None, floats, tc_scratch(q.device).error.data_ptr(), stream))
     elif few >= 0:
         _check("attention_rows8", lib().llmi_attention_rows8(
-            dtype, *rows, start, kv_len, *table, max_q, n_heads, n_kv_heads, head_dim, scale, window, q_f32, at_scratch + 4 * n_q, floats, stream))
+            dtype, *rows, start, kv_len, *table, T, max_q, n_heads, n_kv_heads, head_dim, scale, window, q_f32, at_scratch + 4 * n_q, floats, stream))
     else:
         seq, pos = _index8(name, "tok_seq", ctx.tok_seq, T, device), _index8(name, "tok_pos", ctx.tok_pos, T, device)
         _check("attention_any8", lib().llmi_attention_any8(dtype, *rows, seq, pos, *table, T, n_heads, n_kv_heads, head_dim, scale, window, q_f32, stream))

@@ -2235,6 +2235,14 @@ def _rows8_floats(dtype: int, n_tokens: int, n_seqs: int, max_q: int, n_heads: i
 
 
 _PROMPT8_PART_PAGES = 4       # the least pages of a part of a block of 256 query rows
+
+
+def _prompt8_pages(table_pages: int, window: int, group: int, max_q: int) -> int:
+    """Most pages that a block of 256 query rows sees: under a window, those of its tokens' positions and of the window before them."""
+    tokens = min(max_q, 255 // group + 2)        # (a block may start and end within a token's heads)
+    return min(table_pages, (window + tokens - 3) // 64 + 2) if window > 0 else table_pages
+
+
 # Query rows of a kv head up to which the kernel for few rows takes a step, its largest tile (rows / prompt kernel, us, at 32 and 48
 # rows: 64 sequences of 200 to 4,000 positions, 32 heads by 8 of 128: 126 / 156 and 176 / 159; one of 30,000: 42 / 46 and 52 / 48;
 # eight of 500 to 3,000, 32 heads of 64: 52 / 66 and 71 / 67).
@@ -2244,6 +2252,7 @@ _ROWS8_MOST = 32
 @functools.lru_cache(maxsize=4096)
 def prompt8_parts(n_rows: int, n_kv_heads: int, head_dim: int, n_seqs: int, table_pages: int, max_q: int, sms: int) -> int:
     """In how many parts at most the prompt kernel of 8-bit rows cuts the pages of a block of 256 query rows, with one block a SM.
+    ``table_pages``: the most pages that a block sees.
     Blocks of whole prompts differ in their pages and start with the longest, so that a wave of them fills the device evenly; blocks
     of a message behind a long history all see nearly all of it, and are cut so that the device is busy and done soonest.
 
@@ -2309,7 +2318,7 @@ def attention8(q: torch.Tensor, out: torch.Tensor, k: Rows8, v: Rows8, ctx, seq_
     prompt = kernel in (None, "prompt") and fast and dtype == 1 and n_blocks <= 65535 and (few < 0 or max_q * group > _ROWS8_MOST)
     if not prompt and few < 0 and kernel not in (None, "any"):
         raise KernelError(f"{name}: the kernel {kernel!r} does not take this call")
-    parts = prompt8_parts(T * group, n_kv_heads, head_dim, S, P, max_q, sm_count()) if prompt else 1
+    parts = prompt8_parts(T * group, n_kv_heads, head_dim, S, _prompt8_pages(P, window, group, max_q), max_q, sm_count()) if prompt else 1
     floats = (n_blocks * n_kv_heads * parts * 256 * (head_dim + 2) if parts > 1 else 0) if prompt else max(few, 0)
     scratch = None
     if n_q + floats:

@@ -2130,6 +2130,7 @@ def softcap_rows(v: torch.Tensor, cap: float) -> None:
 #
 # These launchers run between two kernels of a few microseconds each, so what they check and collect is asked of every tensor once.
 
+ROWS8_MOST_DIM = 256          # the largest head size
 _HELD_CODE = {torch.int8: 0, torch.float8_e4m3fn: 1}
 _DTYPE8 = {torch.float32: 0, torch.bfloat16: 1}
 _current_device = torch._C._cuda_getDevice if hasattr(torch._C, "_cuda_getDevice") else torch.cuda.current_device
@@ -2156,8 +2157,8 @@ def _check8(name: str, x: torch.Tensor, k: Rows8, v: Rows8, seq_pages, n_heads: 
         raise KernelError(f"{name}: keys and values are held in int8 or float8_e4m3fn, both in one of them")
     if n_heads < 1 or n_kv_heads < 1 or n_heads % n_kv_heads != 0:
         raise KernelError(f"{name}: n_heads must be a multiple of n_kv_heads")
-    if not 1 <= head_dim <= 256:
-        raise KernelError(f"{name}: head_dim must be 1 to 256")
+    if not 1 <= head_dim <= ROWS8_MOST_DIM:
+        raise KernelError(f"{name}: head_dim must be 1 to {ROWS8_MOST_DIM}")
     shape = kc.shape
     if vc.shape != shape or len(shape) != 4 or shape[0] < 1 or shape[1] != n_kv_heads or shape[2] != 64 or shape[3] != head_dim:
         raise KernelError(f"{name}: codes must be [pages, n_kv_heads, 64, head_dim]")

@@ -57,8 +57,9 @@ class GQAttention:
 
     @property
     def holds_8bit(self) -> bool:
-        """Whether the cache may hold keys and values in 8 bits: if all the position part does is the rotation of pairs."""
-        return self.position.fused_rotation() is not None
+        """Whether the cache may hold keys and values in 8 bits: if all the position part does is the rotation of pairs, and the heads are of
+        a size that the kernels take."""
+        return self.position.fused_rotation() is not None and self.head_dim <= kernels.ROWS8_MOST_DIM
 
     def weight_bytes(self) -> int:
         return sum(t.numel() * t.element_size() for t in (self.w_qkv, self.w_o))

@@ -1,4 +1,4 @@
-"""How a step over a cache held in 8 bits is laid out for the prompt kernel (no GPU)."""
+"""How a step over a cache held in 8 bits is laid out for the prompt kernel, and which heads such a cache is offered for (no GPU)."""
 import numpy as np
 
 from llmi_b200.ops.kernels import _prompt8_pages, prompt8_parts
@@ -52,3 +52,12 @@ def test_attention_plans_with_the_window(monkeypatch):
         except Stop:
             pass
     assert [a[4] for a in asked] == [500, _prompt8_pages(500, 512, 4, 300)]
+
+
+def test_heads_that_the_kernels_do_not_take_get_no_such_cache():
+    """Refused where the cache is made, not in its first step."""
+    import types
+
+    from llmi_b200.parts.attention import GQAttention
+    position = types.SimpleNamespace(fused_rotation=lambda: (None, 0))
+    assert [GQAttention.holds_8bit.fget(types.SimpleNamespace(position=position, head_dim=d)) for d in (64, 256, 257, 320)] == [True, True, False, False]

@@ -1,4 +1,4 @@
-"""Attention over a cache held in 8 bits by the kernel for few rows: steps of several prompts (GPU)."""
+"""Attention over a cache held in 8 bits by the kernel for few rows: steps of several prompts, long histories (GPU)."""
 import pytest
 import torch
 
@@ -28,4 +28,16 @@ def test_steps_of_several_prompts(dtype, H, G, D, step):
     b = Batch(PROMPTS[step], G, D, "int8", seed=6, pad_tokens=3)
     b.fill()
     q = torch.tensor(b.rng.normal(size=(b.T, H * D)) * 1.5).to(DT[dtype]).cuda()
+    check(b, H, q, by_rows(b, H, q, dtype), dtype)
+
+
+@pytest.mark.parametrize("dtype,H,G,D,step", [("bfloat16", 16, 1, 64, [(1, 100001)]), ("bfloat16", 4, 1, 128, [(3, 20011)]), ("float32", 6, 1, 64, [(1, 100001)]),
+                                              ("float32", 4, 2, 128, [(1, 30000), (2, 100)]), ("bfloat16", 9, 3, 64, [(1, 60001), (1, 7), (2, 30000)])])
+@pytest.mark.parametrize("size", [1.0, 12.0])
+def test_long_histories(dtype, H, G, D, step, size):
+    """A (sequence, kv head) in up to 200 parts, which are joined 32 and 8 at a time; with scores of ordinary size, and of 12 times that:
+    parts whose maxima are far apart."""
+    b = Batch(step, G, D, "int8", seed=8)
+    b.fill()
+    q = torch.tensor(b.rng.normal(size=(b.T, H * D)) * size).to(DT[dtype]).cuda()
     check(b, H, q, by_rows(b, H, q, dtype), dtype)

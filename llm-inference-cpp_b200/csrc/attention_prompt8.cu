@@ -15,8 +15,9 @@
 //                 log2 vmax its offset.  (A page whose scales are more than 2^12 apart would lose bits of its small rows, which may be
 //                 all that a query sees: there K' and V' are the codes themselves and the softmax takes each key's scales.)
 //   S = Q' K'^T   tcgen05.mma, Q' the queries times a power of two per row that brings its largest near 2^15, in fp16: bf16 queries
-//                 exactly, down to 2^-29 of the row's largest entry; 32-bit ones (those that `rope` makes) rounded to 11 bits, which
-//                 costs a score no more than what the keys' rounding costs it
+//                 exactly, down to 2^-29 of the row's largest entry; 32-bit ones (those that `rope` makes, which every layer of a
+//                 model passes) rounded to 11 bits, as the keys are: kept as two fp16 numbers they would double the products, for an
+//                 output that is rounded to bf16
 //   softmax       two threads own a row, 32 keys of a page each: tcgen05.ld, mask, maximum, exp2, sum; P = 2^(s + log2 vmax - m) goes
 //                 back to tensor memory as fp16 over the S it has read; the sum of w is that of P / vmax
 //   O += P V'     tcgen05.mma with A in tensor memory, accumulating in fp32; m lies 7 below the running maximum (of s + log2 vmax)

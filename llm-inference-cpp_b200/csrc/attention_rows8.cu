@@ -4,7 +4,7 @@
 // (reference loop: src/model/transformer.cpp:263-282).  Every code is read once and takes part in a handful of operations, so what
 // bounds the kernel is HBM: 2 (D + 4) bytes a position and kv head; behind that the instructions that make codes fp16 numbers, and
 // the join.  Measured: 8 x 4,096 positions of 32 heads of 64 30 us with the append (4.7 TB/s), 60,001 to 131,071 positions of three
-// sequences 41 us (4.5), 64 of 200 to 4,400, 32 heads by 8 of 128, 47 us (4.0); a copy reaches 6.5.
+// sequences 41 us (4.5), 64 of 200 to 4,400, 32 heads by 8 of 128, 46 us (4.0); a copy reaches 6.5.
 //
 //  * All pages that the step's rows see, kv head by kv head and sequence by sequence, are one line of units (a unit: one page of one
 //    kv head), cut into as many equal ranges as there are blocks resident on the device.  A block works through its range whatever

@@ -102,7 +102,7 @@ template <int HELD> __device__ __forceinline__ void halves8x4(uint32_t w, uint32
   }
 }
 
-// A sum of weights relative to a maximum that is `down` >= 0 below the new one (base 2).  In two steps: the maxima are those of score +
+// A sum of weights relative to a maximum, relative to a new one: times 2^down, `down` the old maximum less the new one, at most 0.  In two steps: the maxima are those of score +
 // log2 of a value's scale, so the factor alone may be below what fp32 has where the sum times it is not.
 __device__ __forceinline__ float rescale8(float sum, float down) {
   const float h = fast_exp2(0.5f * down);

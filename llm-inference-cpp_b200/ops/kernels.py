@@ -2244,8 +2244,8 @@ def _prompt8_pages(table_pages: int, window: int, group: int, max_q: int) -> int
     return min(table_pages, (window + tokens - 3) // 64 + 2) if window > 0 else table_pages
 
 
-# Query rows of a kv head up to which the kernel for few rows takes a step, its largest tile (rows / prompt kernel, us, at 32 and 48
-# rows: 64 sequences of 200 to 4,000 positions, 32 heads by 8 of 128: 126 / 156 and 176 / 159; one of 30,000: 42 / 46 and 52 / 48;
+# Query rows of a kv head up to which the kernel for few rows takes a step: its largest tile at head size 64, two tiles at 128 (rows /
+# prompt kernel, us, at 32 and 48 rows: 64 sequences of 200 to 4,000 positions, 32 heads by 8 of 128: 126 / 156 and 176 / 159; one of 30,000: 42 / 46 and 52 / 48;
 # eight of 500 to 3,000, 32 heads of 64: 52 / 66 and 71 / 67).
 _ROWS8_MOST = 32
 

@@ -138,7 +138,7 @@ __global__ void __launch_bounds__(ANY8_WARPS * 32) attention_any8_kernel(Any8Par
     float x = 0.f;
 #pragma unroll
     for (int w = 0; w < ANY8_WARPS; ++w) x = fmaf(s_acc[w][d], expf(s_m[w] - top), x);
-    o[d] = from_f32<T>(sum == 0.f ? 0.f : x / sum);
+    o[d] = from_f32<T>(x / sum);                  // (scores that are all -infinity: NaN)
   }
 }
 

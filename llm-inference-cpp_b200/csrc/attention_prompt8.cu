@@ -637,8 +637,8 @@ __global__ void __launch_bounds__(P8_THREADS, 1) attention_prompt8_kernel(Prompt
             if (row_ok) *reinterpret_cast<float4*>(dst + c + e) = make_float4(o[e], o[e + 1], o[e + 2], o[e + 3]);
         }
       } else {
-        // (without a page, or with weights that are all zero, the row sees nothing)
-        const float inv = l_all == 0.f ? 0.f : 1.f / l_all;
+        // (a position below 0 sees nothing: zeros; scores that are all -infinity: NaN)
+        const float inv = qpos < 0 ? 0.f : 1.f / l_all;
         __nv_bfloat16* dst = p.out + (size_t)(d.q_start + tok) * p.ldo + (size_t)head * D + HD * half;
 #pragma unroll 1
         for (int c = 0; c < HD; c += 16) {
@@ -782,7 +782,7 @@ __global__ void __launch_bounds__(256) prompt8_join_kernel(Prompt8Params p) {
       }
     }
     const int row = d.row0 + r;
-    const float inv = l == 0.f ? 0.f : 1.f / l;
+    const float inv = d.pos0 + row / G < 0 ? 0.f : 1.f / l;
     __nv_bfloat162* dst = reinterpret_cast<__nv_bfloat162*>(p.out + (size_t)(d.q_start + row / G) * p.ldo + (size_t)(kvh * G + row % G) * D);
 #pragma unroll
     for (int c = 0; c < D / 64; ++c) dst[lane + 32 * c] = __floats2bfloat162_rn(o[c].x * inv, o[c].y * inv);

@@ -183,7 +183,8 @@ __device__ __forceinline__ void rw8_write(const Rows8Params& p, const Rw8Entry& 
     const int r8 = (pair % NT) * 8 + 2 * t + j;
     if (r8 >= d.rows) continue;
     const int row = d.row0 + r8;
-    const float inv = r.l[j] == 0.f ? 0.f : 1.f / r.l[j];
+    // (a position below 0 sees nothing: zeros; scores that are all -infinity: NaN)
+    const float inv = d.pos0 + row / G < 0 ? 0.f : 1.f / r.l[j];
     T* at = (T*)p.out + (size_t)(d.q_start + row / G) * p.ldo + (size_t)(kvh * G + row % G) * D + g * (D / 8) + 2 * (pair / NT);
     if (sizeof(T) == 4) *reinterpret_cast<float2*>(at) = make_float2(r.o[j] * inv, r.o[j + 2] * inv);
     else *reinterpret_cast<__nv_bfloat162*>(at) = __floats2bfloat162_rn(r.o[j] * inv, r.o[j + 2] * inv);

@@ -1,5 +1,6 @@
 """Attention over a cache held in 8 bits where numbers are far apart or small: factors of a page's scores that underflow,
-queries far below 1 and with one entry far above the others, a weight far above many (GPU)."""
+queries far below 1 and with one entry far above the others, a weight far above many,
+queries that are no numbers (GPU)."""
 import numpy as np
 import pytest
 import torch
@@ -145,3 +146,26 @@ def test_many_values_near_the_least_that_there_are(kernel, dtype, D):
     want = 127 * 2.0 ** -107
     tol = (2.0 ** -10 + 2.0 ** -8 if dtype == "bfloat16" else 2.0 ** -17) + n / 64 * 2.0 ** -24
     assert bool(((out - want).abs() <= tol * want).all()), (float(out.min() / want), float(out.max() / want))
+
+
+@pytest.mark.parametrize("kernel,dtype", [("rows", "bfloat16"), ("prompt", "bfloat16"), ("any", "bfloat16"), ("rows", "float32")])
+@pytest.mark.parametrize("H,G,D,step", [(4, 2, 64, "prompts"), (8, 2, 128, "messages"), (4, 4, 128, "single tokens")])
+@pytest.mark.parametrize("bad", [float("nan"), float("inf"), -float("inf")])
+def test_queries_that_are_not_finite_reach_only_their_rows(kernel, dtype, H, G, D, step, bad):
+    """They are NaN, as a softmax over infinite scores is; with -infinity and keys above zero all of a row's scores are that."""
+    b = Batch(STEPS[step], G, D, "int8", seed=3)
+    b.fill()
+    b.k.codes[..., 7] = 5
+    q = torch.tensor(b.rng.normal(size=(b.T, H, D))).to(DT[dtype]).cuda()
+    hit = torch.zeros(b.T, H, dtype=torch.bool, device="cuda")
+    hit[::3, 1] = hit[1, 2] = True
+    outs = []
+    for x in (q, torch.where(hit[..., None] & (torch.arange(D, device="cuda") == 7), bad, q)):
+        out = torch.full((b.T, H * D), 7.0, dtype=DT[dtype], device="cuda")
+        K().attention8(x.view(b.T, -1), out, b.k, b.v, b.ctx, b.table, H, G, D, D ** -0.5, kernel=kernel)
+        K().check_device_errors("cuda:0")
+        outs.append(out.view(b.T, H, D))
+    assert bool(outs[1][hit].isnan().all())
+    off = (outs[1][~hit].double() - outs[0][~hit].double()).abs()
+    # (the other rows' maxima may move on other pages: two roundings of the output)
+    assert bool((off <= 2.0 ** -7 * outs[0][~hit].double().abs() + 2.0 ** -9).all())
